@@ -224,6 +224,56 @@ int ozk_certificate(const double* A, const double* B, int m, int n, int k, const
 int ozk_rule_certified(const double* nA, const double* nB, const int32_t* flag, int m, int n, int k,
                        const double* xmin, int32_t* dec, int32_t* p_dev, double* aux, ozk_stream_t stream);
 
+/* ---- microscaled (MX) products ---------------------------------------------------------------------------- *
+ * Products of low-bit operands with shared power-of-two scales, beside the exact INT8 residue products above.  A
+ * number is code x 2^(s - 127): an element of 4 bits (e2m1) or 8 bits (e4m3) and one scale byte s (e8m0; 255 = NaN)
+ * for each block of 32 along the contracted axis.  An operand is `groups` x `rows` vectors of length k, laid out for
+ * the tensor cores (ozk_mx_code_bytes / ozk_mx_scale_bytes; both buffers 16-byte aligned, codes 32-byte):
+ *   codes:  [group][row][kp], kp = k rounded up to 128, zero from k to kp; e2m1 holds two codes a byte, the even one
+ *           in the lower half;
+ *   scales: [group][ceil(rows / 128)][kp / 128][512]; row r and block b of a 128 x 128 tile at 16 (r % 32) +
+ *           4 (r / 32) + b.
+ * No shape rule: any rows, k >= 1.  dtype: OZK_F32, OZK_F16 or OZK_BF16.                                      */
+#define OZK_MX_E2M1 0
+#define OZK_MX_E4M3 1
+#define OZK_F32 0
+#define OZK_F16 1
+#define OZK_BF16 2
+#define OZK_MX_KMAX (1 << 28)     /* longest contracted axis               */
+#define OZK_MX_MAX_GROUPS 1024    /* most experts of one grouped product   */
+/* bytes of an operand's codes and scales; 0 for an invalid format or size */
+size_t ozk_mx_code_bytes(int fmt, int groups, int rows, int k);
+size_t ozk_mx_scale_bytes(int groups, int rows, int k);
+/* Element (g, r, l) of x sits at x[g group_stride + r row_stride + l k_stride] (strides in elements, >= 0).  Scale of
+ * a block: floor(log2 max|x|) - emax + 127 (emax 2 / 8), clamped at 0; with round_up one more where the largest value
+ * would saturate.  Codes: x 2^(127 - s) to the nearest element (ties to even), saturating at 6 / 448.  A block with an
+ * infinite or NaN value gets the scale 255.                                                                  */
+int ozk_mx_quantize(const void* x, int dtype, int groups, int rows, int k, int64_t group_stride, int64_t row_stride,
+                    int64_t k_stride, int fmt, int round_up, uint8_t* codes, uint8_t* scales, ozk_stream_t stream);
+/* out[g][r][l] (contiguous, 16-byte aligned) = code 2^(s - 127), computed in FP32, rounded to dtype           */
+int ozk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int fmt, int groups, int rows, int k, void* out,
+                      int dtype, ozk_stream_t stream);
+/* C[i][j] = sum_l A[i][l] B[j][l] for i < m, j < n, summed in FP32 on the tensor cores (tcgen05.mma block_scale, the
+ * scales in TMEM) and rounded once to dtype; any pair of formats.  C: row stride ldc elements.  err: device int32,
+ * OR'ed OZK_DEVERR_TIMEOUT_* flags of the bounded waits.                                                     */
+int ozk_mx_gemm(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
+                const uint8_t* B_scales, int B_fmt, int m, int n, int k, void* C, int64_t ldc, int dtype, int32_t* err,
+                ozk_stream_t stream);
+/* The product grouped by expert: rows [ends[g - 1], ends[g]) of A (from 0 for g = 0) are multiplied with group g of
+ * B (groups x n x k).  ends[groups]: device int32, ascending; a value below its predecessor or above `rows` is read as
+ * the nearest one in order.  Rows from the last end on are set to zero when `fill` is non-zero and left alone
+ * otherwise.  groups <= OZK_MX_MAX_GROUPS.                                                                   */
+int ozk_mx_grouped_gemm(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
+                        const uint8_t* B_scales, int B_fmt, int rows, int n, int k, int groups, const int32_t* ends,
+                        int fill, void* C, int64_t ldc, int dtype, int32_t* err, ozk_stream_t stream);
+/* Root-mean-square norm with an MX output: t = x + residual (residual may be NULL), y = t / sqrt(mean(t^2) + eps)
+ * weight over rows of d values, all in FP32; y quantised as ozk_mx_quantize does, into an operand of `rows` vectors of
+ * length d; t rounded to dtype into sum (rows x d, contiguous; may be NULL).  x, residual: contiguous rows, row strides
+ * in elements; weight[d] of dtype, or FP32 with weight_f32.                                                   */
+int ozk_mx_rms_norm(const void* x, const void* residual, const void* weight, int dtype, int weight_f32, int rows, int d,
+                    int64_t x_stride, int64_t residual_stride, float eps, int fmt, int round_up, void* sum,
+                    uint8_t* codes, uint8_t* scales, ozk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -18,6 +18,8 @@ _lib = None
 
 P = ctypes.c_void_p
 I32 = ctypes.c_int
+I64 = ctypes.c_int64
+F32 = ctypes.c_float
 F64 = ctypes.c_double
 SZ = ctypes.c_size_t
 
@@ -56,6 +58,13 @@ _SIGNATURES = {
     "ozk_gemm_i32": ([P, P, I32, I32, I32, P, P, P], I32),
     "ozk_wait_selftest": ([I32, ctypes.c_int64, P, P, P], I32),
     "ozk_reconstruct": ([P, P, P, P, I32, I32, I32, P, P, P], I32),
+    "ozk_mx_code_bytes": ([I32, I32, I32, I32], SZ),
+    "ozk_mx_scale_bytes": ([I32, I32, I32], SZ),
+    "ozk_mx_quantize": ([P, I32, I32, I32, I32, I64, I64, I64, I32, I32, P, P, P], I32),
+    "ozk_mx_dequantize": ([P, P, I32, I32, I32, I32, P, I32, P], I32),
+    "ozk_mx_gemm": ([P, P, I32, P, P, I32, I32, I32, I32, P, I64, I32, P, P], I32),
+    "ozk_mx_grouped_gemm": ([P, P, I32, P, P, I32, I32, I32, I32, I32, P, I32, P, I64, I32, P, P], I32),
+    "ozk_mx_rms_norm": ([P, P, P, I32, I32, I32, I32, I64, I64, F32, I32, I32, P, P, P, P], I32),
     "ozk_core": ([P, P, P, P, P, P, I32, I32, I32, I32, I32, P, P, P, P, P, P], I32),
 }
 

@@ -18,8 +18,9 @@ OUT_DIR = os.path.join(PKG, "lib")
 OBJ_DIR = os.path.join(ROOT, "_build", "ozaki_b200")
 LIB = os.path.join(OUT_DIR, "libozaki_b200.so")
 
-SOURCES = ["capi.cu", "stats.cu", "rule.cu", "split.cu", "split_tc.cu", "gemm_tc.cu", "recon.cu", "certificate.cu", "chain.cu"]
-HEADERS = ["ozk_common.cuh", "tc_ptx.cuh"]
+SOURCES = ["capi.cu", "stats.cu", "rule.cu", "split.cu", "split_tc.cu", "gemm_tc.cu", "recon.cu", "certificate.cu", "chain.cu",
+           "mx.cu", "mx_gemm.cu"]
+HEADERS = ["ozk_common.cuh", "tc_ptx.cuh", "mx_common.cuh"]
 
 
 def nvcc() -> str:

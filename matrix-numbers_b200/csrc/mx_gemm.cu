@@ -1,0 +1,703 @@
+// Products of microscaled (MX) operands on the 5th-generation tensor cores, plain and grouped by expert:
+//   C[i][j] = sum_l A[i][l] B[j][l],   A[i][l] = a 2^(sa - 127), B[j][l] = b 2^(sb - 127), scales shared by 32 l's.
+// tcgen05.mma multiplies the codes, applies both scales to each block's partial sum and accumulates in FP32 in TMEM, so
+// nothing is unpacked on the way: kind::mxf4 for two 4-bit operands (K = 64 an instruction), kind::mxf8f6f4 otherwise
+// (K = 32; a 4-bit operand is spread to one code a byte by its TMA load).
+//
+// One persistent kernel, one CTA per SM:
+//   - warp 0 (one lane): producer; a stage is 128 bytes of K of 128 "left" rows (M) and BN "right" rows (N) by TMA with
+//     the 128-byte swizzle, and their scale tiles by contiguous bulk copies;
+//   - warp 1 (one lane): lays a stage's scales into TMEM (tcgen05.cp, in order with the MMAs that use them, two buffers
+//     of columns) and issues the four MMAs of the stage;
+//   - warps 2..9: epilogue, TMEM -> registers -> one rounding -> C.
+// Left is A and right is B (`SWAP` false), or, for few rows of A, left is B and right is A: the 128 rows that the
+// instruction has at least are then rows of B, which there are plenty of, and A's tile is as small as 32 rows; C^T comes
+// out of TMEM, whose lanes are then neighbours in a row of C.
+// Where there are fewer tiles than SMs, a cluster of CTAs shares one tile: each takes a part of K, leaves its FP32 sums
+// in its shared memory, and every CTA adds one slice of the tile over the cluster in a fixed order (no workspace, no
+// atomics, one launch).
+// Grouped: `ends` is read on the device; a group's rows are covered by the windows of A (of 128 or BN rows, at multiples
+// of that) that they touch, and each window is multiplied with the group's B and stored for the group's rows only.
+// Windows at fixed places keep A's rows where the quantisation put them, whatever the routing, for at most one more
+// tile per group than packing would need.
+// Every mbarrier wait is bounded; on a timeout the CTA records a flag in *err, stops, waits (bounded) for its own copies
+// and MMAs in flight, frees TMEM and exits.  No multicast is used.
+#include <cuda.h>
+
+#include <atomic>
+
+#include "mx_common.cuh"
+#include "tc_ptx.cuh"
+
+using namespace ozk_mx;
+using namespace ozk_ptx;
+
+namespace {
+
+constexpr int BM = 128;                      // rows of the left operand's tile
+constexpr int ROW_BYTES = 128;               // K bytes of one stage row (shared memory)
+constexpr int EPI_WARPS = 8;
+constexpr int THREADS = (2 + EPI_WARPS) * 32;
+constexpr int GROUP_L = 16;                  // left tiles per raster group
+constexpr uint64_t WAIT_LIMIT_NS = 4000000000ull;   // 4 s of wall time per wait
+constexpr int MXF4 = 0, MXF8F6F4 = 1;
+constexpr size_t SMEM_MAX = 232448;
+constexpr size_t TABLE_BYTES = (2 * (OZK_MX_MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
+
+template <int KIND, int BN>
+struct Shape {
+    static constexpr int KT = KIND == MXF4 ? 2 : 1;             // scale tiles (128 elements of K) of a stage
+    static constexpr int SUBS = (BN + TILE - 1) / TILE;         // row tiles of the right operand's scales
+    static constexpr uint32_t L_BYTES = BM * ROW_BYTES, R_BYTES = BN * ROW_BYTES;
+    static constexpr uint32_t SL_BYTES = KT * TILE_BYTES, SR_BYTES = SUBS * KT * TILE_BYTES;
+    static constexpr uint32_t STAGE_BYTES = L_BYTES + R_BYTES + SL_BYTES + SR_BYTES;
+    static constexpr int FIT = (int)((SMEM_MAX - 1024 - 256 - TABLE_BYTES) / STAGE_BYTES);
+    static constexpr int STAGES = FIT < 8 ? FIT : 8;
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + 1024 + 256 + TABLE_BYTES;
+    static constexpr int NUM_BARS = 2 * STAGES + 5;             // full[S], empty[S], acc_full[2], acc_empty[2], drain
+    // TMEM: two accumulators, then two buffers of scale columns.  With BN = 256 the accumulators overlap by 48 columns,
+    // which makes room for the scales: the epilogue reads the shared columns first, and the next tile waits for those.
+    static constexpr int SCALE_COLS = KT * 4 * (1 + SUBS);
+    static constexpr int ACC_STRIDE = BN == 256 ? 208 : BN;
+    static constexpr int SCALE_BASE = ACC_STRIDE + BN;
+    static constexpr int USED = SCALE_BASE + 2 * SCALE_COLS;
+    static constexpr uint32_t TMEM_COLS = USED <= 128 ? 128 : USED <= 256 ? 256 : 512;
+    static constexpr int LAG = BN == 256 ? 1 : 2;               // tiles between an accumulator's drain and its next use
+    static constexpr int HALF = BN / 2;                         // accumulator columns of one epilogue warp
+    static constexpr int CHUNK = HALF < 32 ? HALF : 32;
+    static_assert(USED <= 512 && NUM_BARS * 8 + 16 <= 256 && STAGES >= 3, "fits");
+    static_assert((size_t)BN * BM * 4 <= (size_t)STAGES * STAGE_BYTES, "a tile of partial sums fits into the stages");
+};
+
+struct Args {
+    const uint8_t *sl, *sr;                  // scales of the left and right operand
+    long long sl_group, sr_group;            // bytes of one group of them
+    int l_rows, r_rows;                      // rows (per group) of the left and right operand
+    int ktiles;                              // scale tiles along K
+    int kblocks;                             // stages along K
+    uint32_t load_bytes;                     // what the two TMA loads of a stage count on its barrier
+    int groups;                              // 0: no groups
+    const int32_t* ends;
+    int tokens, n;                           // rows and columns of C
+    int fill;
+    void* C;
+    long long ldc;
+    int dtype;
+    bool vec;                                // rows of C are 16-byte aligned
+    uint32_t idesc;
+    int32_t* err;
+};
+
+struct Unit {
+    int lt, rt;                              // tile indices
+    int lg, rg;                              // group coordinates
+    int first, last;                         // rows of A (and C) that belong to this unit's group: [first, last)
+};
+
+template <int BN, bool SWAP>
+struct Work {
+    const Args& a;
+    const int *pre, *bound;                  // grouped: windows before group g, first row of group g
+    int ltiles, rtiles;
+    long long units;
+
+    __device__ Work(const Args& a_, const int* pre_, const int* bound_) : a(a_), pre(pre_), bound(bound_) {
+        ltiles = (a.l_rows + BM - 1) / BM;
+        rtiles = (a.r_rows + BN - 1) / BN;
+        units = a.groups ? (long long)pre[a.groups] * (SWAP ? ltiles : rtiles) : (long long)ltiles * rtiles;
+    }
+    __device__ __forceinline__ Unit at(long long u) const {
+        Unit w;
+        if (a.groups) {
+            const int other = SWAP ? ltiles : rtiles;
+            const int q = (int)(u / other);
+            int lo = 0, hi = a.groups - 1;                  // the last group with pre[g] <= q: it has windows
+            while (lo < hi) {
+                const int mid = (lo + hi + 1) >> 1;
+                if (pre[mid] <= q) lo = mid; else hi = mid - 1;
+            }
+            w.first = bound[lo];
+            w.last = bound[lo + 1];
+            const long long in = u - (long long)pre[lo] * other;
+            const int nw = pre[lo + 1] - pre[lo];
+            const int win = w.first / (SWAP ? BN : BM) + (int)(in % nw), o = (int)(in / nw);
+            w.lt = SWAP ? o : win;
+            w.rt = SWAP ? win : o;
+            w.lg = SWAP ? lo : 0;
+            w.rg = SWAP ? 0 : lo;
+        } else {
+            const int per = GROUP_L * rtiles;
+            const int g = (int)(u / per), l0 = g * GROUP_L, gl = min(ltiles - l0, GROUP_L);
+            const int in = (int)(u - (long long)g * per);
+            w.lt = l0 + in % gl;
+            w.rt = in / gl;
+            w.lg = w.rg = 0;
+            w.first = 0;
+            w.last = a.tokens;
+        }
+        return w;
+    }
+};
+
+__device__ __forceinline__ void raise_abort(volatile int* abort_flag, int32_t* err, int code) {
+    *abort_flag = 1;
+    atomicOr(err, code);
+}
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
+    if (dtype == OZK_BF16) {
+        const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    }
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void store1(void* C, long long at, float v, int dtype) {
+    if (dtype == OZK_F32) static_cast<float*>(C)[at] = v;
+    else if (dtype == OZK_BF16) static_cast<__nv_bfloat16*>(C)[at] = __float2bfloat16_rn(v);
+    else static_cast<__half*>(C)[at] = __float2half_rn(v);
+}
+
+// One thread's CHUNK consecutive accumulator columns (`r` the first one's right row, `l` the lane's left row) to C
+template <int CHUNK, bool SWAP>
+__device__ __forceinline__ void store_chunk(const Args& a, const Unit& w, int l, int r, const uint32_t (&v)[CHUNK]) {
+    if (SWAP) {                              // l: column of C, r: row of C; the warp's lanes are neighbours in a row
+        if (l >= a.n) return;
+#pragma unroll
+        for (int e = 0; e < CHUNK; e++)
+            if (r + e >= w.first && r + e < w.last)
+                store1(a.C, (long long)(r + e) * a.ldc + l, __uint_as_float(v[e]), a.dtype);
+        return;
+    }
+    if (l < w.first || l >= w.last || r >= a.n) return;
+    const long long at = (long long)l * a.ldc + r;
+    if (a.vec && r + CHUNK <= a.n) {
+        if (a.dtype == OZK_F32) {
+            uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(a.C) + at);
+#pragma unroll
+            for (int q = 0; q < CHUNK / 4; q++) d[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        } else {
+            uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.C) + at);
+#pragma unroll
+            for (int q = 0; q < CHUNK / 8; q++) {
+                uint32_t p[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    p[j] = pack2(__uint_as_float(v[8 * q + 2 * j]), __uint_as_float(v[8 * q + 2 * j + 1]), a.dtype);
+                d[q] = make_uint4(p[0], p[1], p[2], p[3]);
+            }
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < CHUNK; e++)
+            if (r + e < a.n) store1(a.C, at + e, __uint_as_float(v[e]), a.dtype);
+    }
+}
+
+// Grouped: clamp `ends` to an ascending sequence within [0, rows] and count the windows each group touches (one warp)
+template <int WIN>
+__device__ __forceinline__ void group_tables(const Args& a, int* pre, int* bound, int lane) {
+    int end_before = 0, windows_before = 0;
+    if (lane == 0) { pre[0] = 0; bound[0] = 0; }
+    for (int base = 0; base < a.groups; base += 32) {
+        const int g = base + lane;
+        int e = g < a.groups ? min(max(a.ends[g], 0), a.tokens) : 0;
+        e = max(e, end_before);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, e, o);
+            if (lane >= o) e = max(e, p);
+        }
+        int s = __shfl_up_sync(0xffffffffu, e, 1);
+        if (lane == 0) s = end_before;
+        int w = e > s ? (e - 1) / WIN - s / WIN + 1 : 0;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int p = __shfl_up_sync(0xffffffffu, w, o);
+            if (lane >= o) w += p;
+        }
+        w += windows_before;
+        if (g < a.groups) { pre[g + 1] = w; bound[g + 1] = e; }
+        end_before = __shfl_sync(0xffffffffu, e, 31);
+        windows_before = __shfl_sync(0xffffffffu, w, 31);
+    }
+}
+
+template <int CHUNK>
+__device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, uint32_t (&v)[CHUNK]) {
+    if constexpr (CHUNK == 32) tmem_ld_32x32b_x32(taddr, v);
+    else tmem_ld_32x32b_x16(taddr, v);
+}
+
+template <int KIND, int BN, bool SWAP>
+__global__ void __launch_bounds__(THREADS, 1)
+    mx_gemm_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmR,
+                   const __grid_constant__ Args a, int parts) {
+    using S = Shape<KIND, BN>;
+    constexpr int STAGES = S::STAGES, CHUNK = S::CHUNK;
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint8_t* sL = smem;
+    uint8_t* sR = sL + STAGES * S::L_BYTES;
+    uint8_t* sSL = sR + STAGES * S::R_BYTES;
+    uint8_t* sSR = sSL + STAGES * S::SL_BYTES;
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * S::STAGE_BYTES);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::NUM_BARS);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    int* pre = reinterpret_cast<int*>(smem + STAGES * S::STAGE_BYTES + 256);
+    int* bound = pre + OZK_MX_MAX_GROUPS + 1;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t bar0 = smem_addr(bars);
+    auto full_bar = [&](int s) { return bar0 + 8u * (uint32_t)s; };
+    auto empty_bar = [&](int s) { return bar0 + 8u * (uint32_t)(STAGES + s); };
+    auto accf_bar = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + b); };
+    auto acce_bar = [&](int b) { return bar0 + 8u * (uint32_t)(2 * STAGES + 2 + b); };
+    const uint32_t drain_bar = bar0 + 8u * (uint32_t)(2 * STAGES + 4);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < STAGES; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
+        for (int b = 0; b < 2; b++) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), EPI_WARPS); }
+        mbar_init(drain_bar, 1);
+        *abort_flag = 0;
+        mbar_fence_init();
+        tma_prefetch_desc(&tmL);
+        tma_prefetch_desc(&tmR);
+    }
+    if (warp == 1) {
+        tmem_alloc(smem_addr(tmem_slot), S::TMEM_COLS);
+        tmem_relinquish();
+    }
+    if (warp == 2 && a.groups) group_tables<SWAP ? BN : BM>(a, pre, bound, lane);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem_base = *tmem_slot;
+
+    const Work<BN, SWAP> work(a, pre, bound);
+    // parts > 1: one unit per cluster of `parts` CTAs, each with its part of K; else units round robin over the grid
+    const int part = parts > 1 ? (int)cluster_ctarank() : 0;
+    const long long u0 = blockIdx.x / parts, du = gridDim.x / parts;
+    const int kb0 = (int)((long long)a.kblocks * part / parts), kb1 = (int)((long long)a.kblocks * (part + 1) / parts);
+
+    if (warp == 0) {
+        if (lane == 0) {
+            // ------------------------------------------------------------ producer
+            int stage = 0;
+            uint32_t phase = 0;
+            long long issued = 0;
+            bool ok = true;
+            for (long long u = u0; ok && u < work.units; u += du) {
+                const Unit w = work.at(u);
+                const int r_tile = w.rt * BN / TILE;
+                const int subs = min(S::SUBS, row_tiles(a.r_rows) - r_tile);
+                const uint8_t* gl = a.sl + w.lg * a.sl_group + (long long)w.lt * a.ktiles * TILE_BYTES;
+                const uint8_t* gr = a.sr + w.rg * a.sr_group + (long long)r_tile * a.ktiles * TILE_BYTES;
+                for (int kb = kb0; kb < kb1; kb++) {
+                    if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
+                        if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_PRODUCER);
+                        ok = false;
+                        break;
+                    }
+                    const uint32_t sb = (uint32_t)min(S::KT, a.ktiles - kb * S::KT) * TILE_BYTES;
+                    const uint32_t bar = full_bar(stage);
+                    mbar_arrive_expect_tx(bar, a.load_bytes + sb * (uint32_t)(1 + subs));
+                    const int kc = kb * (KIND == MXF4 ? ROW_BYTES : TILE);      // bytes (mxf4) or elements
+                    tma_load_3d(smem_addr(sL + stage * S::L_BYTES), &tmL, kc, w.lt * BM, w.lg, bar);
+                    tma_load_3d(smem_addr(sR + stage * S::R_BYTES), &tmR, kc, w.rt * BN, w.rg, bar);
+                    const long long so = (long long)kb * S::KT * TILE_BYTES;
+                    bulk_load(smem_addr(sSL + stage * S::SL_BYTES), gl + so, sb, bar);
+                    for (int i = 0; i < subs; i++)
+                        bulk_load(smem_addr(sSR + stage * S::SR_BYTES + i * S::SL_BYTES),
+                                  gr + (long long)i * a.ktiles * TILE_BYTES + so, sb, bar);
+                    issued++;
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+            }
+            if (!ok) {
+                // let the loads already issued land before the CTA exits (bounded)
+                const long long first = issued > STAGES ? issued - STAGES : 0;
+                for (long long j = first; j < issued; j++) {
+                    int dummy = 0;
+                    mbar_wait_bounded(full_bar((int)(j % STAGES)), (uint32_t)((j / STAGES) & 1), &dummy, WAIT_LIMIT_NS);
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0) {
+            // ------------------------------------------------------------ scales to TMEM, MMAs
+            int stage = 0;
+            uint32_t phase = 0, it = 0, step = 0;
+            bool ok = true, issued_any = false;
+            for (long long u = u0; ok && u < work.units; u += du) {
+                const Unit w = work.at(u);
+                const int b = (int)(it & 1u);
+                if (it >= (uint32_t)S::LAG) {
+                    const uint32_t bar = S::LAG == 1 ? acce_bar(0) : acce_bar(b);
+                    const uint32_t par = S::LAG == 1 ? (it - 1u) & 1u : ((it >> 1) - 1u) & 1u;
+                    if (!mbar_wait_bounded(bar, par, abort_flag, WAIT_LIMIT_NS)) {
+                        if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_MMA);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                }
+                const uint32_t d_tmem = tmem_base + (uint32_t)(b * S::ACC_STRIDE);
+                // the second tile of 64 right rows in a scale tile starts two columns on (32 rows a column; an MMA takes
+                // its scales from an even column, so tiles of 32 rows exist for a first tile only)
+                const uint32_t r_col = BN == 64 ? (uint32_t)(w.rt & 1) * 2u : 0u;
+                for (int kb = kb0; kb < kb1; kb++) {
+                    if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
+                        if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_MMA);
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const int tiles = min(S::KT, a.ktiles - kb * S::KT);
+                    const uint32_t tl = tmem_base + (uint32_t)(S::SCALE_BASE + (int)(step & 1u) * S::SCALE_COLS);
+                    const uint32_t tr = tl + (uint32_t)(4 * S::KT);
+                    for (int t = 0; t < tiles; t++) {
+                        tmem_cp_scales(tl + 4u * t, smem_desc_scales(smem_addr(sSL + stage * S::SL_BYTES + t * TILE_BYTES)));
+#pragma unroll
+                        for (int i = 0; i < S::SUBS; i++)
+                            tmem_cp_scales(tr + 4u * (uint32_t)(t * S::SUBS + i),
+                                           smem_desc_scales(smem_addr(sSR + stage * S::SR_BYTES + i * S::SL_BYTES + t * TILE_BYTES)));
+                    }
+                    const uint64_t ld = umma_desc_sw128(smem_addr(sL + stage * S::L_BYTES));
+                    const uint64_t rd = umma_desc_sw128(smem_addr(sR + stage * S::R_BYTES));
+                    // four instructions of 32 bytes along K inside the swizzle atom (+2 in the >> 4 address field)
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) {
+                        const int t = KIND == MXF4 ? kk >> 1 : 0;
+                        if (t >= tiles) break;
+                        const uint32_t id = KIND == MXF4 ? 2u * (kk & 1) : (uint32_t)kk;
+                        const uint32_t idesc = a.idesc | umma_idesc_scale_id(id);
+                        const uint32_t acc = (kb > kb0 || kk > 0) ? 1u : 0u;
+                        const uint32_t ca = tl + 4u * t, cb = tr + 4u * (uint32_t)(t * S::SUBS) + r_col;
+                        if (KIND == MXF4) umma_mxf4(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
+                        else umma_mxf8f6f4(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
+                    }
+                    issued_any = true;
+                    step++;
+                    umma_commit(empty_bar(stage));
+                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+                }
+                if (!ok) break;
+                umma_commit(accf_bar(b));
+                it++;
+            }
+            if (!ok && issued_any) {
+                // all MMAs issued by this thread must finish before TMEM is released
+                umma_commit(drain_bar);
+                int dummy = 0;
+                mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
+            }
+        }
+    } else {
+        // ---------------------------------------------------------------- epilogue warps
+        const int ew = warp - 2;
+        const int quarter = warp & 3;          // TMEM lanes this warp may access: [32 quarter, 32 quarter + 32)
+        const int half = ew >> 2;              // column half of the accumulator
+        constexpr int NCH = S::HALF / CHUNK;
+        uint32_t it = 0;
+        bool ok = true;
+        for (long long u = u0; ok && u < work.units; u += du) {
+            const Unit w = work.at(u);
+            const int b = (int)(it & 1u);
+            if (!mbar_wait_bounded(accf_bar(b), (it >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
+                if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_EPILOGUE);
+                ok = false;
+                break;
+            }
+            __syncwarp();
+            tc_fence_after();
+            const int l = w.lt * BM + quarter * 32 + lane;
+            const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * S::ACC_STRIDE + half * S::HALF);
+            const int r = w.rt * BN + half * S::HALF;
+            if (parts > 1) {
+                float* mine = reinterpret_cast<float*>(smem);
+#pragma unroll 1
+                for (int c = 0; c < NCH; c++) {
+                    uint32_t v[CHUNK];
+                    tmem_ld_chunk<CHUNK>(acc + (uint32_t)(c * CHUNK), v);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < CHUNK; e++)
+                        mine[(half * S::HALF + c * CHUNK + e) * BM + quarter * 32 + lane] = __uint_as_float(v[e]);
+                }
+            } else if (S::LAG == 1) {
+                // the columns shared with the other accumulator: the last 48 of buffer 0, the first 48 of buffer 1
+                const bool shared_half = half == 1 - b;
+                const int c0 = b == 0 ? NCH - 1 : 0, dc = b == 0 ? -1 : 1;
+                uint32_t v0[CHUNK], v1[CHUNK];
+                if (!shared_half) {
+                    if (lane == 0) mbar_arrive(acce_bar(0));
+                }
+#pragma unroll 1
+                for (int c = 0; c < NCH; c += 2) {
+                    const int ca = c0 + dc * c, cb = c0 + dc * (c + 1);
+                    tmem_ld_chunk<CHUNK>(acc + (uint32_t)(ca * CHUNK), v0);
+                    tmem_ld_chunk<CHUNK>(acc + (uint32_t)(cb * CHUNK), v1);
+                    tmem_wait_ld();
+                    if (c == 0 && shared_half) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acce_bar(0));
+                    }
+                    store_chunk<CHUNK, SWAP>(a, w, l, r + ca * CHUNK, v0);
+                    store_chunk<CHUNK, SWAP>(a, w, l, r + cb * CHUNK, v1);
+                }
+                tc_fence_before();
+                __syncwarp();
+            } else {
+#pragma unroll 1
+                for (int c = 0; c < NCH; c++) {
+                    uint32_t v[CHUNK];
+                    tmem_ld_chunk<CHUNK>(acc + (uint32_t)(c * CHUNK), v);
+                    tmem_wait_ld();
+                    if (c == NCH - 1) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(acce_bar(b));
+                    }
+                    store_chunk<CHUNK, SWAP>(a, w, l, r + c * CHUNK, v);
+                }
+            }
+            it++;
+        }
+        // rows of C behind the last group
+        if (a.groups && a.fill) {
+            const int size = a.dtype == OZK_F32 ? 4 : 2;
+            const long long bytes = (long long)a.n * size;
+            for (long long row = (long long)bound[a.groups] + blockIdx.x; row < a.tokens; row += gridDim.x) {
+                uint8_t* p = static_cast<uint8_t*>(a.C) + row * a.ldc * size;
+                const long long vecs = a.vec ? bytes / 16 : 0;
+                for (long long i = threadIdx.x - 64; i < vecs; i += EPI_WARPS * 32)
+                    reinterpret_cast<uint4*>(p)[i] = make_uint4(0u, 0u, 0u, 0u);
+                for (long long i = vecs * 8 * 2 / size + threadIdx.x - 64; i < a.n; i += EPI_WARPS * 32)
+                    store1(p, i, 0.0f, a.dtype);
+            }
+        }
+    }
+
+    if (parts > 1) {
+        // add one slice of the tile's columns over the cluster, CTA 0's sums first
+        __syncwarp();
+        cluster_sync();
+        if (warp >= 2 && u0 < work.units && !*abort_flag) {
+            const Unit w = work.at(u0);
+            const int row = (threadIdx.x - 64) & (BM - 1);
+            const int c0 = BN * part / parts, c1 = BN * (part + 1) / parts;
+            const uint32_t base = smem_addr(smem) + 4u * (uint32_t)row;
+            for (int c = c0 + ((threadIdx.x - 64) >> 7); c < c1; c += EPI_WARPS * 32 / BM) {
+                float sum = 0.0f;
+                for (int q = 0; q < parts; q++)
+                    sum += ld_cluster_f32(map_to_rank(base + 4u * (uint32_t)(c * BM), (uint32_t)q));
+                const int l = w.lt * BM + row, r = w.rt * BN + c;
+                const int token = SWAP ? r : l, col = SWAP ? l : r;
+                if (token >= w.first && token < w.last && col < a.n)
+                    store1(a.C, (long long)token * a.ldc + col, sum, a.dtype);
+            }
+        }
+        __syncwarp();
+        cluster_sync();                        // no CTA leaves while another reads its sums
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 1) {
+        __syncwarp();
+        tmem_dealloc(tmem_base, S::TMEM_COLS);
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiledFn find_encode_fn() {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+        return reinterpret_cast<EncodeTiledFn>(p);
+    return nullptr;
+}
+
+struct Operand {
+    const uint8_t *codes, *scales;
+    int fmt, groups, rows;
+};
+
+bool spreads(const Operand& o, int kind) { return kind == MXF8F6F4 && o.fmt == OZK_MX_E2M1; }
+
+// codes [groups][rows][kp], box of 128 bytes of K (after the spreading of 4-bit codes, where `spread`) x box_rows rows,
+// 128-byte swizzle; rows past the end are zero
+int make_map(CUtensorMap* map, const Operand& o, int k, int box_rows, int kind) {
+    static const EncodeTiledFn fn = find_encode_fn();
+    if (!fn) return OZK_ERR_DRIVER;
+    const bool spread = spreads(o, kind);
+    const cuuint64_t pitch = (cuuint64_t)code_pitch(o.fmt, k);
+    const cuuint64_t dims[3] = {spread ? (cuuint64_t)padded_k(k) : pitch, (cuuint64_t)o.rows, (cuuint64_t)o.groups};
+    const cuuint64_t strides[2] = {pitch, pitch * (cuuint64_t)o.rows};
+    const cuuint32_t box[3] = {(cuuint32_t)ROW_BYTES, (cuuint32_t)box_rows, 1u};
+    const cuuint32_t estr[3] = {1u, 1u, 1u};
+    const CUresult r = fn(map, spread ? CU_TENSOR_MAP_DATA_TYPE_16U4_ALIGN16B : CU_TENSOR_MAP_DATA_TYPE_UINT8, 3,
+                          const_cast<uint8_t*>(o.codes), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? OZK_OK : OZK_ERR_DRIVER;
+}
+
+// SM count of the current device, 0 when it is not a B200
+int sm_count(int* dev_out) {
+    static std::atomic<int> known[64];
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+    int sms = known[dev].load(std::memory_order_relaxed);
+    if (sms == 0) {
+        int major = 0;
+        if (cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev) != cudaSuccess || major != 10) return 0;
+        if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+        known[dev].store(sms, std::memory_order_relaxed);
+    }
+    *dev_out = dev;
+    return sms;
+}
+
+struct Call {
+    Operand A, B;
+    int n, k, kind;
+    Args args;
+    cudaStream_t st;
+    int dev, sms;
+};
+
+uint32_t format_bits(int kind, int fmt) { return kind == MXF4 ? 1u : fmt == OZK_MX_E2M1 ? 5u : 0u; }
+
+template <int KIND, int BN, bool SWAP>
+int launch(const Call& c, int parts) {
+    using S = Shape<KIND, BN>;
+    auto kern = mx_gemm_kernel<KIND, BN, SWAP>;
+    static std::atomic<bool> ready[64];
+    if (!ready[c.dev].load(std::memory_order_acquire)) {
+        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
+        ready[c.dev].store(true, std::memory_order_release);
+    }
+    const Operand &L = SWAP ? c.B : c.A, &R = SWAP ? c.A : c.B;
+    Args a = c.args;
+    a.sl = L.scales;
+    a.sr = R.scales;
+    a.sl_group = scale_group_bytes(L.rows, c.k);
+    a.sr_group = scale_group_bytes(R.rows, c.k);
+    a.l_rows = L.rows;
+    a.r_rows = R.rows;
+    a.ktiles = padded_k(c.k) / TILE;
+    a.kblocks = (a.ktiles + S::KT - 1) / S::KT;
+    // a load that spreads 4-bit codes counts the bytes it reads, not the bytes it fills
+    a.load_bytes = S::L_BYTES / (spreads(L, KIND) ? 2u : 1u) + S::R_BYTES / (spreads(R, KIND) ? 2u : 1u);
+    a.idesc = umma_idesc_mx(format_bits(KIND, L.fmt), format_bits(KIND, R.fmt), BM, BN);
+    CUtensorMap tl, tr;
+    int rc;
+    if ((rc = make_map(&tl, L, c.k, BM, KIND)) != OZK_OK) return rc;
+    if ((rc = make_map(&tr, R, c.k, BN, KIND)) != OZK_OK) return rc;
+    const long long lt = (L.rows + BM - 1) / BM, rt = (R.rows + BN - 1) / BN;
+    if (lt * rt > 0x7fffffffLL || (BN == 32 && rt > 1)) return OZK_ERR_ARG;
+    // grouped: the number of tiles is known on the device only
+    const long long units = a.groups ? c.sms : lt * rt;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute cluster[1];
+    cluster[0].id = cudaLaunchAttributeClusterDimension;
+    cluster[0].val.clusterDim.x = (unsigned)parts;
+    cluster[0].val.clusterDim.y = 1;
+    cluster[0].val.clusterDim.z = 1;
+    cfg.blockDim = dim3(THREADS, 1, 1);
+    cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = c.st;
+    cfg.attrs = cluster;
+    cfg.numAttrs = parts > 1 ? 1 : 0;
+    cfg.gridDim = dim3((unsigned)(parts > 1 ? units * parts : units < c.sms ? units : c.sms), 1, 1);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tl, tr, a, parts);
+    if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
+    OZK_CHECK_LAUNCH();
+    return OZK_OK;
+}
+
+// CTAs that share one tile along K: as many as keep the grid within the SMs and leave each at least two stages
+int parts_for(long long units, int kblocks, int sms) {
+    int p = 1;
+    while (p < 8 && units * p * 2 <= sms && kblocks >= 4 * p) p *= 2;
+    return p;
+}
+
+template <int KIND>
+int choose(const Call& c) {
+    const int kblocks = (padded_k(c.k) / TILE + (KIND == MXF4 ? 1 : 0)) / (KIND == MXF4 ? 2 : 1);
+    if (c.args.groups) {
+        const int per = c.args.tokens / c.args.groups;            // rows of an average group
+        if (per <= 64) return launch<KIND, 64, true>(c, 1);
+        if (per <= 128) return launch<KIND, 128, true>(c, 1);
+        return launch<KIND, 256, false>(c, 1);
+    }
+    const long long m = c.A.rows, nt = (c.n + BM - 1) / BM;
+    if (m <= 32) return launch<KIND, 32, true>(c, parts_for(nt, kblocks, c.sms));
+    if (m <= 64) return launch<KIND, 64, true>(c, parts_for(nt, kblocks, c.sms));
+    const long long wide = ((m + BM - 1) / BM) * ((c.n + 255) / 256);
+    if (wide * 2 > c.sms) return launch<KIND, 256, false>(c, 1);
+    return launch<KIND, 128, false>(c, parts_for(((m + BM - 1) / BM) * nt, kblocks, c.sms));
+}
+
+bool fmt_ok(int fmt) { return fmt == OZK_MX_E2M1 || fmt == OZK_MX_E4M3; }
+
+int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const uint8_t* Bs, int Bf, int m, int n, int k,
+        int groups, const int32_t* ends, int fill, void* C, int64_t ldc, int dtype, int32_t* err, ozk_stream_t stream) {
+    if (!Ac || !As || !Bc || !Bs || !C || !err || !fmt_ok(Af) || !fmt_ok(Bf)) return OZK_ERR_ARG;
+    if (m < 1 || n < 1 || k < 1 || k > OZK_MX_KMAX || ldc < n) return OZK_ERR_ARG;
+    if (dtype != OZK_F32 && dtype != OZK_F16 && dtype != OZK_BF16) return OZK_ERR_ARG;
+    const uintptr_t align = reinterpret_cast<uintptr_t>(Ac) | reinterpret_cast<uintptr_t>(Bc);
+    const uintptr_t align_s = reinterpret_cast<uintptr_t>(As) | reinterpret_cast<uintptr_t>(Bs);
+    const uintptr_t size = dtype == OZK_F32 ? 4 : 2;
+    if ((align & 31) || (align_s & 15) || (reinterpret_cast<uintptr_t>(C) & (size - 1))) return OZK_ERR_ARG;
+    Call c;
+    c.sms = sm_count(&c.dev);
+    if (c.sms == 0) return OZK_ERR_DEVICE;
+    c.A = {Ac, As, Af, 1, m};
+    c.B = {Bc, Bs, Bf, groups ? groups : 1, n};
+    c.n = n;
+    c.k = k;
+    c.kind = Af == OZK_MX_E2M1 && Bf == OZK_MX_E2M1 ? MXF4 : MXF8F6F4;
+    c.st = reinterpret_cast<cudaStream_t>(stream);
+    Args& a = c.args;
+    a = Args{};
+    a.groups = groups;
+    a.ends = ends;
+    a.tokens = m;
+    a.n = n;
+    a.fill = fill;
+    a.C = C;
+    a.ldc = ldc;
+    a.dtype = dtype;
+    a.vec = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && ldc * (int64_t)size % 16 == 0;
+    a.err = err;
+    return c.kind == MXF4 ? choose<MXF4>(c) : choose<MXF8F6F4>(c);
+}
+
+}  // namespace
+
+extern "C" int ozk_mx_gemm(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
+                           const uint8_t* B_scales, int B_fmt, int m, int n, int k, void* C, int64_t ldc, int dtype,
+                           int32_t* err, ozk_stream_t stream) {
+    return run(A_codes, A_scales, A_fmt, B_codes, B_scales, B_fmt, m, n, k, 0, nullptr, 0, C, ldc, dtype, err, stream);
+}
+
+extern "C" int ozk_mx_grouped_gemm(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
+                                   const uint8_t* B_scales, int B_fmt, int rows, int n, int k, int groups,
+                                   const int32_t* ends, int fill, void* C, int64_t ldc, int dtype, int32_t* err,
+                                   ozk_stream_t stream) {
+    if (!ends || (reinterpret_cast<uintptr_t>(ends) & 3) || groups < 1 || groups > OZK_MX_MAX_GROUPS) return OZK_ERR_ARG;
+    return run(A_codes, A_scales, A_fmt, B_codes, B_scales, B_fmt, rows, n, k, groups, ends, fill, C, ldc, dtype, err,
+               stream);
+}

@@ -171,6 +171,44 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
         "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(z), "r"(z), "r"(z), "r"(z)
         : "memory");
 }
+// D[tmem] (+)= (A * scale_A)[smem desc] * (B * scale_B)[smem desc]^T with one e8m0 scale per 32 elements of K, the scales
+// in TMEM: kind::mxf4 (e2m1 x e2m1, K = 64, two scales a row) and kind::mxf8f6f4 (8-bit containers, K = 32, one scale)
+__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                          uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+}
+__device__ __forceinline__ void umma_mxf8f6f4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t scale_a, uint32_t scale_b, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %6, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(scale_a), "r"(scale_b), "r"(accumulate)
+        : "memory");
+}
+// 32 rows of 16 bytes (512 contiguous bytes of shared memory) to four TMEM columns of all four lane quarters.  Runs in
+// issue order with the MMAs of the same thread.
+__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
+    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc) : "memory");
+}
+// `bytes` contiguous bytes (a multiple of 16, both addresses 16-byte aligned) into this CTA's shared memory
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(bar)
+                 : "memory");
+}
+// a 32-bit word of this location in the shared memory of CTA `rank` of the cluster (address from map_to_rank)
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // arrive once on `bar` when every tcgen05 operation issued so far by this thread has completed
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -262,6 +300,19 @@ __device__ __forceinline__ uint64_t umma_desc_sw128_mn(uint32_t saddr, uint32_t 
     d |= (uint64_t)2u << 61;
     return d;
 }
+
+// Shared-memory descriptor without swizzle for tmem_cp_scales: 8-row groups of 16-byte rows, 128 bytes apart.
+__device__ __forceinline__ uint64_t smem_desc_scales(uint32_t saddr) {
+    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)1u << 16) | ((uint64_t)(128u >> 4) << 32) | ((uint64_t)1u << 46);
+}
+
+// Instruction descriptor of the block-scaled kinds: element formats at bits 7-9 (A) and 10-12 (B), both K-major, N >> 3
+// at bits 17-22, e8m0 scales (bit 23), M >> 7 at bits 27-28; the byte of the scale columns that one MMA uses goes to
+// bits 4-5 (B) and 29-30 (A).
+__host__ __device__ constexpr uint32_t umma_idesc_mx(uint32_t fmt_a, uint32_t fmt_b, int M, int N) {
+    return (fmt_a << 7) | (fmt_b << 10) | ((uint32_t)(N >> 3) << 17) | (1u << 23) | ((uint32_t)(M >> 7) << 27);
+}
+__host__ __device__ constexpr uint32_t umma_idesc_scale_id(uint32_t id) { return (id << 4) | (id << 29); }
 
 // Instruction descriptor, kind::i8 with UNSIGNED 8-bit A and B (formats 0), D = S32, A MN-major (bit 15), B K-major.
 __host__ __device__ constexpr uint32_t umma_idesc_u8_amn(int M, int N) {
