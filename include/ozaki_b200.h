@@ -250,6 +250,11 @@ size_t ozk_mx_scale_bytes(int groups, int rows, int k);
  * infinite or NaN value gets the scale 255.                                                                  */
 int ozk_mx_quantize(const void* x, int dtype, int groups, int rows, int k, int64_t group_stride, int64_t row_stride,
                     int64_t k_stride, int fmt, int round_up, uint8_t* codes, uint8_t* scales, ozk_stream_t stream);
+/* Both operands of x (rows x cols, any strides >= 0) from one read of it: along_rows holds the rows (contracted axis:
+ * cols), along_cols the columns (contracted axis: rows).  Here and below an operand is one 32-byte aligned buffer, its
+ * codes followed by its scales.                                                                              */
+int ozk_mx_quantize_both(const void* x, int dtype, int rows, int cols, int64_t row_stride, int64_t col_stride, int fmt,
+                         int round_up, uint8_t* along_rows, uint8_t* along_cols, ozk_stream_t stream);
 /* out[g][r][l] (contiguous, 16-byte aligned) = code 2^(s - 127), computed in FP32, rounded to dtype           */
 int ozk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int fmt, int groups, int rows, int k, void* out,
                       int dtype, ozk_stream_t stream);
@@ -266,6 +271,19 @@ int ozk_mx_gemm(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, cons
 int ozk_mx_grouped_gemm(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
                         const uint8_t* B_scales, int B_fmt, int rows, int n, int k, int groups, const int32_t* ends,
                         int fill, void* C, int64_t ldc, int dtype, int32_t* err, ozk_stream_t stream);
+/* A linear layer and its gradients as MX products: y (m x n, of x's dtype) = Q(x) Q(w)^T for x (m x k), w (n x k);
+ * dx (m x k) = Q(dy) Q(w^T)^T, dw (n x k) = Q(dy^T) Q(x^T)^T, each operand quantised along the axis its product
+ * contracts.  The forward call writes the operands along k (scratch), and those along m and n that the backward call
+ * takes where they are not NULL; the backward call writes dy's (scratch) and the gradients that are not NULL.  x, w and
+ * dy of any strides >= 0; y, dx and dw contiguous.                                                            */
+int ozk_mx_linear_forward(const void* x, int x_dtype, int64_t x_row_stride, int64_t x_col_stride, const void* w,
+                          int w_dtype, int64_t w_row_stride, int64_t w_col_stride, int m, int n, int k, int fmt,
+                          int round_up, uint8_t* x_along_k, uint8_t* w_along_k, uint8_t* x_along_m, uint8_t* w_along_n,
+                          void* y, int32_t* err, ozk_stream_t stream);
+int ozk_mx_linear_backward(const void* dy, int dy_dtype, int64_t dy_row_stride, int64_t dy_col_stride,
+                           const uint8_t* x_along_m, const uint8_t* w_along_n, int m, int n, int k, int fmt, int round_up,
+                           uint8_t* dy_along_n, uint8_t* dy_along_m, void* dx, int dx_dtype, void* dw, int dw_dtype,
+                           int32_t* err, ozk_stream_t stream);
 /* Root-mean-square norm with an MX output: t = x + residual (residual may be NULL), y = t / sqrt(mean(t^2) + eps)
  * weight over rows of d values, all in FP32; y quantised as ozk_mx_quantize does, into an operand of `rows` vectors of
  * length d; t rounded to dtype into sum (rows x d, contiguous; may be NULL).  x, residual: contiguous rows, row strides

@@ -32,8 +32,8 @@ def __getattr__(name):
     if name in ("ResidueChain", "planes_for", "chain_bound"):
         from . import chain
         return getattr(chain, name)
-    if name in ("MXMatrix", "mx_quantize", "mx_matmul", "mx_grouped_matmul", "mx_rms_norm", "mx_linear",
-                "mx_check_errors"):
+    if name in ("MXMatrix", "mx_quantize", "mx_quantize_both", "mx_matmul", "mx_grouped_matmul", "mx_rms_norm",
+                "mx_linear", "mx_check_errors"):
         from . import mx
         return getattr(mx, name)
     if name in ("coprime_ip", "int8_crt", "chain_cost_model"):
@@ -50,5 +50,5 @@ __all__ = ["OzakiCRT", "DistributedOzakiCRT", "PersistA", "full_certificate", "M
            "sigma_of", "make_config_table", "pick_config", "limbs_for", "_limbs_for", "_pow2tab", "modulus_product",
            "make_inputs", "make_inputs_w", "config_inputs", "Sample", "exact_sample", "audit_bound", "CONFIGS",
            "AccuracySample", "correctly_rounded_products", "two_products", "coprime_ip", "int8_crt",
-           "chain_cost_model", "ResidueChain", "planes_for", "chain_bound", "MXMatrix", "mx_quantize", "mx_matmul",
-           "mx_grouped_matmul", "mx_rms_norm", "mx_linear", "mx_check_errors", "_lib"]
+           "chain_cost_model", "ResidueChain", "planes_for", "chain_bound", "MXMatrix", "mx_quantize",
+           "mx_quantize_both", "mx_matmul", "mx_grouped_matmul", "mx_rms_norm", "mx_linear", "mx_check_errors", "_lib"]

@@ -61,6 +61,9 @@ _SIGNATURES = {
     "ozk_mx_code_bytes": ([I32, I32, I32, I32], SZ),
     "ozk_mx_scale_bytes": ([I32, I32, I32], SZ),
     "ozk_mx_quantize": ([P, I32, I32, I32, I32, I64, I64, I64, I32, I32, P, P, P], I32),
+    "ozk_mx_quantize_both": ([P, I32, I32, I32, I64, I64, I32, I32, P, P, P], I32),
+    "ozk_mx_linear_forward": ([P, I32, I64, I64, P, I32, I64, I64, I32, I32, I32, I32, I32, P, P, P, P, P, P, P], I32),
+    "ozk_mx_linear_backward": ([P, I32, I64, I64, P, P, I32, I32, I32, I32, I32, P, P, P, I32, P, I32, P, P], I32),
     "ozk_mx_dequantize": ([P, P, I32, I32, I32, I32, P, I32, P], I32),
     "ozk_mx_gemm": ([P, P, I32, P, P, I32, I32, I32, I32, P, I64, I32, P, P], I32),
     "ozk_mx_grouped_gemm": ([P, P, I32, P, P, I32, I32, I32, I32, I32, P, I32, P, I64, I32, P, P], I32),

@@ -10,247 +10,246 @@ namespace {
 
 constexpr int THREADS = 256;
 
-// ---- quantisation, contracted axis contiguous ----------------------------------------------------------------------
-// One CTA per scale tile (128 rows x 128 elements): 16 lanes hold a row's 128 elements, eight each, so a block of 32 is
-// four lanes and its largest magnitude two shuffles away.  All of a thread's eight loads are issued before the first is
-// used.  The tile's 512 scale bytes are gathered in shared memory and leave as one contiguous store.
-template <typename T, int FMT>
-__global__ void __launch_bounds__(THREADS)
-    quantize_rows_kernel(const T* __restrict__ x, long long group_stride, long long row_stride, int rows, int k,
-                         bool up, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+// ---- quantisation ---------------------------------------------------------------------------------------------------
+// A job reads an I x J matrix (times groups; element (i, j) at x + i si + j sj) in tiles of 128 x 128 and writes it as the
+// operand that contracts j (vectors are rows, `row_*`), as the one that contracts i (vectors are columns, `col_*`), or
+// as both from one read.
+struct QuantJob {
+    const void* x;
+    long long gs, si, sj;
+    int groups, I, J;
+    uint8_t *row_codes, *row_scales, *col_codes, *col_scales;
+    const void *begin, *end;                 // the bytes that the matrix occupies (rows kernel)
+};
+
+__device__ __forceinline__ void copy_scale_tile(uint8_t* __restrict__ to, const uint8_t* sc) {
+    if (threadIdx.x < TILE_BYTES / 16)
+        reinterpret_cast<uint4*>(to)[threadIdx.x] = reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+}
+
+// Eight consecutive values of which 16 bytes need not be aligned: the aligned vectors around them, shifted into place,
+// where those lie within [begin, end); one by one otherwise.
+template <typename T>
+__device__ __forceinline__ void load8_any(const T* __restrict__ p, int count, const void* begin, const void* end,
+                                          float (&v)[8]) {
+    constexpr int NV = sizeof(T) == 4 ? 3 : 2, NW = 4 * NV;
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p), a0 = at & ~(uintptr_t)15;
+    const uint32_t sh = (uint32_t)(at & 15);
+    if (count < 8 || a0 < reinterpret_cast<uintptr_t>(begin) || a0 + 16 * NV > reinterpret_cast<uintptr_t>(end)) {
+        load8(p, false, count, v);
+        return;
+    }
+    uint32_t w[NW + 2];
+#pragma unroll
+    for (int q = 0; q < NV; q++) {
+        const uint4 u = __ldg(reinterpret_cast<const uint4*>(a0) + q);
+        w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
+    }
+    w[NW] = w[NW + 1] = 0u;
+    if (sh & 8u) {
+#pragma unroll
+        for (int j = 0; j < NW; j++) w[j] = w[j + 2];
+    }
+    if (sh & 4u) {
+#pragma unroll
+        for (int j = 0; j < NW; j++) w[j] = w[j + 1];
+    }
+    if (sizeof(T) == 2 && (sh & 2u)) {
+#pragma unroll
+        for (int j = 0; j < NW; j++) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
+    }
+    const T* e = reinterpret_cast<const T*>(w);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = to_f32(e[j]);
+}
+
+// One row's eight values per lane (16 lanes a row of the tile) to codes in global memory and the scale byte in `sc`: a
+// block of 32 is four lanes, its largest magnitude two shuffles away.
+template <int FMT>
+__device__ __forceinline__ void emit_row(float (&v)[8], bool up, int r, int here, int lane16, uint8_t* __restrict__ ct,
+                                         long long pitch, uint8_t* sc) {
+    const int s = block_scale<FMT>(quad_max(max_bits8(v)), up);
+    const float inv = scale_inverse(s);
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] *= inv;
+    const uint2 c = encode8<FMT>(v, s == 255);
+    if (r < here) {
+        if (FMT == OZK_MX_E2M1)
+            *reinterpret_cast<uint32_t*>(ct + r * pitch + lane16 * 4) = c.x;
+        else
+            *reinterpret_cast<uint2*>(ct + r * pitch + lane16 * 8) = c;
+    }
+    if ((lane16 & 3) == 0) sc[scale_slot(r, lane16 >> 2)] = (uint8_t)s;
+}
+
+// The row operand, rows contiguous.  One CTA per scale tile; all of a thread's eight loads are issued before the first is
+// used, and the tile's 512 scale bytes leave as one contiguous store.  ALIGNED: rows start on 16-byte boundaries.
+template <typename T, int FMT, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const __grid_constant__ QuantJob q, bool up) {
     __shared__ __align__(16) uint8_t sc[TILE_BYTES];
-    const int ktiles = padded_k(k) / TILE, rtiles = row_tiles(rows);
+    const int ktiles = padded_k(q.J) / TILE, rtiles = row_tiles(q.I);
     const int kt = (int)(blockIdx.x % (unsigned)ktiles);
     const int t = (int)(blockIdx.x / (unsigned)ktiles);
     const int rt = t % rtiles, g = t / rtiles;
     const int lane16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
     const int col = kt * TILE + lane16 * 8;
-    const int here = min(TILE, rows - rt * TILE);
-    const T* xt = x + g * group_stride + (long long)rt * TILE * row_stride + col;
-    const bool whole = col + 8 <= k;
-    const int count = max(0, k - col);
+    const int here = min(TILE, q.I - rt * TILE);
+    const T* xt = static_cast<const T*>(q.x) + g * q.gs + (long long)rt * TILE * q.si + col;
+    const int count = max(0, q.J - col);
 
     float v[8][8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
         const int r = r0 + 16 * i;
-        load8(xt + (long long)r * row_stride, whole && r < here, r < here ? count : 0, v[i]);
+        const int n = r < here ? count : 0;
+        if (ALIGNED) load8(xt + (long long)r * q.si, n >= 8, n, v[i]);
+        else load8_any(xt + (long long)r * q.si, n, q.begin, q.end, v[i]);
     }
-    const long long pitch = code_pitch(FMT, k);
-    uint8_t* ct = codes + ((long long)g * rows + (long long)rt * TILE) * pitch;
+    const long long pitch = code_pitch(FMT, q.J);
+    uint8_t* ct = q.row_codes + ((long long)g * q.I + (long long)rt * TILE) * pitch + kt * (FMT == OZK_MX_E2M1 ? 64 : 128);
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int r = r0 + 16 * i;
-        const int s = block_scale<FMT>(quad_max(max_bits8(v[i])), up);
-        const float inv = scale_inverse(s);
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[i][j] *= inv;
-        const uint2 c = encode8<FMT>(v[i], s == 255);
-        if (r < here) {
-            if (FMT == OZK_MX_E2M1)
-                *reinterpret_cast<uint32_t*>(ct + r * pitch + col / 2) = c.x;
-            else
-                *reinterpret_cast<uint2*>(ct + r * pitch + col) = c;
-        }
-        if ((lane16 & 3) == 0) sc[scale_slot(r, lane16 >> 2)] = (uint8_t)s;
-    }
+    for (int i = 0; i < 8; i++) emit_row<FMT>(v[i], up, r0 + 16 * i, here, lane16, ct, pitch, sc);
     __syncthreads();
-    if (threadIdx.x < TILE_BYTES / 16)
-        reinterpret_cast<uint4*>(scales + (long long)blockIdx.x * TILE_BYTES)[threadIdx.x] =
-            reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+    copy_scale_tile(q.row_scales + (long long)blockIdx.x * TILE_BYTES, sc);
 }
 
-// ---- quantisation, any strides --------------------------------------------------------------------------------------
-// The tile goes through shared memory as [element][row], so that whichever axis is contiguous is read along the lanes
-// (`LOAD` 0: rows contiguous and 16-byte aligned, vector loads; 1: one element a lane along the rows; 2: along the
-// contracted axis).  A thread then owns a block of a row pair (16-bit types: both rows' elements are one 32-bit word) or
-// of one row (FP32), so a block's largest magnitude needs no exchange.  The codes go back through the same memory to
-// leave as whole row segments.
-template <typename T>
-struct TileOf {
-    static constexpr int PITCH = sizeof(T) == 4 ? 129 : 130;   // odd in 32-bit words: rows and columns free of conflicts
-    static constexpr int BYTES = (TILE * PITCH * (int)sizeof(T) + 15) / 16 * 16;
-};
-
-template <typename T, int LOAD>
-__device__ __forceinline__ void load_tile(T* __restrict__ tile, const T* __restrict__ xt, long long row_stride,
-                                          long long k_stride, int here, int kept) {
-    constexpr int P = TileOf<T>::PITCH;
-    if (LOAD == 0) {
-        constexpr int VEC = 16 / (int)sizeof(T);               // elements of a 16-byte load
-        constexpr int PER = TILE / VEC;                        // loads of one k row of the tile
-        constexpr int WORDS = (int)sizeof(T) * VEC / 4;
-        static_assert(TILE * PER % THREADS == 0, "whole passes");
-#pragma unroll 8
-        for (int i = 0; i < TILE * PER / THREADS; i++) {
-            const int id = threadIdx.x + i * THREADS;
-            const int kk = id / PER, r = id % PER * VEC;
-            uint4 w = make_uint4(0u, 0u, 0u, 0u);
-            if (kk < kept) {
-                const T* p = xt + kk * k_stride + r;
-                if (r + VEC <= here) {
-                    w = __ldg(reinterpret_cast<const uint4*>(p));
-                } else {
-                    T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-                    for (int j = 0; j < VEC; j++)
-                        if (r + j < here) e[j] = p[j];
-                }
-            }
-            uint32_t* d = reinterpret_cast<uint32_t*>(tile + kk * P + r);   // 4-byte aligned: P and r are even or T is
-            const uint32_t ww[4] = {w.x, w.y, w.z, w.w};                    // 4 bytes wide
-#pragma unroll
-            for (int j = 0; j < WORDS; j++) d[j] = ww[j];
-        }
-    } else {
-#pragma unroll 8
-        for (int i = 0; i < TILE * TILE / THREADS; i++) {
-            const int id = threadIdx.x + i * THREADS;
-            const int kk = LOAD == 1 ? id / TILE : id % TILE, r = LOAD == 1 ? id % TILE : id / TILE;
-            T e = from_f32<T>(0.0f);
-            if (kk < kept && r < here) e = xt[r * row_stride + kk * k_stride];
-            tile[kk * P + r] = e;
-        }
-    }
-}
-
-// The 32 values of block `b` of row `r` (FP32) or rows r, r + 1 (16-bit types) to codes and scale bytes
-template <int FMT>
-__device__ __forceinline__ void encode_block(const float* tile, int r, int b, bool up, uint4 (&c)[2], int& s) {
-    constexpr int P = TileOf<float>::PITCH;
-    const float* p = tile + b * BLOCK * P + r;
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < BLOCK; j++) m = max(m, __float_as_uint(p[j * P]) & 0x7fffffffu);
-    s = block_scale<FMT>(m, up);
+// The 32 values of one block, largest magnitude `m` (FP32 bits), to its code bytes
+template <int FMT, typename Get>
+__device__ __forceinline__ int encode_block(uint32_t m, bool up, uint4 (&c)[2], Get get) {
+    const int s = block_scale<FMT>(m, up);
     const float inv = scale_inverse(s);
     uint2 w[4];
 #pragma unroll
     for (int q = 0; q < 4; q++) {
         float v[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = p[(8 * q + j) * P] * inv;
+        for (int j = 0; j < 8; j++) v[j] = get(8 * q + j) * inv;
         w[q] = encode8<FMT>(v, s == 255);
     }
     c[0] = FMT == OZK_MX_E2M1 ? make_uint4(w[0].x, w[1].x, w[2].x, w[3].x) : make_uint4(w[0].x, w[0].y, w[1].x, w[1].y);
     c[1] = make_uint4(w[2].x, w[2].y, w[3].x, w[3].y);
+    return s;
 }
 
-__device__ __forceinline__ uint32_t bits_of_max(__half*, uint32_t m16) {
-    return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m16)));
-}
-__device__ __forceinline__ uint32_t bits_of_max(__nv_bfloat16*, uint32_t m16) { return m16 << 16; }
+__device__ __forceinline__ float low_half(uint32_t w, __half*) { return __half2float(__ushort_as_half((unsigned short)w)); }
+__device__ __forceinline__ float high_half(uint32_t w, __half*) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
+__device__ __forceinline__ float low_half(uint32_t w, __nv_bfloat16*) { return __uint_as_float(w << 16); }
+__device__ __forceinline__ float high_half(uint32_t w, __nv_bfloat16*) { return __uint_as_float(w & 0xffff0000u); }
 
-template <typename T, int FMT>
-__device__ __forceinline__ void encode_pair(const T* tile, int r, int b, bool up, uint4 (&c)[2][2], int (&s)[2]) {
-    constexpr int P = TileOf<T>::PITCH;
-    const T* p = tile + b * BLOCK * P + r;
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < BLOCK; j++) m = __vmaxu2(m, *reinterpret_cast<const uint32_t*>(p + j * P) & 0x7fff7fffu);
-#pragma unroll
-    for (int h = 0; h < 2; h++) s[h] = block_scale<FMT>(bits_of_max((T*)nullptr, h ? m >> 16 : m & 0xffffu), up);
-    const float inv[2] = {scale_inverse(s[0]), scale_inverse(s[1])};
-    uint2 w[2][4];
-#pragma unroll
-    for (int q = 0; q < 4; q++) {
-        float v[2][8];
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            v[0][j] = to_f32(p[(8 * q + j) * P]) * inv[0];
-            v[1][j] = to_f32(p[(8 * q + j) * P + 1]) * inv[1];
-        }
-        w[0][q] = encode8<FMT>(v[0], s[0] == 255);
-        w[1][q] = encode8<FMT>(v[1], s[1] == 255);
-    }
-#pragma unroll
-    for (int h = 0; h < 2; h++) {
-        c[h][0] = FMT == OZK_MX_E2M1 ? make_uint4(w[h][0].x, w[h][1].x, w[h][2].x, w[h][3].x)
-                                     : make_uint4(w[h][0].x, w[h][0].y, w[h][1].x, w[h][1].y);
-        c[h][1] = make_uint4(w[h][2].x, w[h][2].y, w[h][3].x, w[h][3].y);
-    }
-}
-
-template <typename T, int FMT, int LOAD>
+// The column operand, alone or with the row operand (one or two jobs in one launch).  A thread owns a block of 32
+// values down a column (FP32) or a pair of columns (16-bit types, one 32-bit word a row), which it reads straight into
+// registers: a warp reads 128 contiguous bytes a row, nothing is transposed in memory, and a block's largest magnitude
+// needs no exchange.  Only the codes go through shared memory, to leave as whole segments of the operand's vectors.
+// The row operand then reads the tile again, from L1.  WORDS: the pairs are aligned 32-bit words (else element by element,
+// any strides, and no row operand).
+template <typename T, int FMT, bool WORDS>
 __global__ void __launch_bounds__(THREADS)
-    quantize_tile_kernel(const T* __restrict__ x, long long group_stride, long long row_stride, long long k_stride,
-                         int rows, int k, bool up, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ __align__(16) uint8_t sc[TILE_BYTES];
-    constexpr int SEG = FMT == OZK_MX_E2M1 ? TILE / 2 : TILE;   // code bytes of a row of the tile
+    quantize_dual_kernel(const __grid_constant__ QuantJob q0, const __grid_constant__ QuantJob q1, unsigned tiles0, bool up) {
+    constexpr int SEG = FMT == OZK_MX_E2M1 ? TILE / 2 : TILE;   // code bytes of a vector of the tile
     constexpr int CP = SEG + 16;
-    static_assert(TILE * CP <= TileOf<T>::BYTES, "codes fit where the values were");
-    T* tile = reinterpret_cast<T*>(smem);
-    const int ktiles = padded_k(k) / TILE, rtiles = row_tiles(rows);
-    // rows contiguous: neighbouring CTAs take neighbouring row tiles, so that their reads share DRAM pages
-    int kt, rt, g;
-    if (LOAD == 2) {
-        kt = (int)(blockIdx.x % (unsigned)ktiles);
-        const int t = (int)(blockIdx.x / (unsigned)ktiles);
-        rt = t % rtiles;
-        g = t / rtiles;
-    } else {
-        rt = (int)(blockIdx.x % (unsigned)rtiles);
-        const int t = (int)(blockIdx.x / (unsigned)rtiles);
-        kt = t % ktiles;
-        g = t / ktiles;
+    __shared__ __align__(16) uint8_t staged[TILE * CP];
+    __shared__ __align__(16) uint8_t sc[2][TILE_BYTES];
+    const bool second = blockIdx.x >= tiles0;
+    const QuantJob& q = second ? q1 : q0;
+    const unsigned tile = second ? blockIdx.x - tiles0 : blockIdx.x;
+    const int jtiles = padded_k(q.J) / TILE, itiles = padded_k(q.I) / TILE;
+    const int jt = (int)(tile % (unsigned)jtiles);
+    const int t = (int)(tile / (unsigned)jtiles);
+    const int it = t % itiles, g = t / itiles;
+    const int rows = min(TILE, q.I - it * TILE), cols = min(TILE, q.J - jt * TILE);
+    const T* xt = static_cast<const T*>(q.x) + g * q.gs + (long long)it * TILE * q.si + (long long)jt * TILE * q.sj;
+
+    if (q.col_codes) {
+        if constexpr (sizeof(T) == 4) {
+            const int c = threadIdx.x & (TILE - 1);
+#pragma unroll 1
+            for (int h = 0; h < 2; h++) {
+                const int b = (threadIdx.x >> 7) + 2 * h;
+                float v[BLOCK];
+                uint32_t m = 0;
+                const T* p = xt + (long long)(b * BLOCK) * q.si + c * q.sj;
+#pragma unroll
+                for (int j = 0; j < BLOCK; j++) v[j] = (c < cols && b * BLOCK + j < rows) ? __ldg(p + j * q.si) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < BLOCK; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+                uint4 o[2];
+                sc[0][scale_slot(c, b)] = (uint8_t)encode_block<FMT>(m, up, o, [&](int j) { return v[j]; });
+                uint4* d = reinterpret_cast<uint4*>(staged + c * CP + b * (SEG / 4));
+                d[0] = o[0];
+                if (FMT != OZK_MX_E2M1) d[1] = o[1];
+            }
+        } else {
+            const int c = 2 * (threadIdx.x & 63), b = threadIdx.x >> 6;
+            uint32_t v[BLOCK];
+            const T* p = xt + (long long)(b * BLOCK) * q.si + c * q.sj;
+#pragma unroll
+            for (int j = 0; j < BLOCK; j++) {
+                v[j] = 0u;
+                if (b * BLOCK + j < rows) {
+                    if (WORDS && c + 1 < cols) {
+                        v[j] = __ldg(reinterpret_cast<const uint32_t*>(p + j * q.si));
+                    } else if (c < cols) {
+                        v[j] = __ldg(reinterpret_cast<const unsigned short*>(p + j * q.si));
+                        if (c + 1 < cols) v[j] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p + j * q.si + q.sj)) << 16;
+                    }
+                }
+            }
+            uint32_t m = 0;                                      // magnitudes of 16-bit types are ordered like their bits
+#pragma unroll
+            for (int j = 0; j < BLOCK; j++) m = __vmaxu2(m, v[j] & 0x7fff7fffu);
+            T* const type = nullptr;
+            uint4 o[2];
+            uint4* d = reinterpret_cast<uint4*>(staged + c * CP + b * (SEG / 4));
+            sc[0][scale_slot(c, b)] = (uint8_t)encode_block<FMT>(__float_as_uint(low_half(m, type)), up, o,
+                                                                 [&](int j) { return low_half(v[j], type); });
+            d[0] = o[0];
+            if (FMT != OZK_MX_E2M1) d[1] = o[1];
+            d = reinterpret_cast<uint4*>(staged + (c + 1) * CP + b * (SEG / 4));
+            sc[0][scale_slot(c + 1, b)] = (uint8_t)encode_block<FMT>(__float_as_uint(high_half(m, type)), up, o,
+                                                                     [&](int j) { return high_half(v[j], type); });
+            d[0] = o[0];
+            if (FMT != OZK_MX_E2M1) d[1] = o[1];
+        }
     }
-    const int here = min(TILE, rows - rt * TILE), kept = min(TILE, k - kt * TILE);
-    load_tile<T, LOAD>(tile, x + g * group_stride + (long long)rt * TILE * row_stride + (long long)kt * TILE * k_stride,
-                       row_stride, k_stride, here, kept);
-    __syncthreads();
-    if constexpr (sizeof(T) == 4) {
-        uint4 c[2][2];
-        const int r = threadIdx.x & (TILE - 1);
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            int s;
-            const int b = (threadIdx.x >> 7) + 2 * i;
-            encode_block<FMT>(tile, r, b, up, c[i], s);
-            sc[scale_slot(r, b)] = (uint8_t)s;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 2; i++) {
-            uint4* d = reinterpret_cast<uint4*>(smem + r * CP + ((threadIdx.x >> 7) + 2 * i) * (SEG / 4));
-            d[0] = c[i][0];
-            if (FMT != OZK_MX_E2M1) d[1] = c[i][1];
-        }
-    } else {
-        uint4 c[2][2];
-        int s[2];
-        const int r = 2 * (threadIdx.x & 63), b = threadIdx.x >> 6;
-        encode_pair<T, FMT>(tile, r, b, up, c, s);
-        sc[scale_slot(r, b)] = (uint8_t)s[0];
-        sc[scale_slot(r + 1, b)] = (uint8_t)s[1];
-        __syncthreads();
+    if (WORDS && q.row_codes) {
+        const int lane16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+        const long long pitch = code_pitch(FMT, q.J);
+        uint8_t* ct = q.row_codes + ((long long)g * q.I + (long long)it * TILE) * pitch + (long long)jt * SEG;
+        const int count = max(0, cols - lane16 * 8);
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            uint4* d = reinterpret_cast<uint4*>(smem + (r + h) * CP + b * (SEG / 4));
-            d[0] = c[h][0];
-            if (FMT != OZK_MX_E2M1) d[1] = c[h][1];
+            float v[4][8];
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = r0 + 16 * (4 * h + i), n = r < rows ? count : 0;
+                load8(xt + (long long)r * q.si + lane16 * 8, n >= 8, n, v[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) emit_row<FMT>(v[i], up, r0 + 16 * (4 * h + i), rows, lane16, ct, pitch, sc[1]);
         }
     }
     __syncthreads();
-    const long long pitch = code_pitch(FMT, k);
-    uint8_t* ct = codes + ((long long)g * rows + (long long)rt * TILE) * pitch + (long long)kt * SEG;
-    constexpr int VECS = SEG / 16;
+    if (q.col_codes) {
+        const long long pitch = code_pitch(FMT, q.I);
+        uint8_t* ct = q.col_codes + ((long long)g * q.J + (long long)jt * TILE) * pitch + (long long)it * SEG;
+        constexpr int VECS = SEG / 16;
 #pragma unroll
-    for (int i = 0; i < TILE * VECS / THREADS; i++) {
-        const int id = threadIdx.x + i * THREADS;
-        const int r = id / VECS, q = id % VECS;
-        if (r < here)
-            *reinterpret_cast<uint4*>(ct + r * pitch + 16 * q) = *reinterpret_cast<const uint4*>(smem + r * CP + 16 * q);
+        for (int i = 0; i < TILE * VECS / THREADS; i++) {
+            const int id = threadIdx.x + i * THREADS;
+            const int r = id / VECS, k = id % VECS;
+            if (r < cols)
+                *reinterpret_cast<uint4*>(ct + r * pitch + 16 * k) = *reinterpret_cast<const uint4*>(staged + r * CP + 16 * k);
+        }
+        copy_scale_tile(q.col_scales + (((long long)g * jtiles + jt) * itiles + it) * TILE_BYTES, sc[0]);
     }
-    if (threadIdx.x < TILE_BYTES / 16)
-        reinterpret_cast<uint4*>(scales + (((long long)g * rtiles + rt) * ktiles + kt) * TILE_BYTES)[threadIdx.x] =
-            reinterpret_cast<const uint4*>(sc)[threadIdx.x];
+    if (WORDS && q.row_codes)
+        copy_scale_tile(q.row_scales + (((long long)g * itiles + it) * jtiles + jt) * TILE_BYTES, sc[1]);
 }
 
 // ---- the way back ---------------------------------------------------------------------------------------------------
 // One CTA per scale tile, 16 lanes a row as in the quantisation; each value is one multiplication in FP32 and one
 // rounding to the output type (none for the values of ordinary scales, which BF16 and FP32 hold exactly).
-template <typename T, int FMT>
+template <typename T, int FMT, bool ALIGNED>
 __global__ void __launch_bounds__(THREADS)
     dequantize_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ scales, int rows, int k,
                       T* __restrict__ out) {
@@ -280,46 +279,82 @@ __global__ void __launch_bounds__(THREADS)
         reinterpret_cast<uint4*>(sc)[threadIdx.x] =
             __ldg(reinterpret_cast<const uint4*>(scales + (long long)blockIdx.x * TILE_BYTES) + threadIdx.x);
     __syncthreads();
-    const bool whole = col + 8 <= k && (k * (int)sizeof(T)) % 16 == 0;
-    const int count = max(0, k - col);
-    T* ot = out + ((long long)g * rows + (long long)rt * TILE) * k + col;
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int r = r0 + 16 * i;
-        if (r >= here) continue;
-        const float s = scale_value(sc[scale_slot(r, lane16 >> 2)]);
-        float v[8];
+    T* ot = out + ((long long)g * rows + (long long)rt * TILE) * k + kt * TILE;
+    auto values = [&](int i, float (&v)[8]) {
+        const float s = scale_value(sc[scale_slot(r0 + 16 * i, lane16 >> 2)]);
         decode8<FMT>(c[i], v);
 #pragma unroll
         for (int j = 0; j < 8; j++) v[j] *= s;
-        store8(ot + (long long)r * k, whole, count, v);
+    };
+    if (ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = r0 + 16 * i;
+            if (r >= here) continue;
+            float v[8];
+            values(i, v);
+            store8(ot + (long long)r * k + lane16 * 8, col + 8 <= k, max(0, k - col), v);
+        }
+    } else {
+        // rows that start anywhere: through shared memory, so that a warp's lanes write neighbouring elements
+        extern __shared__ __align__(16) uint8_t smem[];
+        T* tile = reinterpret_cast<T*>(smem);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float v[8];
+            values(i, v);
+            store8(tile + (r0 + 16 * i) * TILE + lane16 * 8, true, 8, v);
+        }
+        __syncthreads();
+        const int cols = min(TILE, k - kt * TILE);
+        for (int r = threadIdx.x >> 5; r < here; r += THREADS / 32)
+#pragma unroll
+            for (int j = 0; j < TILE / 32; j++) {
+                const int e = (threadIdx.x & 31) + 32 * j;
+                if (e < cols) ot[(long long)r * k + e] = tile[r * TILE + e];
+            }
     }
 }
 
 // ---- root-mean-square norm with an MX output -----------------------------------------------------------------------
 // t = x (+ residual), y = t / sqrt(mean(t^2) + eps) weight, y quantised; t, rounded to the type of x, is the next
-// residual.  Everything between the loads and the codes stays in FP32 registers: one pass over x and the residual, TPR
-// threads a row with NC chunks of eight values each (longer rows read the rest a second time).  The sums are taken in a
-// fixed order.
+// residual.  Everything between the loads and the codes stays in registers: one pass over x and the residual, TPR threads
+// a row with NC chunks of eight values each (longer rows read the rest a second time).  The sums are taken in a fixed
+// order.  y is computed to its last FP32 bit: a rounding on the way would move values across the borders between codes.
 template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* part) {
+__device__ __forceinline__ double row_sum(double v, double* part) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if (TPR == 32) return v;
+    __syncthreads();                                           // `part` may still be read from an earlier sum
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = (threadIdx.x & 31) < TPR / 32 ? part[threadIdx.x & 31] : 0.0f;
+    v = (threadIdx.x & 31) < TPR / 32 ? part[threadIdx.x & 31] : 0.0;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
+    for (int o = TPR / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return __shfl_sync(0xffffffffu, v, 0);
+}
+
+// 1 / sqrt(a) as a sum of two FP32 numbers: the FP32 root and one Newton step whose residual 1 - a r^2 is taken exactly
+__device__ __forceinline__ float2 inverse_root(double a) {
+    if (!(a < 3.0e38)) {                                        // beyond FP32 (or NaN)
+        const double r = 1.0 / sqrt(a);
+        const float h = (float)r;
+        return make_float2(h, (float)(r - (double)h));
+    }
+    const float ah = (float)a, al = (float)(a - (double)ah);
+    const float r = rsqrtf(ah);
+    const float q = ah * r, qe = fmaf(ah, r, -q);
+    const float e = fmaf(-q, r, 1.0f) - fmaf(qe, r, al * r * r);
+    return make_float2(r, 0.5f * r * e);
 }
 
 template <typename T, typename W, int FMT, int TPR, int NC>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
     rms_norm_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ residual, long long res_stride,
-                    const W* __restrict__ weight, int rows, int d, float eps, bool aligned, bool up,
+                    const W* __restrict__ weight, int rows, int d, double inv_d, float eps, bool aligned, bool up,
                     T* __restrict__ sum, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
-    __shared__ float part[32];
+    __shared__ double part[32];
     constexpr int RPB = TPR == 32 ? 4 : 1;
     const long long row = (long long)blockIdx.x * RPB + (RPB == 1 ? 0 : threadIdx.x / TPR);
     const int t = RPB == 1 ? threadIdx.x : threadIdx.x % TPR;
@@ -330,7 +365,6 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
     T* sr = sum ? sum + row * (long long)d : nullptr;
 
     float v[NC][8];
-    float sq = 0.0f;
     auto fetch = [&](int c, float (&o)[8]) {
         const int col = c * 8;
         const bool whole = aligned && col + 8 <= d;
@@ -343,27 +377,33 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
             for (int j = 0; j < 8; j++) o[j] += q[j];
         }
     };
-    auto note = [&](int c, const float (&o)[8]) {
-        if (sr) store8(sr + c * 8, aligned && c * 8 + 8 <= d, max(0, d - c * 8), o);
+    // sum of (t scale)^2: a thread's share in FP32, the shares in FP64
+    auto squares = [&](float scale, bool store) {
+        float sq = 0.0f;
+        auto note = [&](int c, const float (&o)[8]) {
+            if (store && sr) store8(sr + c * 8, aligned && c * 8 + 8 <= d, max(0, d - c * 8), o);
 #pragma unroll
-        for (int j = 0; j < 8; j++) sq = fmaf(o[j], o[j], sq);
+            for (int j = 0; j < 8; j++) {
+                const float u = o[j] * scale;
+                sq = fmaf(u, u, sq);
+            }
+        };
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+            if (t + i * TPR < chunks) note(t + i * TPR, v[i]);
+        for (int c = t + NC * TPR; c < chunks; c += TPR) {
+            float o[8];
+            fetch(c, o);
+            note(c, o);
+        }
+        return row_sum<TPR>((double)sq, part);
     };
 #pragma unroll
-    for (int i = 0; i < NC; i++) {
-        const int c = t + i * TPR;
-        if (c < chunks) fetch(c, v[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < NC; i++) {
-        const int c = t + i * TPR;
-        if (c < chunks) note(c, v[i]);
-    }
-    for (int c = t + NC * TPR; c < chunks; c += TPR) {
-        float o[8];
-        fetch(c, o);
-        note(c, o);
-    }
-    const float rstd = 1.0f / sqrtf(row_sum<TPR>(sq, part) / (float)d + eps);
+    for (int i = 0; i < NC; i++)
+        if (t + i * TPR < chunks) fetch(t + i * TPR, v[i]);
+    double total = squares(1.0f, true);
+    if (!(total < 3.0e38)) total = squares(0x1p-70f, false) * 0x1p140;   // squares beyond FP32: once more, scaled
+    const float2 rstd = inverse_root(total * inv_d + (double)eps);
 
     const long long pitch = code_pitch(FMT, d);
     uint8_t* cr = codes + row * pitch;
@@ -373,7 +413,11 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
         float w[8];
         load8(weight + c * 8, in && aligned && c * 8 + 8 <= d, in ? max(0, d - c * 8) : 0, w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = in ? o[j] * rstd * w[j] : 0.0f;
+        for (int j = 0; j < 8; j++) {
+            // t w rstd rounded once: the product's rounding error and the low part of rstd go along
+            const float p = o[j] * w[j], e = fmaf(o[j], w[j], -p);
+            o[j] = in ? fmaf(p, rstd.x, fmaf(p, rstd.y, e * rstd.x)) : 0.0f;
+        }
         const int s = block_scale<FMT>(quad_max(max_bits8(o)), up);
         const float inv = scale_inverse(s);
 #pragma unroll
@@ -412,23 +456,102 @@ long long tile_count(int groups, int rows, int k) {
 }
 
 template <typename T, int FMT>
-int launch_quantize(const T* x, int groups, int rows, int k, long long gs, long long rs, long long ks, bool up,
-                    uint8_t* codes, uint8_t* scales, cudaStream_t st) {
-    const unsigned grid = (unsigned)tile_count(groups, rows, k);
+int launch_rows(const QuantJob& q, bool aligned, bool up, cudaStream_t st) {
+    const unsigned grid = (unsigned)tile_count(q.groups, q.I, q.J);
+    if (aligned) quantize_rows_kernel<T, FMT, true><<<grid, THREADS, 0, st>>>(q, up);
+    else quantize_rows_kernel<T, FMT, false><<<grid, THREADS, 0, st>>>(q, up);
+    OZK_CHECK_LAUNCH();
+    return OZK_OK;
+}
+
+template <typename T, int FMT>
+int launch_dual(const QuantJob& a, const QuantJob& b, bool words, bool up, cudaStream_t st) {
+    const unsigned t0 = (unsigned)tile_count(a.groups, a.I, a.J);
+    const unsigned t1 = b.x ? (unsigned)tile_count(b.groups, b.I, b.J) : 0u;
+    if (words) quantize_dual_kernel<T, FMT, true><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
+    else quantize_dual_kernel<T, FMT, false><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
+    OZK_CHECK_LAUNCH();
+    return OZK_OK;
+}
+
+// `unit` bytes divide the starts of all rows (along i) of the job
+bool rows_aligned(const QuantJob& q, long long size, uintptr_t unit) {
+    return q.sj == 1 && reinterpret_cast<uintptr_t>(q.x) % unit == 0 && (q.I == 1 || q.si * size % (long long)unit == 0) &&
+           (q.groups == 1 || q.gs * size % (long long)unit == 0);
+}
+
+QuantJob swapped(const QuantJob& q) {
+    QuantJob t = q;
+    t.si = q.sj; t.sj = q.si; t.I = q.J; t.J = q.I;
+    t.row_codes = q.col_codes; t.row_scales = q.col_scales; t.col_codes = q.row_codes; t.col_scales = q.row_scales;
+    return t;
+}
+
+// One direction of a job (the row operand of q): the rows kernel where the contracted axis is contiguous, the column
+// operand of the matrix read the other way otherwise
+template <typename T, int FMT>
+int quantize_one(QuantJob q, bool up, cudaStream_t st) {
     const long long size = (long long)sizeof(T);
-    const bool base = aligned16(x) && (groups == 1 || gs * size % 16 == 0);
-    if (ks == 1 && base && (rows == 1 || rs * size % 16 == 0)) {
-        quantize_rows_kernel<T, FMT><<<grid, THREADS, 0, st>>>(x, gs, rs, rows, k, up, codes, scales);
+    q.col_codes = q.col_scales = nullptr;
+    if (q.sj == 1) {
+        q.begin = q.x;
+        q.end = static_cast<const T*>(q.x) + (q.groups - 1) * q.gs + (q.I - 1) * q.si + q.J;
+        return launch_rows<T, FMT>(q, rows_aligned(q, size, 16), up, st);
+    }
+    const QuantJob t = swapped(q);
+    return launch_dual<T, FMT>(t, QuantJob{}, sizeof(T) == 4 || rows_aligned(t, size, 4), up, st);
+}
+
+// Jobs of one type: in one launch where a row operand has to be written beside a column operand or there are two jobs,
+// and the alignment allows; one launch per operand otherwise
+template <typename T, int FMT>
+int quantize_jobs(const QuantJob* jobs, int count, bool up, cudaStream_t st) {
+    bool joint = true;
+    for (int i = 0; i < count; i++) {
+        const bool both = jobs[i].row_codes && jobs[i].col_codes;
+        if (!rows_aligned(jobs[i], (long long)sizeof(T), 16)) joint = false;
+        if (count == 1 && !both) joint = false;
+    }
+    long long tiles = 0;
+    for (int i = 0; i < count; i++) tiles += tile_count(jobs[i].groups, jobs[i].I, jobs[i].J);
+    if (joint && tiles <= 0x7fffffffLL) return launch_dual<T, FMT>(jobs[0], count > 1 ? jobs[1] : QuantJob{}, true, up, st);
+    for (int i = 0; i < count; i++) {
+        int rc = OZK_OK;
+        if (jobs[i].row_codes) rc = quantize_one<T, FMT>(jobs[i], up, st);
+        if (rc == OZK_OK && jobs[i].col_codes) rc = quantize_one<T, FMT>(swapped(jobs[i]), up, st);
+        if (rc != OZK_OK) return rc;
+    }
+    return OZK_OK;
+}
+
+int quantize(const QuantJob* jobs, int count, int dtype, int fmt, bool up, cudaStream_t st) {
+    switch (dtype) {
+        case OZK_F32:
+            return fmt == OZK_MX_E2M1 ? quantize_jobs<float, OZK_MX_E2M1>(jobs, count, up, st)
+                                      : quantize_jobs<float, OZK_MX_E4M3>(jobs, count, up, st);
+        case OZK_F16:
+            return fmt == OZK_MX_E2M1 ? quantize_jobs<__half, OZK_MX_E2M1>(jobs, count, up, st)
+                                      : quantize_jobs<__half, OZK_MX_E4M3>(jobs, count, up, st);
+        case OZK_BF16:
+            return fmt == OZK_MX_E2M1 ? quantize_jobs<__nv_bfloat16, OZK_MX_E2M1>(jobs, count, up, st)
+                                      : quantize_jobs<__nv_bfloat16, OZK_MX_E4M3>(jobs, count, up, st);
+        default: return OZK_ERR_ARG;
+    }
+}
+
+template <typename T, int FMT>
+int launch_dequantize_fmt(const uint8_t* codes, const uint8_t* scales, int groups, int rows, int k, T* out, cudaStream_t st) {
+    const unsigned grid = (unsigned)tile_count(groups, rows, k);
+    if ((long long)k * (int)sizeof(T) % 16 == 0 || (rows == 1 && groups == 1)) {
+        dequantize_kernel<T, FMT, true><<<grid, THREADS, 0, st>>>(codes, scales, rows, k, out);
     } else {
-        constexpr int bytes = TileOf<T>::BYTES;
-        const int load = rs == 1 && base && (k == 1 || ks * size % 16 == 0) ? 0 : rs == 1 || (rs < ks && ks != 1) ? 1 : 2;
-        auto kern = load == 0 ? quantize_tile_kernel<T, FMT, 0>
-                              : load == 1 ? quantize_tile_kernel<T, FMT, 1> : quantize_tile_kernel<T, FMT, 2>;
+        constexpr int bytes = TILE * TILE * (int)sizeof(T);
         if (bytes > 48 * 1024 - TILE_BYTES) {
-            const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            const cudaError_t e = cudaFuncSetAttribute(dequantize_kernel<T, FMT, false>,
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
             if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
         }
-        kern<<<grid, THREADS, bytes, st>>>(x, gs, rs, ks, rows, k, up, codes, scales);
+        dequantize_kernel<T, FMT, false><<<grid, THREADS, bytes, st>>>(codes, scales, rows, k, out);
     }
     OZK_CHECK_LAUNCH();
     return OZK_OK;
@@ -437,13 +560,8 @@ int launch_quantize(const T* x, int groups, int rows, int k, long long gs, long 
 template <typename T>
 int launch_dequantize(const uint8_t* codes, const uint8_t* scales, int fmt, int groups, int rows, int k, T* out,
                       cudaStream_t st) {
-    const unsigned grid = (unsigned)tile_count(groups, rows, k);
-    if (fmt == OZK_MX_E2M1)
-        dequantize_kernel<T, OZK_MX_E2M1><<<grid, THREADS, 0, st>>>(codes, scales, rows, k, out);
-    else
-        dequantize_kernel<T, OZK_MX_E4M3><<<grid, THREADS, 0, st>>>(codes, scales, rows, k, out);
-    OZK_CHECK_LAUNCH();
-    return OZK_OK;
+    return fmt == OZK_MX_E2M1 ? launch_dequantize_fmt<T, OZK_MX_E2M1>(codes, scales, groups, rows, k, out, st)
+                              : launch_dequantize_fmt<T, OZK_MX_E4M3>(codes, scales, groups, rows, k, out, st);
 }
 
 struct NormArgs {
@@ -469,7 +587,7 @@ int launch_norm(const NormArgs& a) {
     rms_norm_kernel<T, W, FMT, TPR, NC>                                                                              \
         <<<(unsigned)((a.rows + (TPR == 32 ? 3 : 0)) / (TPR == 32 ? 4 : 1)), TPR == 32 ? 128 : TPR, 0, a.st>>>(      \
             static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), a.res_stride,                 \
-            static_cast<const W*>(a.weight), a.rows, d, a.eps, aligned, a.up, static_cast<T*>(a.sum), a.codes, a.scales)
+            static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps, aligned, a.up, static_cast<T*>(a.sum), a.codes, a.scales)
     if (d <= 1024) OZK_NORM(32, 4);
     else if (d <= 4096) OZK_NORM(256, 2);
     else if (d <= 8192) OZK_NORM(256, 4);
@@ -504,20 +622,98 @@ extern "C" int ozk_mx_quantize(const void* x, int dtype, int groups, int rows, i
     if (!x || !codes || !scales || !fmt_ok(fmt) || groups < 1 || rows < 1 || k < 1 || k > OZK_MX_KMAX) return OZK_ERR_ARG;
     if (group_stride < 0 || row_stride < 0 || k_stride < 0 || !aligned16(codes) || !aligned16(scales)) return OZK_ERR_ARG;
     if (tile_count(groups, rows, k) < 0) return OZK_ERR_ARG;
+    QuantJob q = {};
+    q.x = x;
+    q.gs = groups == 1 ? 0 : group_stride;
+    q.si = row_stride;
+    q.sj = k == 1 ? 1 : k_stride;
+    q.groups = groups;
+    q.I = rows;
+    q.J = k;
+    q.row_codes = codes;
+    q.row_scales = scales;
+    return quantize(&q, 1, dtype, fmt, round_up != 0, reinterpret_cast<cudaStream_t>(stream));
+}
+
+namespace {
+
+bool operand_ok(const uint8_t* p) { return p && (reinterpret_cast<uintptr_t>(p) & 31) == 0; }
+
+// The job of x (rows x cols) with its operands, each one buffer of codes followed by scales, either of them absent
+QuantJob job_of(const void* x, int rows, int cols, int64_t row_stride, int64_t col_stride, int fmt, uint8_t* along_rows,
+                uint8_t* along_cols) {
+    QuantJob q = {};
+    q.x = x;
+    q.si = row_stride;
+    q.sj = cols == 1 ? 1 : col_stride;
+    q.groups = 1;
+    q.I = rows;
+    q.J = cols;
+    q.row_codes = along_rows;
+    if (along_rows) q.row_scales = along_rows + rows * code_pitch(fmt, cols);
+    q.col_codes = along_cols;
+    if (along_cols) q.col_scales = along_cols + cols * code_pitch(fmt, rows);
+    return q;
+}
+
+bool matrix_ok(const void* x, int dtype, int rows, int cols, int64_t rs, int64_t cs) {
+    return x && (dtype == OZK_F32 || dtype == OZK_F16 || dtype == OZK_BF16) && rows >= 1 && cols >= 1 &&
+           rows <= OZK_MX_KMAX && cols <= OZK_MX_KMAX && rs >= 0 && cs >= 0 && tile_count(1, rows, cols) > 0;
+}
+
+// C (m x n, contiguous) = A B^T for operands that are one buffer each
+int product(const uint8_t* A, const uint8_t* B, int fmt, int m, int n, int k, void* C, int dtype, int32_t* err,
+            ozk_stream_t stream) {
+    const long long pitch = code_pitch(fmt, k);
+    return ozk_mx_gemm(A, A + m * pitch, fmt, B, B + n * pitch, fmt, m, n, k, C, n, dtype, err, stream);
+}
+
+}  // namespace
+
+extern "C" int ozk_mx_quantize_both(const void* x, int dtype, int rows, int cols, int64_t row_stride, int64_t col_stride,
+                                    int fmt, int round_up, uint8_t* along_rows, uint8_t* along_cols,
+                                    ozk_stream_t stream) {
+    if (!matrix_ok(x, dtype, rows, cols, row_stride, col_stride) || !fmt_ok(fmt)) return OZK_ERR_ARG;
+    if (!operand_ok(along_rows) || !operand_ok(along_cols)) return OZK_ERR_ARG;
+    const QuantJob q = job_of(x, rows, cols, row_stride, col_stride, fmt, along_rows, along_cols);
+    return quantize(&q, 1, dtype, fmt, round_up != 0, reinterpret_cast<cudaStream_t>(stream));
+}
+
+extern "C" int ozk_mx_linear_forward(const void* x, int x_dtype, int64_t x_row_stride, int64_t x_col_stride, const void* w,
+                                     int w_dtype, int64_t w_row_stride, int64_t w_col_stride, int m, int n, int k, int fmt,
+                                     int round_up, uint8_t* x_along_k, uint8_t* w_along_k, uint8_t* x_along_m,
+                                     uint8_t* w_along_n, void* y, int32_t* err, ozk_stream_t stream) {
+    if (!matrix_ok(x, x_dtype, m, k, x_row_stride, x_col_stride) || !matrix_ok(w, w_dtype, n, k, w_row_stride, w_col_stride))
+        return OZK_ERR_ARG;
+    if (!fmt_ok(fmt) || !operand_ok(x_along_k) || !operand_ok(w_along_k) || !y || !err) return OZK_ERR_ARG;
+    if ((x_along_m && !operand_ok(x_along_m)) || (w_along_n && !operand_ok(w_along_n))) return OZK_ERR_ARG;
+    const QuantJob q[2] = {job_of(x, m, k, x_row_stride, x_col_stride, fmt, x_along_k, x_along_m),
+                           job_of(w, n, k, w_row_stride, w_col_stride, fmt, w_along_k, w_along_n)};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-#define OZK_QUANT(T)                                                                                                 \
-    (fmt == OZK_MX_E2M1                                                                                              \
-         ? launch_quantize<T, OZK_MX_E2M1>(static_cast<const T*>(x), groups, rows, k, group_stride, row_stride,      \
-                                           k_stride, round_up != 0, codes, scales, st)                               \
-         : launch_quantize<T, OZK_MX_E4M3>(static_cast<const T*>(x), groups, rows, k, group_stride, row_stride,      \
-                                           k_stride, round_up != 0, codes, scales, st))
-    switch (dtype) {
-        case OZK_F32: return OZK_QUANT(float);
-        case OZK_F16: return OZK_QUANT(__half);
-        case OZK_BF16: return OZK_QUANT(__nv_bfloat16);
-        default: return OZK_ERR_ARG;
+    int rc;
+    if (x_dtype == w_dtype) {
+        rc = quantize(q, 2, x_dtype, fmt, round_up != 0, st);
+    } else {
+        rc = quantize(q, 1, x_dtype, fmt, round_up != 0, st);
+        if (rc == OZK_OK) rc = quantize(q + 1, 1, w_dtype, fmt, round_up != 0, st);
     }
-#undef OZK_QUANT
+    return rc != OZK_OK ? rc : product(x_along_k, w_along_k, fmt, m, n, k, y, x_dtype, err, stream);
+}
+
+extern "C" int ozk_mx_linear_backward(const void* dy, int dy_dtype, int64_t dy_row_stride, int64_t dy_col_stride,
+                                      const uint8_t* x_along_m, const uint8_t* w_along_n, int m, int n, int k, int fmt,
+                                      int round_up, uint8_t* dy_along_n, uint8_t* dy_along_m, void* dx, int dx_dtype,
+                                      void* dw, int dw_dtype, int32_t* err, ozk_stream_t stream) {
+    if (!matrix_ok(dy, dy_dtype, m, n, dy_row_stride, dy_col_stride) || !fmt_ok(fmt) || k < 1 || k > OZK_MX_KMAX || !err)
+        return OZK_ERR_ARG;
+    if (!dx && !dw) return OZK_ERR_ARG;
+    if (dx && (!operand_ok(w_along_n) || !operand_ok(dy_along_n))) return OZK_ERR_ARG;
+    if (dw && (!operand_ok(x_along_m) || !operand_ok(dy_along_m))) return OZK_ERR_ARG;
+    const QuantJob q = job_of(dy, m, n, dy_row_stride, dy_col_stride, fmt, dx ? dy_along_n : nullptr, dw ? dy_along_m : nullptr);
+    int rc = quantize(&q, 1, dy_dtype, fmt, round_up != 0, reinterpret_cast<cudaStream_t>(stream));
+    if (rc == OZK_OK && dx) rc = product(dy_along_n, w_along_n, fmt, m, k, n, dx, dx_dtype, err, stream);
+    if (rc == OZK_OK && dw) rc = product(dy_along_m, x_along_m, fmt, n, k, m, dw, dw_dtype, err, stream);
+    return rc;
 }
 
 extern "C" int ozk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int fmt, int groups, int rows, int k,

@@ -33,30 +33,35 @@ MAX_GROUPS = 1024
 KMAX = 1 << 28
 _INT_MAX = 2 ** 31 - 1
 
+_current_device = torch._C._cuda_getDevice
+_stream_of = torch._C._cuda_getCurrentRawStream    # handle of a device's current stream
 _error_words = {}                # device index -> int32 word that the products' launches OR their flags into
+
+
+class _Devices(dict):
+    """torch.device objects by index, made once."""
+
+    def __missing__(self, index):
+        d = self[index] = torch.device("cuda", index)
+        return d
+
+
+_DEVICES = _Devices()
+
+
+def _operand_bytes(code, groups, rows, k):
+    """(bytes of the codes, a multiple of 64; bytes of codes and scales) of an operand."""
+    if not 1 <= k <= KMAX:
+        raise ValueError(f"contracted axis of length {k}: 1 to {KMAX} required")
+    kt, rt = -(-k // TILE), -(-rows // TILE)
+    if rows > _INT_MAX or groups * rt * kt > _INT_MAX:
+        raise ValueError(f"operand of {groups} x {rows} x {k} elements is too large")
+    codes = groups * rows * kt * (TILE if code else TILE // 2)
+    return codes, codes + groups * rt * kt * TILE_BYTES
 
 
 def _padded(k: int) -> int:
     return (k + TILE - 1) // TILE * TILE
-
-
-class _On:
-    """Makes ``device`` (an index) current for a launch if it is not, and gives its current stream's handle."""
-
-    __slots__ = ("device", "before")
-
-    def __init__(self, device):
-        self.device = device
-
-    def __enter__(self):
-        self.before = torch.cuda.current_device()
-        if self.before != self.device:
-            torch.cuda.set_device(self.device)
-        return torch._C._cuda_getCurrentRawStream(self.device)
-
-    def __exit__(self, *_):
-        if self.before != self.device:
-            torch.cuda.set_device(self.before)
 
 
 def _error_word(device: int):
@@ -119,20 +124,23 @@ class MXMatrix:
 
     def __init__(self, fmt, groups, rows, k, device: int):
         """An operand with uninitialised contents."""
-        self._fmt = _format(fmt)
-        g = 1 if groups is None else groups
-        if k < 1 or k > KMAX:
-            raise ValueError(f"contracted axis of length {k}: 1 to {KMAX} required")
-        if rows > _INT_MAX or g > _INT_MAX or g * -(-rows // TILE) * (_padded(k) // TILE) > _INT_MAX:
-            raise ValueError(f"operand of {g} x {rows} x {k} elements is too large")
-        self.fmt, self.groups, self.rows, self.k, self.device = fmt, groups, rows, k, device
-        kp = _padded(k)
-        self._code_bytes = g * rows * (kp // 2 if self._fmt == 0 else kp)
-        scale_bytes = g * -(-rows // TILE) * (kp // TILE) * TILE_BYTES
-        # one allocation: the codes (a multiple of 64 bytes), then the scales
-        self._buffer = torch.empty(self._code_bytes + scale_bytes, dtype=torch.uint8, device=torch.device("cuda", device))
-        self._code_ptr = self._buffer.data_ptr()
-        self._scale_ptr = self._code_ptr + self._code_bytes
+        code = _format(fmt)
+        code_bytes, total = _operand_bytes(code, 1 if groups is None else groups, rows, k)
+        self._take(fmt, code, groups, rows, k, device, code_bytes,
+                   torch.empty(total, dtype=torch.uint8, device=_DEVICES[device]))
+
+    def _take(self, fmt, code, groups, rows, k, device, code_bytes, buffer):
+        self.fmt, self._fmt, self.groups, self.rows, self.k, self.device = fmt, code, groups, rows, k, device
+        self._buffer, self._code_bytes = buffer, code_bytes
+        self._code_ptr = p = buffer.data_ptr()               # one allocation: the codes, then the scales
+        self._scale_ptr = p + code_bytes
+
+    @classmethod
+    def _over(cls, fmt, rows, k, device, buffer):
+        """The plain operand that ``buffer`` holds."""
+        out, code = object.__new__(cls), FORMATS[fmt]
+        out._take(fmt, code, None, rows, k, device, _operand_bytes(code, 1, rows, k)[0], buffer)
+        return out
 
     @property
     def shape(self):
@@ -195,12 +203,19 @@ class MXMatrix:
     def dequantize(self, dtype=torch.bfloat16):
         """The numbers the operand stands for, as a contiguous tensor (bfloat16 and float32 hold them exactly while
         their scales are ordinary)."""
-        d = _dtype(dtype, "dequantize")
-        out = torch.empty(self.shape, dtype=dtype, device=self._buffer.device)
-        if self.rows and self._g:
-            with _On(self.device) as stream:
-                check(_lib.lib().ozk_mx_dequantize(self._code_ptr, self._scale_ptr, self._fmt, self._g, self.rows,
-                                                   self.k, out.data_ptr(), d, stream), "ozk_mx_dequantize")
+        d = _DTYPES.get(dtype)
+        if d is None:
+            d = _dtype(dtype, "dequantize")
+        device = self.device
+        if _current_device() != device:
+            with torch.cuda.device(device):
+                return self.dequantize(dtype)
+        out = torch.empty(self.shape, dtype=dtype, device=_DEVICES[device])
+        if self.rows and self.groups != 0:
+            rc = _lib.lib().ozk_mx_dequantize(self._code_ptr, self._scale_ptr, self._fmt, self.groups or 1, self.rows,
+                                              self.k, out.data_ptr(), d, _stream_of(device))
+            if rc:
+                check(rc, "ozk_mx_dequantize")
         return out
 
 
@@ -214,7 +229,8 @@ def mx_quantize(x, fmt="e2m1", axis=-1, rule="floor"):
     number, ties to the even code."""
     d = _tensor(x, "x")
     code, up = _format(fmt), _rule(rule)
-    dim = x.dim()
+    shape, stride = x.shape, x.stride()
+    dim = len(shape)
     if dim not in (2, 3):
         raise ValueError(f"x: 2 or 3 axes required, not {dim}")
     if not -2 <= axis < dim:
@@ -222,18 +238,43 @@ def mx_quantize(x, fmt="e2m1", axis=-1, rule="floor"):
     at = axis % dim
     if at < dim - 2:
         raise ValueError("the groups of x cannot be contracted: axis is one of the last two")
+    device = x.get_device()
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return mx_quantize(x, fmt, axis, rule)
     other = 2 * dim - 3 - at
-    shape, stride = x.shape, x.stride()
     rows, k = shape[other], shape[at]
     groups = shape[0] if dim == 3 else None
-    device = x.device.index
     out = MXMatrix(fmt, groups, rows, k, device)
     if rows and groups != 0:
-        with _On(device) as stream:
-            check(_lib.lib().ozk_mx_quantize(x.data_ptr(), d, groups or 1, rows, k, stride[0] if dim == 3 else 0,
-                                             stride[other], stride[at], code, up, out._code_ptr, out._scale_ptr,
-                                             stream), "ozk_mx_quantize")
+        rc = _lib.lib().ozk_mx_quantize(x.data_ptr(), d, groups or 1, rows, k, stride[0] if dim == 3 else 0,
+                                        stride[other], stride[at], code, up, out._code_ptr, out._scale_ptr,
+                                        _stream_of(device))
+        if rc:
+            check(rc, "ozk_mx_quantize")
     return out
+
+
+def mx_quantize_both(x, fmt="e4m3", rule="floor"):
+    """(mx_quantize(x, fmt, -1, rule), mx_quantize(x, fmt, 0, rule)) of a matrix from one read of it: what a training
+    step needs of an operand whose two axes are contracted in turn."""
+    d = _tensor(x, "x")
+    code, up = _format(fmt), _rule(rule)
+    if x.dim() != 2:
+        raise ValueError(f"x: 2 axes required, not {x.dim()}")
+    device = x.get_device()
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return mx_quantize_both(x, fmt, rule)
+    rows, cols = x.shape
+    if not rows or not cols:
+        raise ValueError("x: both axes are contracted in turn and cannot be empty")
+    along_rows, along_cols = MXMatrix(fmt, None, rows, cols, device), MXMatrix(fmt, None, cols, rows, device)
+    rc = _lib.lib().ozk_mx_quantize_both(x.data_ptr(), d, rows, cols, x.stride(0), x.stride(1), code, up,
+                                         along_rows._code_ptr, along_cols._code_ptr, _stream_of(device))
+    if rc:
+        check(rc, "ozk_mx_quantize_both")
+    return along_rows, along_cols
 
 
 def _operands(A, B):
@@ -251,7 +292,7 @@ def _result(C, rows, cols, dtype, device):
     """The output tensor, its dtype code and row stride."""
     if C is None:
         d = _dtype(dtype, "dtype")
-        return torch.empty((rows, cols), dtype=dtype, device=torch.device("cuda", device)), d, max(cols, 1)
+        return torch.empty((rows, cols), dtype=dtype, device=_DEVICES[device]), d, cols or 1
     d = _tensor(C, "C")
     if C.device.index != device or tuple(C.shape) != (rows, cols) or (cols > 1 and C.stride(1) != 1) \
             or (rows > 1 and C.stride(0) < cols):
@@ -265,12 +306,16 @@ def mx_matmul(A, B, C=None, dtype=torch.bfloat16):
     _operands(A, B)
     if B.groups is not None:
         raise ValueError("B: a plain matrix required (see mx_grouped_matmul)")
-    C, d, ldc = _result(C, A.rows, B.rows, dtype, A.device)
+    device = A.device
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return mx_matmul(A, B, C, dtype)
+    C, d, ldc = _result(C, A.rows, B.rows, dtype, device)
     if A.rows and B.rows:
-        with _On(A.device) as stream:
-            check(_lib.lib().ozk_mx_gemm(A._code_ptr, A._scale_ptr, A._fmt, B._code_ptr, B._scale_ptr, B._fmt, A.rows,
-                                         B.rows, A.k, C.data_ptr(), ldc, d, _error_word(A.device), stream),
-                  "ozk_mx_gemm")
+        rc = _lib.lib().ozk_mx_gemm(A._code_ptr, A._scale_ptr, A._fmt, B._code_ptr, B._scale_ptr, B._fmt, A.rows, B.rows,
+                                    A.k, C.data_ptr(), ldc, d, _error_word(device), _stream_of(device))
+        if rc:
+            check(rc, "ozk_mx_gemm")
     return C
 
 
@@ -288,14 +333,18 @@ def mx_grouped_matmul(A, B, ends, C=None, dtype=torch.bfloat16):
     if not isinstance(ends, torch.Tensor) or ends.dtype != torch.int32 or ends.device != A._buffer.device \
             or tuple(ends.shape) != (B.groups,) or not ends.is_contiguous():
         raise ValueError(f"ends: contiguous int32 tensor of {B.groups} ends on cuda:{A.device} required")
+    device = A.device
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return mx_grouped_matmul(A, B, ends, C, dtype)
     fill = C is None
-    C, d, ldc = _result(C, A.rows, B.rows, dtype, A.device)
+    C, d, ldc = _result(C, A.rows, B.rows, dtype, device)
     if A.rows and B.rows:
-        with _On(A.device) as stream:
-            check(_lib.lib().ozk_mx_grouped_gemm(A._code_ptr, A._scale_ptr, A._fmt, B._code_ptr, B._scale_ptr, B._fmt,
-                                                 A.rows, B.rows, A.k, B.groups, ends.data_ptr(), int(fill),
-                                                 C.data_ptr(), ldc, d, _error_word(A.device), stream),
-                  "ozk_mx_grouped_gemm")
+        rc = _lib.lib().ozk_mx_grouped_gemm(A._code_ptr, A._scale_ptr, A._fmt, B._code_ptr, B._scale_ptr, B._fmt, A.rows,
+                                            B.rows, A.k, B.groups, ends.data_ptr(), fill, C.data_ptr(), ldc, d,
+                                            _error_word(device), _stream_of(device))
+        if rc:
+            check(rc, "ozk_mx_grouped_gemm")
     return C
 
 
@@ -305,64 +354,100 @@ def mx_rms_norm(x, weight, residual=None, eps=1e-6, fmt="e4m3", rule="floor"):
     rounded to the type of x and in its shape, or None without a residual)."""
     d = _tensor(x, "x")
     code, up = _format(fmt), _rule(rule)
-    if x.dim() < 1:
+    shape = x.shape
+    if not shape:
         raise ValueError("x: at least one axis required")
-    n = x.shape[-1]
-    if not isinstance(weight, torch.Tensor) or weight.device != x.device or tuple(weight.shape) != (n,) \
+    n = shape[-1]
+    if not isinstance(weight, torch.Tensor) or weight.device != x.device or weight.dim() != 1 or weight.shape[0] != n \
             or not (weight.dtype == x.dtype or weight.dtype == torch.float32) or not weight.is_contiguous():
         raise ValueError(f"weight: contiguous ({n},) tensor of x's type or float32 on its device required")
     if not 0.0 < eps < float("inf"):
         raise ValueError(f"eps {eps}: a positive number required")
-    x2 = x.reshape(-1, n) if n else x.reshape(0, 0)
-    if n and x2.stride(1) != 1 and n > 1:
-        x2 = x2.contiguous()
-    r2 = None
-    if residual is not None:
-        if not isinstance(residual, torch.Tensor) or residual.shape != x.shape or residual.dtype != x.dtype \
-                or residual.device != x.device:
-            raise ValueError("residual: a tensor of x's shape, type and device required")
-        r2 = residual.reshape(-1, n) if n else x2
-        if n > 1 and r2.stride(1) != 1:
-            r2 = r2.contiguous()
-    rows, device = x2.shape[0], x.device.index
+    if residual is not None and (not isinstance(residual, torch.Tensor) or residual.shape != shape
+                                 or residual.dtype != x.dtype or residual.device != x.device):
+        raise ValueError("residual: a tensor of x's shape, type and device required")
+    device = x.get_device()
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return mx_rms_norm(x, weight, residual, eps, fmt, rule)
+    x2 = _rows(x, n)
+    rows = x2.shape[0]
     out = MXMatrix(fmt, None, rows, n, device)
-    total = None if residual is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    r_ptr = r_stride = t_ptr = 0
+    total = None
+    if residual is not None:
+        r2 = _rows(residual, n)
+        r_ptr, r_stride = r2.data_ptr(), r2.stride(0)
+        total = torch.empty(shape, dtype=x.dtype, device=_DEVICES[device])
+        t_ptr = total.data_ptr()
     if rows:
-        with _On(device) as stream:
-            check(_lib.lib().ozk_mx_rms_norm(x2.data_ptr(), 0 if r2 is None else r2.data_ptr(), weight.data_ptr(), d,
-                                             int(weight.dtype == torch.float32), rows, n, x2.stride(0),
-                                             0 if r2 is None else r2.stride(0), eps, code, up,
-                                             0 if total is None else total.data_ptr(), out._code_ptr, out._scale_ptr,
-                                             stream), "ozk_mx_rms_norm")
+        rc = _lib.lib().ozk_mx_rms_norm(x2.data_ptr(), r_ptr, weight.data_ptr(), d, weight.dtype == torch.float32, rows,
+                                        n, x2.stride(0), r_stride, eps, code, up, t_ptr, out._code_ptr, out._scale_ptr,
+                                        _stream_of(device))
+        if rc:
+            check(rc, "ozk_mx_rms_norm")
     return out, total
+
+
+def _rows(x, n):
+    """x as a matrix of rows of length n >= 1 with contiguous elements: x itself or a view where it can be."""
+    if x.dim() != 2:
+        x = x.reshape(x.numel() // max(n, 1), n)
+    return x if n < 2 or x.stride(1) == 1 else x.contiguous()
+
+
+def _linear_forward(x2, weight, fmt, rule, need_dx, need_dw):
+    """y and the operands that the backward pass takes: x along its rows where dweight is wanted, weight along n where
+    dx is."""
+    device = x2.get_device()
+    m, k = x2.shape
+    n = weight.shape[0]
+    code = FORMATS[fmt]
+    xk, wk = _operand_bytes(code, 1, m, k)[1], _operand_bytes(code, 1, n, k)[1]
+    dev = _DEVICES[device]
+    y = torch.empty((m, n), dtype=x2.dtype, device=dev)
+    scratch = torch.empty(xk + wk, dtype=torch.uint8, device=dev)
+    xm = torch.empty(_operand_bytes(code, 1, k, m)[1], dtype=torch.uint8, device=dev) if need_dw else None
+    wn = torch.empty(_operand_bytes(code, 1, k, n)[1], dtype=torch.uint8, device=dev) if need_dx else None
+    p = scratch.data_ptr()
+    rc = _lib.lib().ozk_mx_linear_forward(x2.data_ptr(), _DTYPES[x2.dtype], *x2.stride(), weight.data_ptr(),
+                                          _DTYPES[weight.dtype], *weight.stride(), m, n, k, code, RULES[rule], p, p + xk,
+                                          xm.data_ptr() if need_dw else 0, wn.data_ptr() if need_dx else 0, y.data_ptr(),
+                                          _error_word(device), _stream_of(device))
+    if rc:
+        check(rc, "ozk_mx_linear_forward")
+    return y, xm, wn
 
 
 class _MXLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, fmt, rule):
-        x2 = x.reshape(-1, x.shape[-1])
-        ctx.save_for_backward(x2, weight)
-        ctx.how = (fmt, rule)
-        ctx.x_shape = x.shape
-        y = mx_matmul(mx_quantize(x2, fmt, rule=rule), mx_quantize(weight, fmt, rule=rule), dtype=x.dtype)
-        return y.view(*x.shape[:-1], weight.shape[0])
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        y, xm, wn = _linear_forward(x, weight, fmt, rule, need_dx, need_dw)
+        ctx.save_for_backward(xm, wn)
+        ctx.how = (fmt, rule, x.dtype, weight.dtype, weight.shape)
+        return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight = ctx.saved_tensors
-        fmt, rule = ctx.how
-        dy = dy.reshape(-1, dy.shape[-1])
-        dx = dw = None
-        if ctx.needs_input_grad[0]:
-            dx = mx_matmul(mx_quantize(dy, fmt, rule=rule), mx_quantize(weight, fmt, axis=0, rule=rule), dtype=x.dtype)
-            dx = dx.view(ctx.x_shape)
-        if ctx.needs_input_grad[1]:
-            if dy.shape[0]:
-                dw = mx_matmul(mx_quantize(dy, fmt, axis=0, rule=rule), mx_quantize(x, fmt, axis=0, rule=rule),
-                               dtype=weight.dtype)
-            else:
-                dw = torch.zeros_like(weight)
+        xm, wn = ctx.saved_tensors
+        fmt, rule, x_dtype, w_dtype, (n, k) = ctx.how
+        need_dx, need_dw = ctx.needs_input_grad[:2]
+        device, m = dy.get_device(), dy.shape[0]
+        code, dev = FORMATS[fmt], _DEVICES[device]
+        dx = torch.empty((m, k), dtype=x_dtype, device=dev) if need_dx else None
+        dw = torch.empty((n, k), dtype=w_dtype, device=dev) if need_dw else None
+        along_n, along_m = _operand_bytes(code, 1, m, n)[1], _operand_bytes(code, 1, n, m)[1]
+        scratch = torch.empty(along_n + along_m, dtype=torch.uint8, device=dev)
+        p = scratch.data_ptr()
+        rc = _lib.lib().ozk_mx_linear_backward(dy.data_ptr(), _DTYPES[dy.dtype], *dy.stride(),
+                                               xm.data_ptr() if need_dw else 0, wn.data_ptr() if need_dx else 0, m, n, k,
+                                               code, RULES[rule], p, p + along_n, dx.data_ptr() if need_dx else 0,
+                                               _DTYPES[x_dtype], dw.data_ptr() if need_dw else 0, _DTYPES[w_dtype],
+                                               _error_word(device), _stream_of(device))
+        if rc:
+            check(rc, "ozk_mx_linear_backward")
         return dx, dw, None, None
 
 
@@ -377,10 +462,25 @@ def mx_linear(x, weight, fmt="e4m3", rule="floor"):
     _tensor(weight, "weight")
     _format(fmt)
     _rule(rule)
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or x.device != weight.device:
-        raise ValueError(f"x (..., k) and weight (n, k) on one device required, not {tuple(x.shape)} and "
+    shape = x.shape
+    if weight.dim() != 2 or not shape or shape[-1] != weight.shape[1] or x.device != weight.device:
+        raise ValueError(f"x (..., k) and weight (n, k) on one device required, not {tuple(shape)} and "
                          f"{tuple(weight.shape)}")
-    return _MXLinear.apply(x, weight, fmt, rule)
+    n, k = weight.shape
+    device = x.get_device()
+    if _current_device() != device:
+        with torch.cuda.device(device):
+            return mx_linear(x, weight, fmt, rule)
+    for rows, length in ((x.numel() // max(k, 1), k), (n, k)):
+        _operand_bytes(0, 1, rows, length)                    # refuses an empty k and sizes beyond the operands'
+    if x.numel() == 0 or n == 0:
+        return torch.matmul(x, weight.t().to(x.dtype))        # nothing to multiply: empty, with its gradients of zero
+    x2 = x if len(shape) == 2 else x.reshape(-1, k)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        y = _MXLinear.apply(x2, weight, fmt, rule)
+    else:
+        y = _linear_forward(x2, weight, fmt, rule, False, False)[0]
+    return y if len(shape) == 2 else y.view(*shape[:-1], n)
 
 
-__all__ = ["MXMatrix", "mx_quantize", "mx_matmul", "mx_grouped_matmul", "mx_rms_norm", "mx_linear", "mx_check_errors"]
+__all__ = ["MXMatrix", "mx_quantize", "mx_quantize_both", "mx_matmul", "mx_grouped_matmul", "mx_rms_norm", "mx_linear", "mx_check_errors"]

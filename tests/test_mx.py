@@ -149,6 +149,19 @@ def test_quantize_strides(pkg, name):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("fmt", FMTS)
+def test_quantize_both(pkg, name, fmt):
+    """Both operands from one read equal the two quantisations, aligned or not."""
+    rng = np.random.default_rng(22)
+    base = _put(_values(rng, (300, 264)), name)
+    for v in (base, base[:, :200], base[:1], base[:, :1], base[:129, 8:137], base[:, 1:], base.T, base[5, 7].expand(33, 65)):
+        a, b = pkg.mx_quantize_both(v, fmt, rule="ceil")
+        _same(a, _f64(v), fmt, "ceil")
+        _same(b, _f64(v).T, fmt, "ceil")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fmt", FMTS)
 def test_quantize_special_values(pkg, fmt):
     """NaN, infinities, the largest and smallest numbers of each type, negative zero, exact ties, saturation."""
@@ -468,6 +481,10 @@ def test_rms_norm_views(pkg):
     q, _ = pkg.mx_rms_norm(x, w)
     got = _f64(q.dequantize())
     assert np.isnan(got[2]).all() and np.isfinite(got[[0, 1, 4, 5]]).all() and np.isnan(got[3, :32]).all()
+    big = torch.full((2, 96), 1e30, device="cuda")             # squares beyond FP32
+    big[0, :48] = -3e25
+    q, _ = pkg.mx_rms_norm(big, w)
+    _near_codes(q, _norm_want(_f64(big), _f64(w), None, 1e-6)[1], "e4m3", "floor")
     q, s = pkg.mx_rms_norm(torch.empty(0, 64, device="cuda"), torch.ones(64, device="cuda"),
                            residual=torch.empty(0, 64, device="cuda"))
     assert q.shape == (0, 64) and s.shape == (0, 64)
@@ -700,7 +717,8 @@ def test_python_refusals(pkg):
            lambda: pkg.mx_rms_norm(x, w, eps=float("nan")), lambda: pkg.mx_rms_norm(x, w, residual=x[:4]),
            lambda: pkg.mx_rms_norm(x, w, residual=x.half()), lambda: pkg.mx_rms_norm(x, w, fmt="fp8"),
            lambda: pkg.mx_rms_norm(x.double(), w), lambda: pkg.mx_linear(x, w), lambda: pkg.mx_linear(x, x[:, :32]),
-           lambda: pkg.mx_linear(x, x.double()), lambda: pkg.mx_linear(x, x, fmt="int8"),
+           lambda: pkg.mx_linear(x, x.double()), lambda: pkg.mx_linear(x[:, :0], x[:, :0]),
+           lambda: pkg.mx_quantize_both(x[:0]), lambda: pkg.mx_quantize_both(x[0]), lambda: pkg.mx_quantize_both(x, "int4"), lambda: pkg.mx_linear(x, x, fmt="int8"),
            lambda: pkg.MXMatrix.from_codes(codes, scales[:, :1], "e2m1"), lambda: pkg.MXMatrix.from_codes(codes, scales, "e4m3"),
            lambda: pkg.MXMatrix.from_codes(codes, scales, "e2m1", 62), lambda: pkg.MXMatrix.from_codes(codes.int(), scales, "e2m1"),
            lambda: pkg.MXMatrix.from_codes(codes.cpu(), scales, "e2m1")]
