@@ -5,14 +5,17 @@
 // (K = 32; a 4-bit operand is spread to one code a byte by its TMA load).
 //
 // One persistent kernel, one CTA per SM:
-//   - warp 0 (one lane): producer; a stage is 128 bytes of K of 128 "left" rows (M) and BN "right" rows (N) by TMA with
-//     the 128-byte swizzle, and their scale tiles by contiguous bulk copies;
-//   - warp 1 (one lane): lays a stage's scales into TMEM (tcgen05.cp, in order with the MMAs that use them, two buffers
-//     of columns) and issues the four MMAs of the stage;
+//   - warp 0 (one lane): producer; a stage is 128 bytes of K of 128 "left" rows (M) and BN "right" rows (N) and their
+//     scale tiles, four TMA loads, the codes with the 128-byte swizzle;
+//   - warp 1 (one lane): lays a stage's scales into TMEM (tcgen05.cp, two buffers of columns), a stage ahead of the four
+//     MMAs that use them, and issues those;
 //   - warps 2..9: epilogue, TMEM -> registers -> one rounding -> C.
 // Left is A and right is B (`SWAP` false), or, for few rows of A, left is B and right is A: the 128 rows that the
 // instruction has at least are then rows of B, which there are plenty of, and A's tile is as small as 32 rows; C^T comes
 // out of TMEM, whose lanes are then neighbours in a row of C.
+// `PAIR`: two CTAs on neighbouring SMs share a 256 x 256 tile (cta_group::2): each holds 128 left rows and 128 right rows,
+// so a stage of the same work brings 32 KB of codes to an SM instead of 48 KB.  One CTA alone is bound by its shared
+// memory: 48 KB written and read at 128 bytes a clock is 768 clocks a stage, the MMAs need 512.
 // Where there are fewer tiles than SMs, a cluster of CTAs shares one tile: each takes a part of K, leaves its FP32 sums
 // in its shared memory, and every CTA adds one slice of the tile over the cluster in a fixed order (no workspace, no
 // atomics, one launch).
@@ -44,11 +47,14 @@ constexpr int MXF4 = 0, MXF8F6F4 = 1;
 constexpr size_t SMEM_MAX = 232448;
 constexpr size_t TABLE_BYTES = (2 * (OZK_MX_MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
 
-template <int KIND, int BN>
+template <int KIND, int BN, bool PAIR>
 struct Shape {
+    static constexpr int CTAS = PAIR ? 2 : 1;
+    static constexpr int BL = BM * CTAS;                        // left rows of a tile
+    static constexpr int RN = BN / CTAS;                        // right rows that one CTA loads
     static constexpr int KT = KIND == MXF4 ? 2 : 1;             // scale tiles (128 elements of K) of a stage
     static constexpr int SUBS = (BN + TILE - 1) / TILE;         // row tiles of the right operand's scales
-    static constexpr uint32_t L_BYTES = BM * ROW_BYTES, R_BYTES = BN * ROW_BYTES;
+    static constexpr uint32_t L_BYTES = BM * ROW_BYTES, R_BYTES = RN * ROW_BYTES;
     static constexpr uint32_t SL_BYTES = KT * TILE_BYTES, SR_BYTES = SUBS * KT * TILE_BYTES;
     static constexpr uint32_t STAGE_BYTES = L_BYTES + R_BYTES + SL_BYTES + SR_BYTES;
     static constexpr int FIT = (int)((SMEM_MAX - 1024 - 256 - TABLE_BYTES) / STAGE_BYTES);
@@ -66,16 +72,15 @@ struct Shape {
     static constexpr int HALF = BN / 2;                         // accumulator columns of one epilogue warp
     static constexpr int CHUNK = HALF < 32 ? HALF : 32;
     static_assert(USED <= 512 && NUM_BARS * 8 + 16 <= 256 && STAGES >= 3, "fits");
-    static_assert((size_t)BN * BM * 4 <= (size_t)STAGES * STAGE_BYTES, "a tile of partial sums fits into the stages");
+    static_assert(PAIR || (size_t)(BN + 4) * BM * 4 <= (size_t)STAGES * STAGE_BYTES, "a tile of partial sums fits into the stages");
+    static_assert(!PAIR || BN == 256, "a pair's tile is 256 x 256");
 };
 
 struct Args {
-    const uint8_t *sl, *sr;                  // scales of the left and right operand
-    long long sl_group, sr_group;            // bytes of one group of them
     int l_rows, r_rows;                      // rows (per group) of the left and right operand
     int ktiles;                              // scale tiles along K
     int kblocks;                             // stages along K
-    uint32_t load_bytes;                     // what the two TMA loads of a stage count on its barrier
+    uint32_t load_bytes;                     // what the loads of a stage count on its barrier
     int groups;                              // 0: no groups
     const int32_t* ends;
     int tokens, n;                           // rows and columns of C
@@ -94,7 +99,7 @@ struct Unit {
     int first, last;                         // rows of A (and C) that belong to this unit's group: [first, last)
 };
 
-template <int BN, bool SWAP>
+template <int BL, int BN, bool SWAP>
 struct Work {
     const Args& a;
     const int *pre, *bound;                  // grouped: windows before group g, first row of group g
@@ -102,7 +107,7 @@ struct Work {
     long long units;
 
     __device__ Work(const Args& a_, const int* pre_, const int* bound_) : a(a_), pre(pre_), bound(bound_) {
-        ltiles = (a.l_rows + BM - 1) / BM;
+        ltiles = (a.l_rows + BL - 1) / BL;
         rtiles = (a.r_rows + BN - 1) / BN;
         units = a.groups ? (long long)pre[a.groups] * (SWAP ? ltiles : rtiles) : (long long)ltiles * rtiles;
     }
@@ -120,7 +125,7 @@ struct Work {
             w.last = bound[lo + 1];
             const long long in = u - (long long)pre[lo] * other;
             const int nw = pre[lo + 1] - pre[lo];
-            const int win = w.first / (SWAP ? BN : BM) + (int)(in % nw), o = (int)(in / nw);
+            const int win = w.first / (SWAP ? BN : BL) + (int)(in % nw), o = (int)(in / nw);
             w.lt = SWAP ? o : win;
             w.rt = SWAP ? win : o;
             w.lg = SWAP ? lo : 0;
@@ -159,7 +164,23 @@ __device__ __forceinline__ void store1(void* C, long long at, float v, int dtype
     else static_cast<__half*>(C)[at] = __float2half_rn(v);
 }
 
-// One thread's CHUNK consecutive accumulator columns (`r` the first one's right row, `l` the lane's left row) to C
+// Four words of 32 bytes that a pair of lanes holds for two rows of C: the even lane's row gets both lanes' low or high
+// half in one store, then the odd lane's, so that every store of the warp fills whole 32-byte sectors.
+__device__ __forceinline__ void store_pair(uint8_t* even_row, uint8_t* odd_row, bool even_in, bool odd_in, bool odd_lane,
+                                           const uint32_t (&w)[8]) {
+    uint4 own, got;
+    own.x = odd_lane ? w[4] : w[0]; own.y = odd_lane ? w[5] : w[1]; own.z = odd_lane ? w[6] : w[2]; own.w = odd_lane ? w[7] : w[3];
+    got.x = __shfl_xor_sync(0xffffffffu, odd_lane ? w[0] : w[4], 1);
+    got.y = __shfl_xor_sync(0xffffffffu, odd_lane ? w[1] : w[5], 1);
+    got.z = __shfl_xor_sync(0xffffffffu, odd_lane ? w[2] : w[6], 1);
+    got.w = __shfl_xor_sync(0xffffffffu, odd_lane ? w[3] : w[7], 1);
+    const int at = odd_lane ? 16 : 0;
+    if (even_in) *reinterpret_cast<uint4*>(even_row + at) = odd_lane ? got : own;
+    if (odd_in) *reinterpret_cast<uint4*>(odd_row + at) = odd_lane ? own : got;
+}
+
+// One thread's CHUNK consecutive accumulator columns (`r` the first one's right row, `l` the lane's left row) to C; called
+// by whole warps
 template <int CHUNK, bool SWAP>
 __device__ __forceinline__ void store_chunk(const Args& a, const Unit& w, int l, int r, const uint32_t (&v)[CHUNK]) {
     if (SWAP) {                              // l: column of C, r: row of C; the warp's lanes are neighbours in a row
@@ -170,28 +191,49 @@ __device__ __forceinline__ void store_chunk(const Args& a, const Unit& w, int l,
                 store1(a.C, (long long)(r + e) * a.ldc + l, __uint_as_float(v[e]), a.dtype);
         return;
     }
-    if (l < w.first || l >= w.last || r >= a.n) return;
-    const long long at = (long long)l * a.ldc + r;
+    if (r >= a.n) return;
     if (a.vec && r + CHUNK <= a.n) {
+        const int le = l & ~1, lo = l | 1, size = a.dtype == OZK_F32 ? 4 : 2;
+        const bool even_in = le >= w.first && le < w.last, odd_in = lo >= w.first && lo < w.last, odd_lane = l & 1;
+        uint8_t* pe = static_cast<uint8_t*>(a.C) + ((long long)le * a.ldc + r) * size;
+        uint8_t* po = pe + a.ldc * size;
         if (a.dtype == OZK_F32) {
-            uint4* d = reinterpret_cast<uint4*>(static_cast<float*>(a.C) + at);
-#pragma unroll
-            for (int q = 0; q < CHUNK / 4; q++) d[q] = make_uint4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
-        } else {
-            uint4* d = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.C) + at);
 #pragma unroll
             for (int q = 0; q < CHUNK / 8; q++) {
-                uint32_t p[4];
+                uint32_t p[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    p[j] = pack2(__uint_as_float(v[8 * q + 2 * j]), __uint_as_float(v[8 * q + 2 * j + 1]), a.dtype);
-                d[q] = make_uint4(p[0], p[1], p[2], p[3]);
+                for (int j = 0; j < 8; j++) p[j] = v[8 * q + j];
+                store_pair(pe + 32 * q, po + 32 * q, even_in, odd_in, odd_lane, p);
+            }
+        } else {
+#pragma unroll
+            for (int q = 0; q < CHUNK / 16; q++) {
+                uint32_t p[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    p[j] = pack2(__uint_as_float(v[16 * q + 2 * j]), __uint_as_float(v[16 * q + 2 * j + 1]), a.dtype);
+                store_pair(pe + 32 * q, po + 32 * q, even_in, odd_in, odd_lane, p);
             }
         }
-    } else {
+    } else if (l >= w.first && l < w.last) {
+        const long long at = (long long)l * a.ldc + r;
 #pragma unroll
         for (int e = 0; e < CHUNK; e++)
             if (r + e < a.n) store1(a.C, at + e, __uint_as_float(v[e]), a.dtype);
+    }
+}
+
+// Four neighbouring values of a row of C
+__device__ __forceinline__ void store4(const Args& a, int token, int col, float4 s) {
+    const long long at = (long long)token * a.ldc + col;
+    if (a.vec && col + 4 <= a.n) {
+        if (a.dtype == OZK_F32) *reinterpret_cast<float4*>(static_cast<float*>(a.C) + at) = s;
+        else *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.C) + at) = make_uint2(pack2(s.x, s.y, a.dtype), pack2(s.z, s.w, a.dtype));
+    } else {
+        const float f[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (col + e < a.n) store1(a.C, at + e, f[e], a.dtype);
     }
 }
 
@@ -230,11 +272,12 @@ __device__ __forceinline__ void tmem_ld_chunk(uint32_t taddr, uint32_t (&v)[CHUN
     else tmem_ld_32x32b_x16(taddr, v);
 }
 
-template <int KIND, int BN, bool SWAP>
+template <int KIND, int BN, bool SWAP, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmR,
+                   const __grid_constant__ CUtensorMap tmSL, const __grid_constant__ CUtensorMap tmSR,
                    const __grid_constant__ Args a, int parts) {
-    using S = Shape<KIND, BN>;
+    using S = Shape<KIND, BN, PAIR>;
     constexpr int STAGES = S::STAGES, CHUNK = S::CHUNK;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -258,27 +301,38 @@ __global__ void __launch_bounds__(THREADS, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < STAGES; s++) { mbar_init(full_bar(s), 1); mbar_init(empty_bar(s), 1); }
-        for (int b = 0; b < 2; b++) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), EPI_WARPS); }
+        for (int b = 0; b < 2; b++) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), S::CTAS * EPI_WARPS); }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
         mbar_fence_init();
         tma_prefetch_desc(&tmL);
         tma_prefetch_desc(&tmR);
+        tma_prefetch_desc(&tmSL);
+        tma_prefetch_desc(&tmSR);
     }
     if (warp == 1) {
-        tmem_alloc(smem_addr(tmem_slot), S::TMEM_COLS);
-        tmem_relinquish();
+        if (PAIR) {
+            tmem_alloc_pair(smem_addr(tmem_slot), S::TMEM_COLS);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(smem_addr(tmem_slot), S::TMEM_COLS);
+            tmem_relinquish();
+        }
     }
-    if (warp == 2 && a.groups) group_tables<SWAP ? BN : BM>(a, pre, bound, lane);
+    if (warp == 2 && a.groups) group_tables<SWAP ? BN : S::BL>(a, pre, bound, lane);
+    __syncwarp();
     tc_fence_before();
     __syncthreads();
+    if (PAIR) cluster_sync();                  // the peer's barriers exist before any remote arrival
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const Work<BN, SWAP> work(a, pre, bound);
-    // parts > 1: one unit per cluster of `parts` CTAs, each with its part of K; else units round robin over the grid
-    const int part = parts > 1 ? (int)cluster_ctarank() : 0;
-    const long long u0 = blockIdx.x / parts, du = gridDim.x / parts;
+    const Work<S::BL, BN, SWAP> work(a, pre, bound);
+    // parts > 1: one unit per cluster of `parts` CTAs, each with its part of K; else units round robin over the CTAs, or
+    // over the pairs, of which CTA 0 issues the MMAs
+    const int rank = PAIR ? (int)cluster_ctarank() : 0;
+    const int part = !PAIR && parts > 1 ? (int)cluster_ctarank() : 0;
+    const long long u0 = blockIdx.x / (parts * S::CTAS), du = gridDim.x / (parts * S::CTAS);
     const int kb0 = (int)((long long)a.kblocks * part / parts), kb1 = (int)((long long)a.kblocks * (part + 1) / parts);
 
     if (warp == 0) {
@@ -290,33 +344,36 @@ __global__ void __launch_bounds__(THREADS, 1)
             bool ok = true;
             for (long long u = u0; ok && u < work.units; u += du) {
                 const Unit w = work.at(u);
-                const int r_tile = w.rt * BN / TILE;
-                const int subs = min(S::SUBS, row_tiles(a.r_rows) - r_tile);
-                const uint8_t* gl = a.sl + w.lg * a.sl_group + (long long)w.lt * a.ktiles * TILE_BYTES;
-                const uint8_t* gr = a.sr + w.rg * a.sr_group + (long long)r_tile * a.ktiles * TILE_BYTES;
                 for (int kb = kb0; kb < kb1; kb++) {
                     if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
                         if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_PRODUCER);
                         ok = false;
                         break;
                     }
-                    const uint32_t sb = (uint32_t)min(S::KT, a.ktiles - kb * S::KT) * TILE_BYTES;
-                    const uint32_t bar = full_bar(stage);
-                    mbar_arrive_expect_tx(bar, a.load_bytes + sb * (uint32_t)(1 + subs));
+                    // a pair's loads all complete on CTA 0's barrier, which expects the bytes of both
+                    if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), a.load_bytes * (uint32_t)S::CTAS);
+                    const uint32_t bar = PAIR ? map_to_rank(full_bar(stage), 0u) : full_bar(stage);
                     const int kc = kb * (KIND == MXF4 ? ROW_BYTES : TILE);      // bytes (mxf4) or elements
-                    tma_load_3d(smem_addr(sL + stage * S::L_BYTES), &tmL, kc, w.lt * BM, w.lg, bar);
-                    tma_load_3d(smem_addr(sR + stage * S::R_BYTES), &tmR, kc, w.rt * BN, w.rg, bar);
-                    const long long so = (long long)kb * S::KT * TILE_BYTES;
-                    bulk_load(smem_addr(sSL + stage * S::SL_BYTES), gl + so, sb, bar);
-                    for (int i = 0; i < subs; i++)
-                        bulk_load(smem_addr(sSR + stage * S::SR_BYTES + i * S::SL_BYTES),
-                                  gr + (long long)i * a.ktiles * TILE_BYTES + so, sb, bar);
+                    const int l0 = w.lt * S::BL + rank * BM, r0 = w.rt * BN + rank * S::RN;
+                    const uint32_t dl = smem_addr(sL + stage * S::L_BYTES), dr = smem_addr(sR + stage * S::R_BYTES);
+                    const uint32_t dsl = smem_addr(sSL + stage * S::SL_BYTES), dsr = smem_addr(sSR + stage * S::SR_BYTES);
+                    if (PAIR) {
+                        tma_load_3d_pair(dl, &tmL, kc, l0, w.lg, bar);
+                        tma_load_3d_pair(dr, &tmR, kc, r0, w.rg, bar);
+                        tma_load_4d_pair(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, w.lg, bar);
+                        tma_load_4d_pair(dsr, &tmSR, 0, kb * S::KT, w.rt * BN / TILE, w.rg, bar);
+                    } else {
+                        tma_load_3d(dl, &tmL, kc, l0, w.lg, bar);
+                        tma_load_3d(dr, &tmR, kc, r0, w.rg, bar);
+                        tma_load_4d(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, w.lg, bar);
+                        tma_load_4d(dsr, &tmSR, 0, kb * S::KT, w.rt * BN / TILE, w.rg, bar);
+                    }
                     issued++;
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
-            if (!ok) {
-                // let the loads already issued land before the CTA exits (bounded)
+            if (!ok && rank == 0) {
+                // let the loads already issued land before the CTA (or the pair) exits (bounded)
                 const long long first = issued > STAGES ? issued - STAGES : 0;
                 for (long long j = first; j < issued; j++) {
                     int dummy = 0;
@@ -325,11 +382,19 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0) {
+        if (lane == 0 && rank == 0) {
             // ------------------------------------------------------------ scales to TMEM, MMAs
-            int stage = 0;
+            int stage = 0, before = 0;
             uint32_t phase = 0, it = 0, step = 0;
             bool ok = true, issued_any = false;
+            auto commit = [&](uint32_t bar) {      // an arrival on that barrier of every CTA when all issued so far is done
+                if (PAIR) {
+                    umma_commit_pair(map_to_rank(bar, 0u));
+                    umma_commit_pair(map_to_rank(bar, 1u));
+                } else {
+                    umma_commit(bar);
+                }
+            };
             for (long long u = u0; ok && u < work.units; u += du) {
                 const Unit w = work.at(u);
                 const int b = (int)(it & 1u);
@@ -347,6 +412,28 @@ __global__ void __launch_bounds__(THREADS, 1)
                 // the second tile of 64 right rows in a scale tile starts two columns on (32 rows a column; an MMA takes
                 // its scales from an even column, so tiles of 32 rows exist for a first tile only)
                 const uint32_t r_col = BN == 64 ? (uint32_t)(w.rt & 1) * 2u : 0u;
+                auto columns = [&](uint32_t st) { return tmem_base + (uint32_t)(S::SCALE_BASE + (int)(st & 1u) * S::SCALE_COLS); };
+                // the four instructions of a stage: 32 bytes along K inside the swizzle atom each (+2 in the >> 4 address
+                // field); the last stage of an odd number of scale tiles has half of them
+                auto multiply = [&](int sg, uint32_t st, int kb) {
+                    const uint64_t ld = umma_desc_sw128(smem_addr(sL + sg * S::L_BYTES));
+                    const uint64_t rd = umma_desc_sw128(smem_addr(sR + sg * S::R_BYTES));
+                    const uint32_t tl = columns(st), tr = tl + (uint32_t)(4 * S::KT);
+                    const int tiles = min(S::KT, a.ktiles - kb * S::KT);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) {
+                        const int t = KIND == MXF4 ? kk >> 1 : 0;
+                        if (t >= tiles) break;
+                        const uint32_t idesc = a.idesc | umma_idesc_scale_id(KIND == MXF4 ? 2u * (kk & 1) : (uint32_t)kk);
+                        const uint32_t acc = (kb > kb0 || kk > 0) ? 1u : 0u;
+                        const uint32_t ca = tl + 4u * t, cb = tr + 4u * (uint32_t)(t * S::SUBS) + r_col;
+                        if (KIND == MXF4 && PAIR) umma_mxf4_pair(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
+                        else if (KIND == MXF4) umma_mxf4(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
+                        else if (PAIR) umma_mxf8f6f4_pair(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
+                        else umma_mxf8f6f4(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
+                    }
+                    commit(empty_bar(sg));
+                };
                 for (int kb = kb0; kb < kb1; kb++) {
                     if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
                         if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_MMA);
@@ -354,42 +441,35 @@ __global__ void __launch_bounds__(THREADS, 1)
                         break;
                     }
                     tc_fence_after();
-                    const int tiles = min(S::KT, a.ktiles - kb * S::KT);
-                    const uint32_t tl = tmem_base + (uint32_t)(S::SCALE_BASE + (int)(step & 1u) * S::SCALE_COLS);
-                    const uint32_t tr = tl + (uint32_t)(4 * S::KT);
-                    for (int t = 0; t < tiles; t++) {
-                        tmem_cp_scales(tl + 4u * t, smem_desc_scales(smem_addr(sSL + stage * S::SL_BYTES + t * TILE_BYTES)));
+                    const uint32_t tl = columns(step), tr = tl + (uint32_t)(4 * S::KT);
 #pragma unroll
-                        for (int i = 0; i < S::SUBS; i++)
-                            tmem_cp_scales(tr + 4u * (uint32_t)(t * S::SUBS + i),
-                                           smem_desc_scales(smem_addr(sSR + stage * S::SR_BYTES + i * S::SL_BYTES + t * TILE_BYTES)));
-                    }
-                    const uint64_t ld = umma_desc_sw128(smem_addr(sL + stage * S::L_BYTES));
-                    const uint64_t rd = umma_desc_sw128(smem_addr(sR + stage * S::R_BYTES));
-                    // four instructions of 32 bytes along K inside the swizzle atom (+2 in the >> 4 address field)
+                    for (int t = 0; t < S::KT; t++) {
+                        const uint64_t dl = smem_desc_scales(smem_addr(sSL + stage * S::SL_BYTES + t * TILE_BYTES));
+                        if (PAIR) tmem_cp_scales_pair(tl + 4u * t, dl);
+                        else tmem_cp_scales(tl + 4u * t, dl);
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++) {
-                        const int t = KIND == MXF4 ? kk >> 1 : 0;
-                        if (t >= tiles) break;
-                        const uint32_t id = KIND == MXF4 ? 2u * (kk & 1) : (uint32_t)kk;
-                        const uint32_t idesc = a.idesc | umma_idesc_scale_id(id);
-                        const uint32_t acc = (kb > kb0 || kk > 0) ? 1u : 0u;
-                        const uint32_t ca = tl + 4u * t, cb = tr + 4u * (uint32_t)(t * S::SUBS) + r_col;
-                        if (KIND == MXF4) umma_mxf4(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
-                        else umma_mxf8f6f4(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
+                        for (int i = 0; i < S::SUBS; i++) {
+                            const uint64_t dr = smem_desc_scales(smem_addr(sSR + stage * S::SR_BYTES + i * S::SL_BYTES + t * TILE_BYTES));
+                            const uint32_t to = tr + 4u * (uint32_t)(t * S::SUBS + i);
+                            if (PAIR) tmem_cp_scales_pair(to, dr);
+                            else tmem_cp_scales(to, dr);
+                        }
                     }
                     issued_any = true;
+                    if (kb > kb0) multiply(before, step - 1u, kb - 1);
+                    before = stage;
                     step++;
-                    umma_commit(empty_bar(stage));
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
-                umma_commit(accf_bar(b));
+                multiply(before, step - 1u, kb1 - 1);
+                commit(accf_bar(b));
                 it++;
             }
             if (!ok && issued_any) {
                 // all MMAs issued by this thread must finish before TMEM is released
-                umma_commit(drain_bar);
+                if (PAIR) umma_commit_pair(map_to_rank(drain_bar, 0u));
+                else umma_commit(drain_bar);
                 int dummy = 0;
                 mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
             }
@@ -402,6 +482,10 @@ __global__ void __launch_bounds__(THREADS, 1)
         constexpr int NCH = S::HALF / CHUNK;
         uint32_t it = 0;
         bool ok = true;
+        auto drained = [&](int b) {            // one arrival a warp, on the barrier that the issuing CTA waits for
+            if (PAIR) mbar_arrive_cluster(map_to_rank(acce_bar(b), 0u));
+            else mbar_arrive(acce_bar(b));
+        };
         for (long long u = u0; ok && u < work.units; u += du) {
             const Unit w = work.at(u);
             const int b = (int)(it & 1u);
@@ -412,19 +496,25 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             __syncwarp();
             tc_fence_after();
-            const int l = w.lt * BM + quarter * 32 + lane;
+            const int l = w.lt * S::BL + rank * BM + quarter * 32 + lane;
             const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * S::ACC_STRIDE + half * S::HALF);
             const int r = w.rt * BN + half * S::HALF;
-            if (parts > 1) {
+            if (!PAIR && parts > 1) {
                 float* mine = reinterpret_cast<float*>(smem);
 #pragma unroll 1
                 for (int c = 0; c < NCH; c++) {
                     uint32_t v[CHUNK];
                     tmem_ld_chunk<CHUNK>(acc + (uint32_t)(c * CHUNK), v);
                     tmem_wait_ld();
+                    const int row = quarter * 32 + lane, col = half * S::HALF + c * CHUNK;
+                    if (SWAP) {                // [column][row]: rows are neighbours in C
 #pragma unroll
-                    for (int e = 0; e < CHUNK; e++)
-                        mine[(half * S::HALF + c * CHUNK + e) * BM + quarter * 32 + lane] = __uint_as_float(v[e]);
+                        for (int e = 0; e < CHUNK; e++) mine[(col + e) * BM + row] = __uint_as_float(v[e]);
+                    } else {                   // [row][column], four words of padding
+#pragma unroll
+                        for (int e = 0; e < CHUNK; e += 4)
+                            *reinterpret_cast<uint4*>(mine + row * (BN + 4) + col + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
+                    }
                 }
             } else if (S::LAG == 1) {
                 // the columns shared with the other accumulator: the last 48 of buffer 0, the first 48 of buffer 1
@@ -432,7 +522,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int c0 = b == 0 ? NCH - 1 : 0, dc = b == 0 ? -1 : 1;
                 uint32_t v0[CHUNK], v1[CHUNK];
                 if (!shared_half) {
-                    if (lane == 0) mbar_arrive(acce_bar(0));
+                    if (lane == 0) drained(0);
                 }
 #pragma unroll 1
                 for (int c = 0; c < NCH; c += 2) {
@@ -443,7 +533,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (c == 0 && shared_half) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(acce_bar(0));
+                        if (lane == 0) drained(0);
                     }
                     store_chunk<CHUNK, SWAP>(a, w, l, r + ca * CHUNK, v0);
                     store_chunk<CHUNK, SWAP>(a, w, l, r + cb * CHUNK, v1);
@@ -459,7 +549,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (c == NCH - 1) {
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(acce_bar(b));
+                        if (lane == 0) drained(b);
                     }
                     store_chunk<CHUNK, SWAP>(a, w, l, r + c * CHUNK, v);
                 }
@@ -481,34 +571,45 @@ __global__ void __launch_bounds__(THREADS, 1)
         }
     }
 
-    if (parts > 1) {
-        // add one slice of the tile's columns over the cluster, CTA 0's sums first
+    if (!PAIR && parts > 1) {
+        // add one slice of the tile over the cluster, four values a thread, CTA 0's sums first
         __syncwarp();
         cluster_sync();
         if (warp >= 2 && u0 < work.units && !*abort_flag) {
             const Unit w = work.at(u0);
-            const int row = (threadIdx.x - 64) & (BM - 1);
-            const int c0 = BN * part / parts, c1 = BN * (part + 1) / parts;
-            const uint32_t base = smem_addr(smem) + 4u * (uint32_t)row;
-            for (int c = c0 + ((threadIdx.x - 64) >> 7); c < c1; c += EPI_WARPS * 32 / BM) {
-                float sum = 0.0f;
-                for (int q = 0; q < parts; q++)
-                    sum += ld_cluster_f32(map_to_rank(base + 4u * (uint32_t)(c * BM), (uint32_t)q));
-                const int l = w.lt * BM + row, r = w.rt * BN + c;
-                const int token = SWAP ? r : l, col = SWAP ? l : r;
-                if (token >= w.first && token < w.last && col < a.n)
-                    store1(a.C, (long long)token * a.ldc + col, sum, a.dtype);
+            constexpr int LINE = SWAP ? BM : BN, LINES = SWAP ? BN : BM, PITCH = SWAP ? BM : BN + 4;
+            constexpr int QUADS = LINES * LINE / 4;
+            const uint32_t base = smem_addr(smem);
+            for (int q = QUADS * part / parts + (int)threadIdx.x - 64; q < QUADS * (part + 1) / parts; q += EPI_WARPS * 32) {
+                const int line = q / (LINE / 4), at = q % (LINE / 4) * 4;
+                const uint32_t addr = base + 4u * (uint32_t)(line * PITCH + at);
+                const int token = (SWAP ? w.rt * BN : w.lt * BM) + line, col = (SWAP ? w.lt * BM : w.rt * BN) + at;
+                if (token < w.first || token >= w.last || col >= a.n) continue;
+                float4 f[8];
+#pragma unroll
+                for (int p = 0; p < 8; p++)
+                    if (p < parts) f[p] = ld_cluster_f32x4(map_to_rank(addr, (uint32_t)p));
+                float4 s = f[0];
+#pragma unroll
+                for (int p = 1; p < 8; p++)
+                    if (p < parts) { s.x += f[p].x; s.y += f[p].y; s.z += f[p].z; s.w += f[p].w; }
+                store4(a, token, col, s);
             }
         }
         __syncwarp();
         cluster_sync();                        // no CTA leaves while another reads its sums
+    }
+    if (PAIR) {
+        __syncwarp();
+        cluster_sync();                        // nor while its peer's MMAs or arrivals still reach it
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     if (warp == 1) {
         __syncwarp();
-        tmem_dealloc(tmem_base, S::TMEM_COLS);
+        if (PAIR) tmem_dealloc_pair(tmem_base, S::TMEM_COLS);
+        else tmem_dealloc(tmem_base, S::TMEM_COLS);
     }
 }
 
@@ -551,6 +652,21 @@ int make_map(CUtensorMap* map, const Operand& o, int k, int box_rows, int kind) 
     return r == CUDA_SUCCESS ? OZK_OK : OZK_ERR_DRIVER;
 }
 
+// scales [groups][row tiles][k tiles][512], box of KT k tiles x `tiles` row tiles; tiles past the end are zero
+int make_scale_map(CUtensorMap* map, const Operand& o, int k, int kt, int tiles) {
+    static const EncodeTiledFn fn = find_encode_fn();
+    if (!fn) return OZK_ERR_DRIVER;
+    const cuuint64_t ktiles = (cuuint64_t)(padded_k(k) / TILE), rtiles = (cuuint64_t)row_tiles(o.rows);
+    const cuuint64_t dims[4] = {TILE_BYTES / 4, ktiles, rtiles, (cuuint64_t)o.groups};
+    const cuuint64_t strides[3] = {TILE_BYTES, TILE_BYTES * ktiles, TILE_BYTES * ktiles * rtiles};
+    const cuuint32_t box[4] = {TILE_BYTES / 4, (cuuint32_t)kt, (cuuint32_t)tiles, 1u};
+    const cuuint32_t estr[4] = {1u, 1u, 1u, 1u};
+    const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 4, const_cast<uint8_t*>(o.scales), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? OZK_OK : OZK_ERR_DRIVER;
+}
+
 // SM count of the current device, 0 when it is not a B200
 int sm_count(int* dev_out) {
     static std::atomic<int> known[64];
@@ -577,50 +693,58 @@ struct Call {
 
 uint32_t format_bits(int kind, int fmt) { return kind == MXF4 ? 1u : fmt == OZK_MX_E2M1 ? 5u : 0u; }
 
-template <int KIND, int BN, bool SWAP>
+template <int KIND, int BN, bool SWAP, bool PAIR = false>
 int launch(const Call& c, int parts) {
-    using S = Shape<KIND, BN>;
-    auto kern = mx_gemm_kernel<KIND, BN, SWAP>;
-    static std::atomic<bool> ready[64];
-    if (!ready[c.dev].load(std::memory_order_acquire)) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
-        if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
-        ready[c.dev].store(true, std::memory_order_release);
-    }
+    using S = Shape<KIND, BN, PAIR>;
+    auto kern = mx_gemm_kernel<KIND, BN, SWAP, PAIR>;
     const Operand &L = SWAP ? c.B : c.A, &R = SWAP ? c.A : c.B;
     Args a = c.args;
-    a.sl = L.scales;
-    a.sr = R.scales;
-    a.sl_group = scale_group_bytes(L.rows, c.k);
-    a.sr_group = scale_group_bytes(R.rows, c.k);
     a.l_rows = L.rows;
     a.r_rows = R.rows;
     a.ktiles = padded_k(c.k) / TILE;
     a.kblocks = (a.ktiles + S::KT - 1) / S::KT;
     // a load that spreads 4-bit codes counts the bytes it reads, not the bytes it fills
-    a.load_bytes = S::L_BYTES / (spreads(L, KIND) ? 2u : 1u) + S::R_BYTES / (spreads(R, KIND) ? 2u : 1u);
-    a.idesc = umma_idesc_mx(format_bits(KIND, L.fmt), format_bits(KIND, R.fmt), BM, BN);
-    CUtensorMap tl, tr;
+    a.load_bytes = S::L_BYTES / (spreads(L, KIND) ? 2u : 1u) + S::R_BYTES / (spreads(R, KIND) ? 2u : 1u) + S::SL_BYTES + S::SR_BYTES;
+    a.idesc = umma_idesc_mx(format_bits(KIND, L.fmt), format_bits(KIND, R.fmt), S::BL, BN);
+    CUtensorMap tl, tr, tsl, tsr;
     int rc;
     if ((rc = make_map(&tl, L, c.k, BM, KIND)) != OZK_OK) return rc;
-    if ((rc = make_map(&tr, R, c.k, BN, KIND)) != OZK_OK) return rc;
-    const long long lt = (L.rows + BM - 1) / BM, rt = (R.rows + BN - 1) / BN;
+    if ((rc = make_map(&tr, R, c.k, S::RN, KIND)) != OZK_OK) return rc;
+    if ((rc = make_scale_map(&tsl, L, c.k, S::KT, 1)) != OZK_OK) return rc;
+    if ((rc = make_scale_map(&tsr, R, c.k, S::KT, S::SUBS)) != OZK_OK) return rc;
+    const long long lt = (L.rows + S::BL - 1) / S::BL, rt = (R.rows + BN - 1) / BN;
     if (lt * rt > 0x7fffffffLL || (BN == 32 && rt > 1)) return OZK_ERR_ARG;
-    // grouped: the number of tiles is known on the device only
-    const long long units = a.groups ? c.sms : lt * rt;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute cluster[1];
     cluster[0].id = cudaLaunchAttributeClusterDimension;
-    cluster[0].val.clusterDim.x = (unsigned)parts;
+    cluster[0].val.clusterDim.x = (unsigned)(PAIR ? 2 : parts);
     cluster[0].val.clusterDim.y = 1;
     cluster[0].val.clusterDim.z = 1;
     cfg.blockDim = dim3(THREADS, 1, 1);
     cfg.dynamicSmemBytes = S::SMEM;
     cfg.stream = c.st;
     cfg.attrs = cluster;
-    cfg.numAttrs = parts > 1 ? 1 : 0;
-    cfg.gridDim = dim3((unsigned)(parts > 1 ? units * parts : units < c.sms ? units : c.sms), 1, 1);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tl, tr, a, parts);
+    cfg.numAttrs = PAIR || parts > 1 ? 1 : 0;
+    // once per device: the shared memory limit, and for pairs how many fit at once
+    static std::atomic<int> resident[64];
+    int fit = resident[c.dev].load(std::memory_order_acquire);
+    if (fit == 0) {
+        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)S::SMEM);
+        if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
+        fit = c.sms;
+        if (PAIR) {
+            cfg.gridDim = dim3((unsigned)(c.sms / 2 * 2), 1, 1);
+            e = cudaOccupancyMaxActiveClusters(&fit, kern, &cfg);
+            if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
+            if (fit < 1) return OZK_ERR_DEVICE;
+        }
+        resident[c.dev].store(fit, std::memory_order_release);
+    }
+    // grouped: the number of tiles is known on the device only
+    const long long units = a.groups ? fit : lt * rt;
+    const long long grid = PAIR ? 2 * (units < fit ? units : fit) : parts > 1 ? units * parts : units < fit ? units : fit;
+    cfg.gridDim = dim3((unsigned)grid, 1, 1);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tl, tr, tsl, tsr, a, parts);
     if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
     OZK_CHECK_LAUNCH();
     return OZK_OK;
@@ -640,12 +764,14 @@ int choose(const Call& c) {
         const int per = c.args.tokens / c.args.groups;            // rows of an average group
         if (per <= 64) return launch<KIND, 64, true>(c, 1);
         if (per <= 128) return launch<KIND, 128, true>(c, 1);
-        return launch<KIND, 256, false>(c, 1);
+        if (per <= 512) return launch<KIND, 256, false>(c, 1);
+        return launch<KIND, 256, false, true>(c, 1);
     }
     const long long m = c.A.rows, nt = (c.n + BM - 1) / BM;
     if (m <= 32) return launch<KIND, 32, true>(c, parts_for(nt, kblocks, c.sms));
     if (m <= 64) return launch<KIND, 64, true>(c, parts_for(nt, kblocks, c.sms));
     const long long wide = ((m + BM - 1) / BM) * ((c.n + 255) / 256);
+    if (((m + 255) / 256) * ((c.n + 255) / 256) * 2 > c.sms) return launch<KIND, 256, false, true>(c, 1);
     if (wide * 2 > c.sms) return launch<KIND, 256, false>(c, 1);
     return launch<KIND, 128, false>(c, parts_for(((m + BM - 1) / BM) * nt, kblocks, c.sms));
 }

@@ -237,7 +237,7 @@ def _exact_operand(pkg, rng, fmt, rows, k, groups=None):
 
 PRODUCT_SHAPES = [(1, 1, 1), (1, 128, 128), (2, 40, 31), (31, 129, 256), (33, 100, 160), (64, 257, 384), (65, 64, 640),
                   (127, 130, 33), (128, 256, 512), (129, 255, 1000), (300, 700, 300), (1, 4096, 4096), (20, 300, 2080),
-                  (513, 770, 1100)]
+                  (513, 770, 1100), (1500, 2400, 300), (2300, 2310, 300), (4100, 3000, 700)]
 
 
 @pytest.mark.gpu
@@ -355,7 +355,8 @@ def _grouped_want(av, bv, ends):
 
 GROUPS = [(1, 1, [1]), (5, 3, [0, 5, 5]), (40, 4, [0, 0, 0, 0]), (200, 5, [1, 2, 130, 131, 200]), (300, 3, [128, 256, 300]),
           (290, 2, [31, 33]), (64, 33, list(range(1, 65, 2)) + [64]), (1000, 2, [3, 1000]), (500, 3, [499, 499, 500]),
-          (260, 1, [259]), (90, 40, [0] * 39 + [90])]
+          (260, 1, [259]), (90, 40, [0] * 39 + [90]),
+          (2100, 3, [700, 701, 2090]), (1300, 1, [1299]), (5000, 2, [3333, 5000])]
 
 
 @pytest.mark.gpu
