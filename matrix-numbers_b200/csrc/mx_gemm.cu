@@ -5,9 +5,9 @@
 // (K = 32; a 4-bit operand is spread to one code a byte by its TMA load).
 //
 // One persistent kernel, one CTA per SM:
-//   - warp 0 (one lane): producer; a stage is 128 bytes of K of 128 "left" rows (M) and BN "right" rows (N) and their
+//   - warp 0: producer; a stage is 128 bytes of K of 128 "left" rows (M) and BN "right" rows (N) and their
 //     scale tiles, four TMA loads, the codes with the 128-byte swizzle;
-//   - warp 1 (one lane): lays a stage's scales into TMEM (tcgen05.cp, two buffers of columns), a stage ahead of the four
+//   - warp 1: lays a stage's scales into TMEM (tcgen05.cp, two buffers of columns), a stage ahead of the four
 //     MMAs that use them, and issues those;
 //   - warps 2..9: epilogue, TMEM -> registers -> one rounding -> C.
 // Left is A and right is B (`SWAP` false), or, for few rows of A, left is B and right is A: the 128 rows that the
@@ -336,27 +336,25 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int kb0 = (int)((long long)a.kblocks * part / parts), kb1 = (int)((long long)a.kblocks * (part + 1) / parts);
 
     if (warp == 0) {
-        if (lane == 0) {
-            // ------------------------------------------------------------ producer
-            int stage = 0;
-            uint32_t phase = 0;
-            long long issued = 0;
-            bool ok = true;
-            for (long long u = u0; ok && u < work.units; u += du) {
-                const Unit w = work.at(u);
-                for (int kb = kb0; kb < kb1; kb++) {
-                    if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
-                        if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_PRODUCER);
-                        ok = false;
-                        break;
-                    }
+        // ---------------------------------------------------------------- producer (the whole warp; one lane issues)
+        int stage = 0;
+        uint32_t phase = 0;
+        long long issued = 0;
+        bool ok = true;
+        const uint32_t aL = smem_addr(sL), aR = smem_addr(sR), aSL = smem_addr(sSL), aSR = smem_addr(sSR);
+        for (long long u = u0; ok && u < work.units; u += du) {
+            const Unit w = work.at(u);
+            const int l0 = w.lt * S::BL + rank * BM, r0 = w.rt * BN + rank * S::RN;
+            for (int kb = kb0; kb < kb1; kb++) {
+                ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS);
+                if (!ok) break;
+                if (elect_one()) {
                     // a pair's loads all complete on CTA 0's barrier, which expects the bytes of both
                     if (rank == 0) mbar_arrive_expect_tx(full_bar(stage), a.load_bytes * (uint32_t)S::CTAS);
                     const uint32_t bar = PAIR ? map_to_rank(full_bar(stage), 0u) : full_bar(stage);
                     const int kc = kb * (KIND == MXF4 ? ROW_BYTES : TILE);      // bytes (mxf4) or elements
-                    const int l0 = w.lt * S::BL + rank * BM, r0 = w.rt * BN + rank * S::RN;
-                    const uint32_t dl = smem_addr(sL + stage * S::L_BYTES), dr = smem_addr(sR + stage * S::R_BYTES);
-                    const uint32_t dsl = smem_addr(sSL + stage * S::SL_BYTES), dsr = smem_addr(sSR + stage * S::SR_BYTES);
+                    const uint32_t dl = aL + stage * S::L_BYTES, dr = aR + stage * S::R_BYTES;
+                    const uint32_t dsl = aSL + stage * S::SL_BYTES, dsr = aSR + stage * S::SR_BYTES;
                     if (PAIR) {
                         tma_load_3d_pair(dl, &tmL, kc, l0, w.lg, bar);
                         tma_load_3d_pair(dr, &tmR, kc, r0, w.rg, bar);
@@ -368,11 +366,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                         tma_load_4d(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, w.lg, bar);
                         tma_load_4d(dsr, &tmSR, 0, kb * S::KT, w.rt * BN / TILE, w.rg, bar);
                     }
-                    issued++;
-                    if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
+                __syncwarp();
+                issued++;
+                if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
-            if (!ok && rank == 0) {
+        }
+        if (!ok) {
+            if (lane == 0 && !*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_PRODUCER);
+            if (rank == 0) {
                 // let the loads already issued land before the CTA (or the pair) exits (bounded)
                 const long long first = issued > STAGES ? issued - STAGES : 0;
                 for (long long j = first; j < issued; j++) {
@@ -382,11 +384,15 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
         }
     } else if (warp == 1) {
-        if (lane == 0 && rank == 0) {
-            // ------------------------------------------------------------ scales to TMEM, MMAs
+        if (rank == 0) {
+            // ------------------------------------------------------------ scales to TMEM, MMAs (the whole warp; one lane issues)
             int stage = 0, before = 0;
             uint32_t phase = 0, it = 0, step = 0;
-            bool ok = true, issued_any = false;
+            bool ok = true;
+            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            // descriptors: the address part advances with the stage, the rest is constant
+            const uint64_t dL = umma_desc_sw128(smem_addr(sL)), dR = umma_desc_sw128(smem_addr(sR));
+            const uint64_t dSL = smem_desc_scales(smem_addr(sSL)), dSR = smem_desc_scales(smem_addr(sSR));
             auto commit = [&](uint32_t bar) {      // an arrival on that barrier of every CTA when all issued so far is done
                 if (PAIR) {
                     umma_commit_pair(map_to_rank(bar, 0u));
@@ -401,23 +407,19 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (it >= (uint32_t)S::LAG) {
                     const uint32_t bar = S::LAG == 1 ? acce_bar(0) : acce_bar(b);
                     const uint32_t par = S::LAG == 1 ? (it - 1u) & 1u : ((it >> 1) - 1u) & 1u;
-                    if (!mbar_wait_bounded(bar, par, abort_flag, WAIT_LIMIT_NS)) {
-                        if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_MMA);
-                        ok = false;
-                        break;
-                    }
+                    ok = mbar_wait_warp(bar, par, abort_flag, WAIT_LIMIT_NS);
+                    if (!ok) break;
                     tc_fence_after();
                 }
-                const uint32_t d_tmem = tmem_base + (uint32_t)(b * S::ACC_STRIDE);
+                const uint32_t d_tmem = tmem + (uint32_t)(b * S::ACC_STRIDE);
                 // the second tile of 64 right rows in a scale tile starts two columns on (32 rows a column; an MMA takes
                 // its scales from an even column, so tiles of 32 rows exist for a first tile only)
                 const uint32_t r_col = BN == 64 ? (uint32_t)(w.rt & 1) * 2u : 0u;
-                auto columns = [&](uint32_t st) { return tmem_base + (uint32_t)(S::SCALE_BASE + (int)(st & 1u) * S::SCALE_COLS); };
+                auto columns = [&](uint32_t st) { return tmem + (uint32_t)(S::SCALE_BASE + (int)(st & 1u) * S::SCALE_COLS); };
                 // the four instructions of a stage: 32 bytes along K inside the swizzle atom each (+2 in the >> 4 address
                 // field); the last stage of an odd number of scale tiles has half of them
                 auto multiply = [&](int sg, uint32_t st, int kb) {
-                    const uint64_t ld = umma_desc_sw128(smem_addr(sL + sg * S::L_BYTES));
-                    const uint64_t rd = umma_desc_sw128(smem_addr(sR + sg * S::R_BYTES));
+                    const uint64_t ld = dL + (uint64_t)(sg * (S::L_BYTES >> 4)), rd = dR + (uint64_t)(sg * (S::R_BYTES >> 4));
                     const uint32_t tl = columns(st), tr = tl + (uint32_t)(4 * S::KT);
                     const int tiles = min(S::KT, a.ktiles - kb * S::KT);
 #pragma unroll
@@ -435,43 +437,51 @@ __global__ void __launch_bounds__(THREADS, 1)
                     commit(empty_bar(sg));
                 };
                 for (int kb = kb0; kb < kb1; kb++) {
-                    if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
-                        if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_MMA);
-                        ok = false;
-                        break;
-                    }
+                    ok = mbar_wait_warp(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS);
+                    if (!ok) break;
                     tc_fence_after();
-                    const uint32_t tl = columns(step), tr = tl + (uint32_t)(4 * S::KT);
+                    if (elect_one()) {
+                        const uint32_t tl = columns(step), tr = tl + (uint32_t)(4 * S::KT);
+                        const uint64_t sl = dSL + (uint64_t)(stage * (S::SL_BYTES >> 4)), sr = dSR + (uint64_t)(stage * (S::SR_BYTES >> 4));
 #pragma unroll
-                    for (int t = 0; t < S::KT; t++) {
-                        const uint64_t dl = smem_desc_scales(smem_addr(sSL + stage * S::SL_BYTES + t * TILE_BYTES));
-                        if (PAIR) tmem_cp_scales_pair(tl + 4u * t, dl);
-                        else tmem_cp_scales(tl + 4u * t, dl);
+                        for (int t = 0; t < S::KT; t++) {
+                            if (PAIR) tmem_cp_scales_pair(tl + 4u * t, sl + (uint64_t)(t * (TILE_BYTES >> 4)));
+                            else tmem_cp_scales(tl + 4u * t, sl + (uint64_t)(t * (TILE_BYTES >> 4)));
 #pragma unroll
-                        for (int i = 0; i < S::SUBS; i++) {
-                            const uint64_t dr = smem_desc_scales(smem_addr(sSR + stage * S::SR_BYTES + i * S::SL_BYTES + t * TILE_BYTES));
-                            const uint32_t to = tr + 4u * (uint32_t)(t * S::SUBS + i);
-                            if (PAIR) tmem_cp_scales_pair(to, dr);
-                            else tmem_cp_scales(to, dr);
+                            for (int i = 0; i < S::SUBS; i++) {
+                                const uint64_t from = sr + (uint64_t)((i * S::SL_BYTES + t * TILE_BYTES) >> 4);
+                                const uint32_t to = tr + 4u * (uint32_t)(t * S::SUBS + i);
+                                if (PAIR) tmem_cp_scales_pair(to, from);
+                                else tmem_cp_scales(to, from);
+                            }
                         }
+                        if (kb > kb0) multiply(before, step - 1u, kb - 1);
                     }
-                    issued_any = true;
-                    if (kb > kb0) multiply(before, step - 1u, kb - 1);
+                    __syncwarp();
                     before = stage;
                     step++;
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
-                multiply(before, step - 1u, kb1 - 1);
-                commit(accf_bar(b));
+                if (elect_one()) {
+                    multiply(before, step - 1u, kb1 - 1);
+                    commit(accf_bar(b));
+                }
+                __syncwarp();
                 it++;
             }
-            if (!ok && issued_any) {
-                // all MMAs issued by this thread must finish before TMEM is released
-                if (PAIR) umma_commit_pair(map_to_rank(drain_bar, 0u));
-                else umma_commit(drain_bar);
-                int dummy = 0;
-                mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
+            if (!ok) {
+                if (lane == 0 && !*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_MMA);
+                if (step > 0) {
+                    // all that this warp issued must finish before TMEM is released
+                    if (elect_one()) {
+                        if (PAIR) umma_commit_pair(map_to_rank(drain_bar, 0u));
+                        else umma_commit(drain_bar);
+                    }
+                    __syncwarp();
+                    int dummy = 0;
+                    mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
+                }
             }
         }
     } else {
@@ -489,8 +499,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (long long u = u0; ok && u < work.units; u += du) {
             const Unit w = work.at(u);
             const int b = (int)(it & 1u);
-            if (!mbar_wait_bounded(accf_bar(b), (it >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
-                if (!*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_EPILOGUE);
+            if (!mbar_wait_warp(accf_bar(b), (it >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
+                if (lane == 0 && !*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_EPILOGUE);
                 ok = false;
                 break;
             }

@@ -55,6 +55,24 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint32_t bar, uint32_t parity,
     }
 }
 
+// true in one lane of a fully active warp.  A loop that the whole warp runs, with its asynchronous instructions in the
+// elected lane, keeps their operands in uniform registers.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(p));
+    return p != 0;
+}
+
+// The same for a whole warp (true in every lane or in none): it polls a while before it looks at the clock, which is slow
+// to read.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, const volatile int* abort_flag,
+                                               uint64_t limit_ns) {
+    bool ok = false;
+    for (int it = 0; it < 256 && !ok; ++it) ok = __all_sync(0xffffffffu, mbar_try_wait(bar, parity));
+    if (!ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, limit_ns));
+    return ok;
+}
+
 // ---- TMA -------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ void tma_prefetch_desc(const CUtensorMap* map) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
