@@ -40,6 +40,7 @@ namespace {
 constexpr int BM = 128;                      // rows of the left operand's tile
 constexpr int ROW_BYTES = 128;               // K bytes of one stage row (shared memory)
 constexpr int EPI_WARPS = 8;
+constexpr uint32_t OUT_WARP_BYTES = 32 * 128;   // one epilogue warp's 32 rows of C, 128 bytes each
 constexpr int THREADS = (2 + EPI_WARPS) * 32;
 constexpr int GROUP_L = 16;                  // left tiles per raster group
 constexpr uint64_t WAIT_LIMIT_NS = 4000000000ull;   // 4 s of wall time per wait
@@ -47,7 +48,7 @@ constexpr int MXF4 = 0, MXF8F6F4 = 1;
 constexpr size_t SMEM_MAX = 232448;
 constexpr size_t TABLE_BYTES = (2 * (OZK_MX_MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
 
-template <int KIND, int BN, bool PAIR>
+template <int KIND, int BN, bool SWAP, bool PAIR>
 struct Shape {
     static constexpr int CTAS = PAIR ? 2 : 1;
     static constexpr int BL = BM * CTAS;                        // left rows of a tile
@@ -57,9 +58,10 @@ struct Shape {
     static constexpr uint32_t L_BYTES = BM * ROW_BYTES, R_BYTES = RN * ROW_BYTES;
     static constexpr uint32_t SL_BYTES = KT * TILE_BYTES, SR_BYTES = SUBS * KT * TILE_BYTES;
     static constexpr uint32_t STAGE_BYTES = L_BYTES + R_BYTES + SL_BYTES + SR_BYTES;
-    static constexpr int FIT = (int)((SMEM_MAX - 1024 - 256 - TABLE_BYTES) / STAGE_BYTES);
+    static constexpr uint32_t OUT_BYTES = SWAP ? 0 : EPI_WARPS * OUT_WARP_BYTES;   // where C leaves by TMA
+    static constexpr int FIT = (int)((SMEM_MAX - 1024 - 256 - TABLE_BYTES - OUT_BYTES) / STAGE_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;
-    static constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + 1024 + 256 + TABLE_BYTES;
+    static constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256 + TABLE_BYTES;
     static constexpr int NUM_BARS = 2 * STAGES + 5;             // full[S], empty[S], acc_full[2], acc_empty[2], drain
     // TMEM: two accumulators, then two buffers of scale columns.  With BN = 256 the accumulators overlap by 48 columns,
     // which makes room for the scales: the epilogue reads the shared columns first, and the next tile waits for those.
@@ -88,7 +90,7 @@ struct Args {
     void* C;
     long long ldc;
     int dtype;
-    bool vec;                                // rows of C are 16-byte aligned
+    bool vec;                                // rows of C are 16-byte aligned, and tmC describes it
     uint32_t idesc;
     int32_t* err;
 };
@@ -223,6 +225,57 @@ __device__ __forceinline__ void store_chunk(const Args& a, const Unit& w, int l,
     }
 }
 
+// One warp's 32 rows x 64 columns of the accumulator (rows from l0, columns from r) to C.  Whole row segments go through
+// this warp's shared memory (128-byte swizzle) and leave by TMA, which clips at C's ends: 4.2 us an epilogue of 128 x 256
+// with direct stores of 32 bytes a row, which were slower than the MMAs of K < 4096.  The edge rows of a group, and a C
+// whose rows are not aligned, take the direct stores; so do the last columns where a row of C does not end on 16 bytes (a
+// clipped box writes zeros up to there).
+__device__ __forceinline__ void store_block(const Args& a, const CUtensorMap* tmC, const Unit& w, int l0, int r, int lane,
+                                            uint32_t out, const uint32_t (&v0)[32], const uint32_t (&v1)[32]) {
+    if (r >= a.n || l0 >= w.last || l0 + 32 <= w.first) return;
+    const bool ends_inside = r + 64 > a.n && a.n * (a.dtype == OZK_F32 ? 4 : 2) % 16 != 0;
+    if (!a.vec || ends_inside || l0 < w.first || (l0 + 32 > w.last && w.last < a.tokens)) {
+        store_chunk<32, false>(a, w, l0 + lane, r, v0);
+        store_chunk<32, false>(a, w, l0 + lane, r + 32, v1);
+        return;
+    }
+    const uint32_t row = out + (uint32_t)lane * 128u, sw = (uint32_t)(lane & 7);
+    auto ready = [&] {                          // the box that was here has been read
+        if (lane == 0) bulk_wait_read();
+        __syncwarp();
+    };
+    auto send = [&](int col) {
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_2d(tmC, out, col, l0);
+            bulk_commit();
+        }
+    };
+    if (a.dtype == OZK_F32) {
+        ready();
+#pragma unroll
+        for (int c = 0; c < 8; c++) st_shared_v4(row + (((uint32_t)c ^ sw) << 4), v0[4 * c], v0[4 * c + 1], v0[4 * c + 2], v0[4 * c + 3]);
+        send(r);
+        if (r + 32 >= a.n) return;
+        ready();
+#pragma unroll
+        for (int c = 0; c < 8; c++) st_shared_v4(row + (((uint32_t)c ^ sw) << 4), v1[4 * c], v1[4 * c + 1], v1[4 * c + 2], v1[4 * c + 3]);
+        send(r + 32);
+    } else {
+        uint32_t p[32];
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            p[j] = pack2(__uint_as_float(v0[2 * j]), __uint_as_float(v0[2 * j + 1]), a.dtype);
+            p[16 + j] = pack2(__uint_as_float(v1[2 * j]), __uint_as_float(v1[2 * j + 1]), a.dtype);
+        }
+        ready();
+#pragma unroll
+        for (int c = 0; c < 8; c++) st_shared_v4(row + (((uint32_t)c ^ sw) << 4), p[4 * c], p[4 * c + 1], p[4 * c + 2], p[4 * c + 3]);
+        send(r);
+    }
+}
+
 // Four neighbouring values of a row of C
 __device__ __forceinline__ void store4(const Args& a, int token, int col, float4 s) {
     const long long at = (long long)token * a.ldc + col;
@@ -276,19 +329,20 @@ template <int KIND, int BN, bool SWAP, bool PAIR>
 __global__ void __launch_bounds__(THREADS, 1)
     mx_gemm_kernel(const __grid_constant__ CUtensorMap tmL, const __grid_constant__ CUtensorMap tmR,
                    const __grid_constant__ CUtensorMap tmSL, const __grid_constant__ CUtensorMap tmSR,
-                   const __grid_constant__ Args a, int parts) {
-    using S = Shape<KIND, BN, PAIR>;
+                   const __grid_constant__ CUtensorMap tmC, const __grid_constant__ Args a, int parts) {
+    using S = Shape<KIND, BN, SWAP, PAIR>;
     constexpr int STAGES = S::STAGES, CHUNK = S::CHUNK;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     uint8_t* sL = smem;
     uint8_t* sR = sL + STAGES * S::L_BYTES;
-    uint8_t* sSL = sR + STAGES * S::R_BYTES;
+    uint8_t* sOut = sR + STAGES * S::R_BYTES;  // boxes of C on 1024-byte boundaries
+    uint8_t* sSL = sOut + S::OUT_BYTES;
     uint8_t* sSR = sSL + STAGES * S::SL_BYTES;
-    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * S::STAGE_BYTES);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(sSR + STAGES * S::SR_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::NUM_BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    int* pre = reinterpret_cast<int*>(smem + STAGES * S::STAGE_BYTES + 256);
+    int* pre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 256);
     int* bound = pre + OZK_MX_MAX_GROUPS + 1;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -526,31 +580,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                             *reinterpret_cast<uint4*>(mine + row * (BN + 4) + col + e) = make_uint4(v[e], v[e + 1], v[e + 2], v[e + 3]);
                     }
                 }
-            } else if (S::LAG == 1) {
-                // the columns shared with the other accumulator: the last 48 of buffer 0, the first 48 of buffer 1
-                const bool shared_half = half == 1 - b;
-                const int c0 = b == 0 ? NCH - 1 : 0, dc = b == 0 ? -1 : 1;
-                uint32_t v0[CHUNK], v1[CHUNK];
-                if (!shared_half) {
-                    if (lane == 0) drained(0);
-                }
-#pragma unroll 1
-                for (int c = 0; c < NCH; c += 2) {
-                    const int ca = c0 + dc * c, cb = c0 + dc * (c + 1);
-                    tmem_ld_chunk<CHUNK>(acc + (uint32_t)(ca * CHUNK), v0);
-                    tmem_ld_chunk<CHUNK>(acc + (uint32_t)(cb * CHUNK), v1);
-                    tmem_wait_ld();
-                    if (c == 0 && shared_half) {
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) drained(0);
-                    }
-                    store_chunk<CHUNK, SWAP>(a, w, l, r + ca * CHUNK, v0);
-                    store_chunk<CHUNK, SWAP>(a, w, l, r + cb * CHUNK, v1);
-                }
-                tc_fence_before();
-                __syncwarp();
-            } else {
+            } else if constexpr (SWAP) {
 #pragma unroll 1
                 for (int c = 0; c < NCH; c++) {
                     uint32_t v[CHUNK];
@@ -561,11 +591,35 @@ __global__ void __launch_bounds__(THREADS, 1)
                         __syncwarp();
                         if (lane == 0) drained(b);
                     }
-                    store_chunk<CHUNK, SWAP>(a, w, l, r + c * CHUNK, v);
+                    store_chunk<CHUNK, true>(a, w, l, r + c * CHUNK, v);
                 }
+            } else {
+                // blocks of 64 columns.  Accumulators that overlap: those with the shared columns (the last 48 of buffer 0,
+                // the first 48 of buffer 1) are read first, and a warp without them has nothing that the next tile waits for
+                constexpr int BLOCKS = S::HALF / 64;
+                const bool shared_half = S::LAG == 2 || half == 1 - b;
+                const bool backward = S::LAG == 1 && b == 0;
+                if (!shared_half && lane == 0) drained(0);
+#pragma unroll 1
+                for (int c = 0; c < BLOCKS; c++) {
+                    const int at = (backward ? BLOCKS - 1 - c : c) * 64;
+                    uint32_t v0[32], v1[32];
+                    tmem_ld_32x32b_x32(acc + (uint32_t)at, v0);
+                    tmem_ld_32x32b_x32(acc + (uint32_t)(at + 32), v1);
+                    tmem_wait_ld();
+                    if (shared_half && c == (S::LAG == 1 ? 0 : BLOCKS - 1)) {
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) drained(S::LAG == 1 ? 0 : b);
+                    }
+                    store_block(a, &tmC, w, l - lane, r + at, lane, smem_addr(sOut + ew * OUT_WARP_BYTES), v0, v1);
+                }
+                tc_fence_before();
+                __syncwarp();
             }
             it++;
         }
+        if (!SWAP && lane == 0) bulk_wait_all();
         // rows of C behind the last group
         if (a.groups && a.fill) {
             const int size = a.dtype == OZK_F32 ? 4 : 2;
@@ -677,6 +731,21 @@ int make_scale_map(CUtensorMap* map, const Operand& o, int k, int kt, int tiles)
     return r == CUDA_SUCCESS ? OZK_OK : OZK_ERR_DRIVER;
 }
 
+// C: boxes of 32 rows x 128 bytes, 128-byte swizzle
+int make_out_map(CUtensorMap* map, const Args& a) {
+    static const EncodeTiledFn fn = find_encode_fn();
+    if (!fn) return OZK_ERR_DRIVER;
+    const cuuint64_t size = a.dtype == OZK_F32 ? 4 : 2;
+    const cuuint64_t dims[2] = {(cuuint64_t)a.n, (cuuint64_t)a.tokens};
+    const cuuint64_t strides[1] = {(cuuint64_t)a.ldc * size};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / size), 32u};
+    const cuuint32_t estr[2] = {1u, 1u};
+    const CUresult r = fn(map, size == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, a.C, dims,
+                          strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? OZK_OK : OZK_ERR_DRIVER;
+}
+
 // SM count of the current device, 0 when it is not a B200
 int sm_count(int* dev_out) {
     static std::atomic<int> known[64];
@@ -705,7 +774,7 @@ uint32_t format_bits(int kind, int fmt) { return kind == MXF4 ? 1u : fmt == OZK_
 
 template <int KIND, int BN, bool SWAP, bool PAIR = false>
 int launch(const Call& c, int parts) {
-    using S = Shape<KIND, BN, PAIR>;
+    using S = Shape<KIND, BN, SWAP, PAIR>;
     auto kern = mx_gemm_kernel<KIND, BN, SWAP, PAIR>;
     const Operand &L = SWAP ? c.B : c.A, &R = SWAP ? c.A : c.B;
     Args a = c.args;
@@ -716,12 +785,13 @@ int launch(const Call& c, int parts) {
     // a load that spreads 4-bit codes counts the bytes it reads, not the bytes it fills
     a.load_bytes = S::L_BYTES / (spreads(L, KIND) ? 2u : 1u) + S::R_BYTES / (spreads(R, KIND) ? 2u : 1u) + S::SL_BYTES + S::SR_BYTES;
     a.idesc = umma_idesc_mx(format_bits(KIND, L.fmt), format_bits(KIND, R.fmt), S::BL, BN);
-    CUtensorMap tl, tr, tsl, tsr;
+    CUtensorMap tl, tr, tsl, tsr, tc = {};
     int rc;
     if ((rc = make_map(&tl, L, c.k, BM, KIND)) != OZK_OK) return rc;
     if ((rc = make_map(&tr, R, c.k, S::RN, KIND)) != OZK_OK) return rc;
     if ((rc = make_scale_map(&tsl, L, c.k, S::KT, 1)) != OZK_OK) return rc;
     if ((rc = make_scale_map(&tsr, R, c.k, S::KT, S::SUBS)) != OZK_OK) return rc;
+    if (!SWAP && parts == 1 && a.vec && (rc = make_out_map(&tc, a)) != OZK_OK) return rc;
     const long long lt = (L.rows + S::BL - 1) / S::BL, rt = (R.rows + BN - 1) / BN;
     if (lt * rt > 0x7fffffffLL || (BN == 32 && rt > 1)) return OZK_ERR_ARG;
     cudaLaunchConfig_t cfg = {};
@@ -754,7 +824,7 @@ int launch(const Call& c, int parts) {
     const long long units = a.groups ? fit : lt * rt;
     const long long grid = PAIR ? 2 * (units < fit ? units : fit) : parts > 1 ? units * parts : units < fit ? units : fit;
     cfg.gridDim = dim3((unsigned)grid, 1, 1);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tl, tr, tsl, tsr, a, parts);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, tl, tr, tsl, tsr, tc, a, parts);
     if (e != cudaSuccess) return OZK_ERR_CUDA_BASE + (int)e;
     OZK_CHECK_LAUNCH();
     return OZK_OK;
@@ -816,7 +886,8 @@ int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const u
     a.C = C;
     a.ldc = ldc;
     a.dtype = dtype;
-    a.vec = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && ldc * (int64_t)size % 16 == 0;
+    // (a tensor map's stride ends at 2^40 bytes)
+    a.vec = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && ldc * (int64_t)size % 16 == 0 && ldc < ((int64_t)1 << 37);
     a.err = err;
     return c.kind == MXF4 ? choose<MXF4>(c) : choose<MXF8F6F4>(c);
 }
