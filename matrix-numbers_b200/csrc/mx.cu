@@ -66,9 +66,9 @@ __device__ __forceinline__ void load8_any(const T* __restrict__ p, int count, co
 // One row's eight values per lane (16 lanes a row of the tile) to codes in global memory and the scale byte in `sc`: a
 // block of 32 is four lanes, its largest magnitude two shuffles away.
 template <int FMT>
-__device__ __forceinline__ void emit_row(float (&v)[8], bool up, int r, int here, int lane16, uint8_t* __restrict__ ct,
+__device__ __forceinline__ void emit_row(float (&v)[8], uint32_t max_bits, bool up, int r, int here, int lane16, uint8_t* __restrict__ ct,
                                          long long pitch, uint8_t* sc) {
-    const int s = block_scale<FMT>(quad_max(max_bits8(v)), up);
+    const int s = block_scale<FMT>(quad_max(max_bits), up);
     const float inv = scale_inverse(s);
 #pragma unroll
     for (int j = 0; j < 8; j++) v[j] *= inv;
@@ -97,18 +97,55 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const __grid_con
     const T* xt = static_cast<const T*>(q.x) + g * q.gs + (long long)rt * TILE * q.si + col;
     const int count = max(0, q.J - col);
 
-    float v[8][8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const int r = r0 + 16 * i;
-        const int n = r < here ? count : 0;
-        if (ALIGNED) load8(xt + (long long)r * q.si, n >= 8, n, v[i]);
-        else load8_any(xt + (long long)r * q.si, n, q.begin, q.end, v[i]);
-    }
     const long long pitch = code_pitch(FMT, q.J);
     uint8_t* ct = q.row_codes + ((long long)g * q.I + (long long)rt * TILE) * pitch + kt * (FMT == OZK_MX_E2M1 ? 64 : 128);
+    if constexpr (ALIGNED && sizeof(T) == 2) {
+        // the words as they are until they are encoded: half the registers, and magnitudes ordered like their bits
+        const T* const type = nullptr;
+        uint4 raw[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) emit_row<FMT>(v[i], up, r0 + 16 * i, here, lane16, ct, pitch, sc);
+        for (int i = 0; i < 8; i++) {
+            const int r = r0 + 16 * i;
+            const T* p = xt + (long long)r * q.si;
+            raw[i] = make_uint4(0u, 0u, 0u, 0u);
+            if (r < here) {
+                if (count >= 8) {
+                    raw[i] = __ldg(reinterpret_cast<const uint4*>(p));
+                } else if (count > 0) {
+                    float v[8];
+                    load8(p, false, count, v);
+                    raw[i] = make_uint4(pack2(v[0], v[1], type), pack2(v[2], v[3], type), pack2(v[4], v[5], type),
+                                        pack2(v[6], v[7], type));
+                }
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            const uint32_t m2 = __vmaxu2(__vmaxu2(w[0] & 0x7fff7fffu, w[1] & 0x7fff7fffu),
+                                         __vmaxu2(w[2] & 0x7fff7fffu, w[3] & 0x7fff7fffu));
+            const float2 m = unpack2(m2, type);
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = unpack2(w[j], type);
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
+            emit_row<FMT>(v, max(__float_as_uint(m.x), __float_as_uint(m.y)), up, r0 + 16 * i, here, lane16, ct, pitch, sc);
+        }
+    } else {
+        float v[8][8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const int r = r0 + 16 * i;
+            const int n = r < here ? count : 0;
+            if (ALIGNED) load8(xt + (long long)r * q.si, n >= 8, n, v[i]);
+            else load8_any(xt + (long long)r * q.si, n, q.begin, q.end, v[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < 8; i++) emit_row<FMT>(v[i], max_bits8(v[i]), up, r0 + 16 * i, here, lane16, ct, pitch, sc);
+    }
     __syncthreads();
     copy_scale_tile(q.row_scales + (long long)blockIdx.x * TILE_BYTES, sc);
 }
@@ -130,11 +167,6 @@ __device__ __forceinline__ int encode_block(uint32_t m, bool up, uint4 (&c)[2], 
     c[1] = make_uint4(w[2].x, w[2].y, w[3].x, w[3].y);
     return s;
 }
-
-__device__ __forceinline__ float low_half(uint32_t w, __half*) { return __half2float(__ushort_as_half((unsigned short)w)); }
-__device__ __forceinline__ float high_half(uint32_t w, __half*) { return __half2float(__ushort_as_half((unsigned short)(w >> 16))); }
-__device__ __forceinline__ float low_half(uint32_t w, __nv_bfloat16*) { return __uint_as_float(w << 16); }
-__device__ __forceinline__ float high_half(uint32_t w, __nv_bfloat16*) { return __uint_as_float(w & 0xffff0000u); }
 
 // The column operand, alone or with the row operand (one or two jobs in one launch).  A thread owns a block of 32
 // values down a column (FP32) or a pair of columns (16-bit types, one 32-bit word a row), which it reads straight into
@@ -166,14 +198,14 @@ __global__ void __launch_bounds__(THREADS)
             for (int h = 0; h < 2; h++) {
                 const int b = (threadIdx.x >> 7) + 2 * h;
                 float v[BLOCK];
-                uint32_t m = 0;
+                float m = 0.0f;
                 const T* p = xt + (long long)(b * BLOCK) * q.si + c * q.sj;
 #pragma unroll
                 for (int j = 0; j < BLOCK; j++) v[j] = (c < cols && b * BLOCK + j < rows) ? __ldg(p + j * q.si) : 0.0f;
 #pragma unroll
-                for (int j = 0; j < BLOCK; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+                for (int j = 0; j < BLOCK; j++) m = max_magnitude(m, v[j]);
                 uint4 o[2];
-                sc[0][scale_slot(c, b)] = (uint8_t)encode_block<FMT>(m, up, o, [&](int j) { return v[j]; });
+                sc[0][scale_slot(c, b)] = (uint8_t)encode_block<FMT>(__float_as_uint(m), up, o, [&](int j) { return v[j]; });
                 uint4* d = reinterpret_cast<uint4*>(staged + c * CP + b * (SEG / 4));
                 d[0] = o[0];
                 if (FMT != OZK_MX_E2M1) d[1] = o[1];
@@ -197,16 +229,16 @@ __global__ void __launch_bounds__(THREADS)
             uint32_t m = 0;                                      // magnitudes of 16-bit types are ordered like their bits
 #pragma unroll
             for (int j = 0; j < BLOCK; j++) m = __vmaxu2(m, v[j] & 0x7fff7fffu);
-            T* const type = nullptr;
+            const T* const type = nullptr;
             uint4 o[2];
             uint4* d = reinterpret_cast<uint4*>(staged + c * CP + b * (SEG / 4));
-            sc[0][scale_slot(c, b)] = (uint8_t)encode_block<FMT>(__float_as_uint(low_half(m, type)), up, o,
-                                                                 [&](int j) { return low_half(v[j], type); });
+            sc[0][scale_slot(c, b)] = (uint8_t)encode_block<FMT>(__float_as_uint(unpack2(m, type).x), up, o,
+                                                                 [&](int j) { return unpack2(v[j], type).x; });
             d[0] = o[0];
             if (FMT != OZK_MX_E2M1) d[1] = o[1];
             d = reinterpret_cast<uint4*>(staged + (c + 1) * CP + b * (SEG / 4));
-            sc[0][scale_slot(c + 1, b)] = (uint8_t)encode_block<FMT>(__float_as_uint(high_half(m, type)), up, o,
-                                                                     [&](int j) { return high_half(v[j], type); });
+            sc[0][scale_slot(c + 1, b)] = (uint8_t)encode_block<FMT>(__float_as_uint(unpack2(m, type).y), up, o,
+                                                                     [&](int j) { return unpack2(v[j], type).y; });
             d[0] = o[0];
             if (FMT != OZK_MX_E2M1) d[1] = o[1];
         }
@@ -225,7 +257,7 @@ __global__ void __launch_bounds__(THREADS)
                 load8(xt + (long long)r * q.si + lane16 * 8, n >= 8, n, v[i]);
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) emit_row<FMT>(v[i], up, r0 + 16 * (4 * h + i), rows, lane16, ct, pitch, sc[1]);
+            for (int i = 0; i < 4; i++) emit_row<FMT>(v[i], max_bits8(v[i]), up, r0 + 16 * (4 * h + i), rows, lane16, ct, pitch, sc[1]);
         }
     }
     __syncthreads();
@@ -320,7 +352,7 @@ __global__ void __launch_bounds__(THREADS)
 // t = x (+ residual), y = t / sqrt(mean(t^2) + eps) weight, y quantised; t, rounded to the type of x, is the next
 // residual.  Everything between the loads and the codes stays in registers: one pass over x and the residual, TPR threads
 // a row with NC chunks of eight values each (longer rows read the rest a second time).  The sums are taken in a fixed
-// order.  y is computed to its last FP32 bit: a rounding on the way would move values across the borders between codes.
+// order; the inverse root is rounded once, t weight and its product with the root once each.
 template <int TPR>
 __device__ __forceinline__ double row_sum(double v, double* part) {
 #pragma unroll
@@ -335,22 +367,18 @@ __device__ __forceinline__ double row_sum(double v, double* part) {
     return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// 1 / sqrt(a) as a sum of two FP32 numbers: the FP32 root and one Newton step whose residual 1 - a r^2 is taken exactly
-__device__ __forceinline__ float2 inverse_root(double a) {
-    if (!(a < 3.0e38)) {                                        // beyond FP32 (or NaN)
-        const double r = 1.0 / sqrt(a);
-        const float h = (float)r;
-        return make_float2(h, (float)(r - (double)h));
-    }
+// 1 / sqrt(a) to the nearest FP32 number or its neighbour: FP32's root and one Newton step with an exact residual 1 - a r^2
+__device__ __forceinline__ float inverse_root(double a) {
+    if (!(a < 3.0e38)) return (float)(1.0 / sqrt(a));           // beyond FP32 (or NaN)
     const float ah = (float)a, al = (float)(a - (double)ah);
     const float r = rsqrtf(ah);
     const float q = ah * r, qe = fmaf(ah, r, -q);
     const float e = fmaf(-q, r, 1.0f) - fmaf(qe, r, al * r * r);
-    return make_float2(r, 0.5f * r * e);
+    return fmaf(0.5f * r, e, r);
 }
 
 template <typename T, typename W, int FMT, int TPR, int NC>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / TPR)
     rms_norm_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ residual, long long res_stride,
                     const W* __restrict__ weight, int rows, int d, double inv_d, float eps, bool aligned, bool up,
                     T* __restrict__ sum, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
@@ -377,14 +405,14 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
             for (int j = 0; j < 8; j++) o[j] += q[j];
         }
     };
-    // sum of (t scale)^2: a thread's share in FP32, the shares in FP64
-    auto squares = [&](float scale, bool store) {
+    // sum of f(t)^2: a thread's share in FP32, the shares in FP64
+    auto squares = [&](auto f, bool store) {
         float sq = 0.0f;
         auto note = [&](int c, const float (&o)[8]) {
             if (store && sr) store8(sr + c * 8, aligned && c * 8 + 8 <= d, max(0, d - c * 8), o);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                const float u = o[j] * scale;
+                const float u = f(o[j]);
                 sq = fmaf(u, u, sq);
             }
         };
@@ -401,9 +429,9 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
 #pragma unroll
     for (int i = 0; i < NC; i++)
         if (t + i * TPR < chunks) fetch(t + i * TPR, v[i]);
-    double total = squares(1.0f, true);
-    if (!(total < 3.0e38)) total = squares(0x1p-70f, false) * 0x1p140;   // squares beyond FP32: once more, scaled
-    const float2 rstd = inverse_root(total * inv_d + (double)eps);
+    double total = squares([](float x) { return x; }, true);
+    if (!(total < 3.0e38)) total = squares([](float x) { return x * 0x1p-70f; }, false) * 0x1p140;   // beyond FP32: scaled
+    const float rstd = inverse_root(total * inv_d + (double)eps);
 
     const long long pitch = code_pitch(FMT, d);
     uint8_t* cr = codes + row * pitch;
@@ -413,11 +441,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR)
         float w[8];
         load8(weight + c * 8, in && aligned && c * 8 + 8 <= d, in ? max(0, d - c * 8) : 0, w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            // t w rstd rounded once: the product's rounding error and the low part of rstd go along
-            const float p = o[j] * w[j], e = fmaf(o[j], w[j], -p);
-            o[j] = in ? fmaf(p, rstd.x, fmaf(p, rstd.y, e * rstd.x)) : 0.0f;
-        }
+        for (int j = 0; j < 8; j++) o[j] = in ? o[j] * w[j] * rstd : 0.0f;
         const int s = block_scale<FMT>(quad_max(max_bits8(o)), up);
         const float inv = scale_inverse(s);
 #pragma unroll
@@ -581,7 +605,7 @@ int launch_norm(const NormArgs& a) {
     const bool aligned = aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) && aligned16(a.sum) &&
                          (a.rows == 1 || (a.x_stride * size % 16 == 0 && (!a.residual || a.res_stride * size % 16 == 0) &&
                                           (!a.sum || a.d * size % 16 == 0)));
-    // threads a row: enough that a row's values stay in registers (4 chunks of eight a thread), a warp for short rows
+    // threads a row: enough that the values of up to 16384 stay in registers, a warp for short rows
     const int d = a.d;
 #define OZK_NORM(TPR, NC)                                                                                            \
     rms_norm_kernel<T, W, FMT, TPR, NC>                                                                              \
@@ -589,9 +613,10 @@ int launch_norm(const NormArgs& a) {
             static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), a.res_stride,                 \
             static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps, aligned, a.up, static_cast<T*>(a.sum), a.codes, a.scales)
     if (d <= 1024) OZK_NORM(32, 4);
+    else if (d <= 2048) OZK_NORM(256, 1);
     else if (d <= 4096) OZK_NORM(256, 2);
-    else if (d <= 8192) OZK_NORM(256, 4);
-    else OZK_NORM(1024, 4);
+    else if (d <= 8192) OZK_NORM(512, 2);
+    else OZK_NORM(1024, 2);
 #undef OZK_NORM
     OZK_CHECK_LAUNCH();
     return OZK_OK;

@@ -107,6 +107,20 @@ __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
+// the two 16-bit values of a 32-bit word (the tag pointer names the type), and back
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __half*) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
+__device__ __forceinline__ float2 unpack2(uint32_t w, const __nv_bfloat16*) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __half*) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, const __nv_bfloat16*) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // Eight consecutive values as FP32.  `whole`: p is 16-byte aligned and all eight are inside; else the first `count`
 // are read one by one (the others are 0).
 template <typename T>
@@ -118,9 +132,13 @@ __device__ __forceinline__ void load8(const T* __restrict__ p, bool whole, int c
             v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
         } else {
             const uint4 a = __ldg(reinterpret_cast<const uint4*>(p));
-            const T* e = reinterpret_cast<const T*>(&a);
+            const uint32_t w[4] = {a.x, a.y, a.z, a.w};
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = to_f32(e[j]);
+            for (int j = 0; j < 4; j++) {
+                const float2 f = unpack2(w[j], (const T*)nullptr);
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
         }
     } else {
 #pragma unroll
@@ -135,11 +153,9 @@ __device__ __forceinline__ void store8(T* __restrict__ p, bool whole, int count,
             reinterpret_cast<float4*>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
             reinterpret_cast<float4*>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
         } else {
-            uint4 a;
-            T* e = reinterpret_cast<T*>(&a);
-#pragma unroll
-            for (int j = 0; j < 8; j++) e[j] = from_f32<T>(v[j]);
-            *reinterpret_cast<uint4*>(p) = a;
+            const T* const type = nullptr;
+            *reinterpret_cast<uint4*>(p) = make_uint4(pack2(v[0], v[1], type), pack2(v[2], v[3], type),
+                                                      pack2(v[4], v[5], type), pack2(v[6], v[7], type));
         }
     } else {
 #pragma unroll
@@ -148,11 +164,18 @@ __device__ __forceinline__ void store8(T* __restrict__ p, bool whole, int count,
     }
 }
 
-__device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < 8; j++) m = max(m, __float_as_uint(v[j]) & 0x7fffffffu);
+// the larger magnitude, NaN if either is
+__device__ __forceinline__ float max_magnitude(float a, float b) {
+    float m;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(fabsf(a)), "f"(fabsf(b)));
     return m;
+}
+
+// bits of the largest magnitude of eight values (at least those of infinity if one is infinite or NaN)
+__device__ __forceinline__ uint32_t max_bits8(const float (&v)[8]) {
+    const float a = max_magnitude(max_magnitude(v[0], v[1]), max_magnitude(v[2], v[3]));
+    const float b = max_magnitude(max_magnitude(v[4], v[5]), max_magnitude(v[6], v[7]));
+    return __float_as_uint(max_magnitude(a, b));
 }
 
 // largest of the four lanes that hold one block (lanes 4 i .. 4 i + 3)
