@@ -353,15 +353,15 @@ __global__ void __launch_bounds__(THREADS)
 // residual.  Everything between the loads and the codes stays in registers: one pass over x and the residual, TPR threads
 // a row with NC chunks of eight values each (longer rows read the rest a second time).  The sums are taken in a fixed
 // order; the inverse root is rounded once, t weight and its product with the root once each.
+// Sum over the threads of a row: a warp's in FP32, the warps' in FP64.  `part` is free again after the block's next barrier.
 template <int TPR>
-__device__ __forceinline__ double row_sum(double v, double* part) {
+__device__ __forceinline__ double row_sum(float share, double* part) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (TPR == 32) return v;
-    __syncthreads();                                           // `part` may still be read from an earlier sum
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    for (int o = 16; o > 0; o >>= 1) share += __shfl_xor_sync(0xffffffffu, share, o);
+    if (TPR == 32) return (double)share;
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = (double)share;
     __syncthreads();
-    v = (threadIdx.x & 31) < TPR / 32 ? part[threadIdx.x & 31] : 0.0;
+    double v = (threadIdx.x & 31) < TPR / 32 ? part[threadIdx.x & 31] : 0.0;
 #pragma unroll
     for (int o = TPR / 64; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return __shfl_sync(0xffffffffu, v, 0);
@@ -375,6 +375,134 @@ __device__ __forceinline__ float inverse_root(double a) {
     const float q = ah * r, qe = fmaf(ah, r, -q);
     const float e = fmaf(-q, r, 1.0f) - fmaf(qe, r, al * r * r);
     return fmaf(0.5f * r, e, r);
+}
+
+// Eight normed values of a row (chunk c) to codes and, from the first of the 16 lanes that hold a k tile, its four scale
+// bytes; called by whole warps (the chunks of a row are a multiple of 16, so those lanes are all in or all out)
+template <int FMT>
+__device__ __forceinline__ void emit_chunk(float (&o)[8], bool up, int c, bool in, uint8_t* __restrict__ cr,
+                                           uint8_t* __restrict__ tr) {
+    const int s = block_scale<FMT>(quad_max(max_bits8(o)), up);
+    const float inv = scale_inverse(s);
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] *= inv;
+    const uint2 e = encode8<FMT>(o, s == 255);
+    if (in) {
+        if (FMT == OZK_MX_E2M1)
+            *reinterpret_cast<uint32_t*>(cr + c * 4) = e.x;
+        else
+            *reinterpret_cast<uint2*>(cr + c * 8) = e;
+    }
+    uint32_t four = (uint32_t)s;
+    four |= __shfl_down_sync(0xffffffffu, four, 4) << 8;
+    four |= __shfl_down_sync(0xffffffffu, four, 8) << 16;
+    if (in && (c & 15) == 0) *reinterpret_cast<uint32_t*>(tr + (long long)(c / 16) * TILE_BYTES) = four;
+}
+
+// Eight values as they lie in memory
+template <typename T>
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                v[4 * i] = __uint_as_float(w[i].x); v[4 * i + 1] = __uint_as_float(w[i].y);
+                v[4 * i + 2] = __uint_as_float(w[i].z); v[4 * i + 3] = __uint_as_float(w[i].w);
+            }
+        } else {
+            const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 f = unpack2(u[j], (const T*)nullptr);
+                v[2 * j] = f.x;
+                v[2 * j + 1] = f.y;
+            }
+        }
+    }
+};
+
+// Many aligned rows that fit into the registers of TPR threads (d a multiple of 8, at most 8 TPR NC): CTAs stay and take
+// rows in turn, with the next row's loads under way while a row is summed and encoded, and the weights in registers.
+template <typename T, typename W, int FMT, int TPR, int NC, bool RES>
+__global__ void __launch_bounds__(TPR, 1024 / TPR)
+    rms_norm_stream_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ residual, long long res_stride,
+                           const W* __restrict__ weight, int rows, int d, double inv_d, float eps, bool up,
+                           T* __restrict__ sum, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
+    __shared__ double part[2][32];
+    const int t = threadIdx.x, full = d / 8, chunks = padded_k(d) / 8;
+    Raw8<T> rx[NC], rr[RES ? NC : 1];
+    Raw8<W> rw[NC];
+    auto fetch = [&](int row) {
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            const int c = t + i * TPR;
+            if (c < full) {
+                rx[i].load(x + row * x_stride + c * 8);
+                if (RES) rr[i].load(residual + row * res_stride + c * 8);
+            }
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NC; i++) {
+        rx[i] = {};
+        if (RES) rr[i] = {};
+        rw[i] = {};
+        if (t + i * TPR < full) rw[i].load(weight + (t + i * TPR) * 8);
+    }
+    fetch(blockIdx.x);
+    const long long pitch = code_pitch(FMT, d);
+    int turn = 0;
+    for (int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+        float v[NC][8];
+        float sq = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            rx[i].get(v[i]);
+            if (RES) {
+                float q[8];
+                rr[i].get(q);
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[i][j] += q[j];
+            }
+#pragma unroll
+            for (int j = 0; j < 8; j++) sq = fmaf(v[i][j], v[i][j], sq);
+        }
+        if (row + (int)gridDim.x < rows) fetch(row + (int)gridDim.x);
+        if (sum) {
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+                if (t + i * TPR < full) store8(sum + row * (long long)d + (t + i * TPR) * 8, true, 8, v[i]);
+        }
+        double total = row_sum<TPR>(sq, part[turn]);
+        if (!(total < 3.0e38)) {                                // squares beyond FP32: once more, scaled
+            sq = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NC; i++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const float u = v[i][j] * 0x1p-70f;
+                    sq = fmaf(u, u, sq);
+                }
+            __syncthreads();
+            total = row_sum<TPR>(sq, part[turn]) * 0x1p140;
+        }
+        const float rstd = inverse_root(total * inv_d + (double)eps);
+        uint8_t* cr = codes + row * pitch;
+        uint8_t* tr = scales + (row / TILE) * (long long)(chunks / 16) * TILE_BYTES + scale_slot(row % TILE, 0);
+#pragma unroll
+        for (int i = 0; i < NC; i++) {
+            float w[8];
+            rw[i].get(w);
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * w[j] * rstd;
+            emit_chunk<FMT>(v[i], up, t + i * TPR, t + i * TPR < chunks, cr, tr);
+        }
+    }
 }
 
 template <typename T, typename W, int FMT, int TPR, int NC>
@@ -405,7 +533,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / 
             for (int j = 0; j < 8; j++) o[j] += q[j];
         }
     };
-    // sum of f(t)^2: a thread's share in FP32, the shares in FP64
+    // sum of f(t)^2
     auto squares = [&](auto f, bool store) {
         float sq = 0.0f;
         auto note = [&](int c, const float (&o)[8]) {
@@ -424,7 +552,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / 
             fetch(c, o);
             note(c, o);
         }
-        return row_sum<TPR>((double)sq, part);
+        if (TPR > 32) __syncthreads();                         // `part` may still be read from an earlier sum
+        return row_sum<TPR>(sq, part);
     };
 #pragma unroll
     for (int i = 0; i < NC; i++)
@@ -436,27 +565,12 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / 
     const long long pitch = code_pitch(FMT, d);
     uint8_t* cr = codes + row * pitch;
     uint8_t* tr = scales + (row / TILE) * (long long)(kp / TILE) * TILE_BYTES + scale_slot((int)(row % TILE), 0);
-    // 16 lanes hold a k tile of the row (chunks is a multiple of 16, so they are all in or all out)
     auto emit = [&](int c, float (&o)[8], bool in) {
         float w[8];
         load8(weight + c * 8, in && aligned && c * 8 + 8 <= d, in ? max(0, d - c * 8) : 0, w);
 #pragma unroll
         for (int j = 0; j < 8; j++) o[j] = in ? o[j] * w[j] * rstd : 0.0f;
-        const int s = block_scale<FMT>(quad_max(max_bits8(o)), up);
-        const float inv = scale_inverse(s);
-#pragma unroll
-        for (int j = 0; j < 8; j++) o[j] *= inv;
-        const uint2 e = encode8<FMT>(o, s == 255);
-        if (in) {
-            if (FMT == OZK_MX_E2M1)
-                *reinterpret_cast<uint32_t*>(cr + c * 4) = e.x;
-            else
-                *reinterpret_cast<uint2*>(cr + c * 8) = e;
-        }
-        uint32_t four = (uint32_t)s;
-        four |= __shfl_down_sync(0xffffffffu, four, 4) << 8;
-        four |= __shfl_down_sync(0xffffffffu, four, 8) << 16;
-        if (in && (c & 15) == 0) *reinterpret_cast<uint32_t*>(tr + (long long)(c / 16) * TILE_BYTES) = four;
+        emit_chunk<FMT>(o, up, c, in, cr, tr);
     };
 #pragma unroll
     for (int i = 0; i < NC; i++) emit(t + i * TPR, v[i], t + i * TPR < chunks);
@@ -597,6 +711,7 @@ struct NormArgs {
     void* sum;
     uint8_t *codes, *scales;
     cudaStream_t st;
+    int sms;
 };
 
 template <typename T, typename W, int FMT>
@@ -612,12 +727,28 @@ int launch_norm(const NormArgs& a) {
         <<<(unsigned)((a.rows + (TPR == 32 ? 3 : 0)) / (TPR == 32 ? 4 : 1)), TPR == 32 ? 128 : TPR, 0, a.st>>>(      \
             static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), a.res_stride,                 \
             static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps, aligned, a.up, static_cast<T*>(a.sum), a.codes, a.scales)
-    if (d <= 1024) OZK_NORM(32, 4);
+#define OZK_STREAM(TPR, NC)                                                                                          \
+    {                                                                                                                \
+        const int grid = a.rows < a.sms * (1024 / TPR) ? a.rows : a.sms * (1024 / TPR);                              \
+        auto kern = a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true> : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false>; \
+        kern<<<(unsigned)grid, TPR, 0, a.st>>>(static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), \
+                                               a.res_stride, static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps,  \
+                                               a.up, static_cast<T*>(a.sum), a.codes, a.scales);                     \
+    }
+    // rows enough for every CTA to take several: the streaming kernel
+    if (aligned && d % 8 == 0 && d > 1024 && d <= 16384 && a.rows >= 4 * a.sms) {
+        if (d <= 2048) OZK_STREAM(256, 1)
+        else if (d <= 4096) OZK_STREAM(256, 2)
+        else if (d <= 8192) OZK_STREAM(512, 2)
+        else OZK_STREAM(1024, 2)
+    }
+    else if (d <= 1024) OZK_NORM(32, 4);
     else if (d <= 2048) OZK_NORM(256, 1);
     else if (d <= 4096) OZK_NORM(256, 2);
     else if (d <= 8192) OZK_NORM(512, 2);
     else OZK_NORM(1024, 2);
 #undef OZK_NORM
+#undef OZK_STREAM
     OZK_CHECK_LAUNCH();
     return OZK_OK;
 }
@@ -762,9 +893,12 @@ extern "C" int ozk_mx_rms_norm(const void* x, const void* residual, const void* 
     if (!x || !weight || !codes || !scales || !fmt_ok(fmt) || rows < 1 || d < 1 || d > OZK_MX_KMAX) return OZK_ERR_ARG;
     if (!(eps > 0.0f) || !(eps < INFINITY) || x_stride < 0 || residual_stride < 0) return OZK_ERR_ARG;
     if (!aligned16(codes) || !aligned16(scales)) return OZK_ERR_ARG;
+    int sms = 0;
+    const int rc = ozk_device_sm_count(&sms);
+    if (rc != OZK_OK) return rc;
     const NormArgs a = {x,    residual,      weight, x_stride, residual_stride, rows,
                         d,    eps,           round_up != 0,    sum,  codes,  scales,
-                        reinterpret_cast<cudaStream_t>(stream)};
+                        reinterpret_cast<cudaStream_t>(stream), sms};
     switch (dtype) {
         case OZK_F32: return dispatch_norm<float>(a, true, fmt);
         case OZK_F16: return dispatch_norm<__half>(a, weight_f32 != 0, fmt);

@@ -464,6 +464,35 @@ def test_rms_norm(pkg, name, fmt):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [1032, 2056, 4104, 8200])
+def test_rms_norm_many_rows(pkg, d):
+    """Rows enough for the kernel that streams them: the last ones against the definition, a row of NaN, one of squares
+    beyond FP32, and all of them against the same rows in small batches (another kernel, other orders of the sum)."""
+    import torch
+    rng = np.random.default_rng(23)
+    rows = 600 + d % 7
+    for name, fmt, with_res in (("bfloat16", "e4m3", True), ("float32", "e2m1", False)):
+        x, w = _put(rng.standard_normal((rows, d)), name), _put(1 + 0.1 * rng.standard_normal(d), name)
+        x[rows - 2] = 1e30
+        x[rows - 3, 9] = float("nan")
+        r = _put(rng.standard_normal((rows, d)), name) if with_res else None
+        q, s = pkg.mx_rms_norm(x, w, residual=r, fmt=fmt)
+        got = q.dequantize(torch.float32)
+        assert np.isnan(_f64(got[rows - 3])).all()
+        if with_res:
+            assert torch.equal(s.nan_to_num(), (x.float() + r.float()).to(x.dtype).nan_to_num())
+        keep = [0, 1, rows // 2, rows - 2, rows - 1]
+        _, y = _norm_want(_f64(x[keep]), _f64(w), None if r is None else _f64(r[keep]), 1e-6)
+        sub = pkg.MXMatrix.from_codes(q.codes()[keep].contiguous(), q.scales()[keep].contiguous(), fmt, d)
+        _near_codes(sub, y, fmt, "floor")
+        few = torch.cat([pkg.mx_rms_norm(x[i:i + 100], w, residual=None if r is None else r[i:i + 100], fmt=fmt)[0]
+                         .dequantize(torch.float32) for i in range(0, rows, 100)])
+        same = (few == got) | (few.isnan() & got.isnan())
+        # a sum in another order moves a value across a border between codes about once in 2^20 values
+        assert (~same).sum() <= 64 + rows * d * 2.0 ** -16
+
+
+@pytest.mark.gpu
 def test_rms_norm_views(pkg):
     """Leading axes, strided rows, rows off a 16-byte boundary, a row of NaN, an empty batch."""
     import torch
