@@ -19,10 +19,10 @@
 // Where there are fewer tiles than SMs, a cluster of CTAs shares one tile: each takes a part of K, leaves its FP32 sums
 // in its shared memory, and every CTA adds one slice of the tile over the cluster in a fixed order (no workspace, no
 // atomics, one launch).
-// Grouped: `ends` is read on the device; a group's rows are covered by the windows of A (of 128 or BN rows, at multiples
-// of that) that they touch, and each window is multiplied with the group's B and stored for the group's rows only.
-// Windows at fixed places keep A's rows where the quantisation put them, whatever the routing, for at most one more
-// tile per group than packing would need.
+// Grouped: `ends` is read on the device; a group's rows are covered by windows of A (of a tile's rows, from the multiple of
+// 128 or of the tile's rows at or before the group's first), and each window is multiplied with the group's B and stored
+// for the group's rows only.  So A's rows and scales stay where the quantisation put them, whatever the routing, for at
+// most one more tile per group than packing would need.
 // Every mbarrier wait is bounded; on a timeout the CTA records a flag in *err, stops, waits (bounded) for its own copies
 // and MMAs in flight, frees TMEM and exits.  No multicast is used.
 #include <cuda.h>
@@ -96,13 +96,16 @@ struct Args {
 };
 
 struct Unit {
-    int lt, rt;                              // tile indices
     int lg, rg;                              // group coordinates
+    int l0, r0;                              // first left and right row of the tile
     int first, last;                         // rows of A (and C) that belong to this unit's group: [first, last)
 };
 
 template <int BL, int BN, bool SWAP>
 struct Work {
+    // rows of A are taken in windows of WIN, the first of a group from a multiple of ALIGN (their scales come in tiles of
+    // 128 rows, of which a smaller window is an even part)
+    static constexpr int WIN = SWAP ? BN : BL, ALIGN = WIN < TILE ? WIN : TILE;
     const Args& a;
     const int *pre, *bound;                  // grouped: windows before group g, first row of group g
     int ltiles, rtiles;
@@ -127,17 +130,17 @@ struct Work {
             w.last = bound[lo + 1];
             const long long in = u - (long long)pre[lo] * other;
             const int nw = pre[lo + 1] - pre[lo];
-            const int win = w.first / (SWAP ? BN : BL) + (int)(in % nw), o = (int)(in / nw);
-            w.lt = SWAP ? o : win;
-            w.rt = SWAP ? win : o;
+            const int row = w.first / ALIGN * ALIGN + (int)(in % nw) * WIN, o = (int)(in / nw);
+            w.l0 = SWAP ? o * BL : row;
+            w.r0 = SWAP ? row : o * BN;
             w.lg = SWAP ? lo : 0;
             w.rg = SWAP ? 0 : lo;
         } else {
             const int per = GROUP_L * rtiles;
             const int g = (int)(u / per), l0 = g * GROUP_L, gl = min(ltiles - l0, GROUP_L);
             const int in = (int)(u - (long long)g * per);
-            w.lt = l0 + in % gl;
-            w.rt = in / gl;
+            w.l0 = (l0 + in % gl) * BL;
+            w.r0 = in / gl * BN;
             w.lg = w.rg = 0;
             w.first = 0;
             w.last = a.tokens;
@@ -291,7 +294,7 @@ __device__ __forceinline__ void store4(const Args& a, int token, int col, float4
 }
 
 // Grouped: clamp `ends` to an ascending sequence within [0, rows] and count the windows each group touches (one warp)
-template <int WIN>
+template <int WIN, int ALIGN>
 __device__ __forceinline__ void group_tables(const Args& a, int* pre, int* bound, int lane) {
     int end_before = 0, windows_before = 0;
     if (lane == 0) { pre[0] = 0; bound[0] = 0; }
@@ -306,7 +309,7 @@ __device__ __forceinline__ void group_tables(const Args& a, int* pre, int* bound
         }
         int s = __shfl_up_sync(0xffffffffu, e, 1);
         if (lane == 0) s = end_before;
-        int w = e > s ? (e - 1) / WIN - s / WIN + 1 : 0;
+        int w = e > s ? (e - s / ALIGN * ALIGN + WIN - 1) / WIN : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int p = __shfl_up_sync(0xffffffffu, w, o);
@@ -331,6 +334,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                    const __grid_constant__ CUtensorMap tmSL, const __grid_constant__ CUtensorMap tmSR,
                    const __grid_constant__ CUtensorMap tmC, const __grid_constant__ Args a, int parts) {
     using S = Shape<KIND, BN, SWAP, PAIR>;
+    using WorkOf = Work<S::BL, BN, SWAP>;
     constexpr int STAGES = S::STAGES, CHUNK = S::CHUNK;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -373,7 +377,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tmem_relinquish();
         }
     }
-    if (warp == 2 && a.groups) group_tables<SWAP ? BN : S::BL>(a, pre, bound, lane);
+    if (warp == 2 && a.groups) group_tables<WorkOf::WIN, WorkOf::ALIGN>(a, pre, bound, lane);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -381,7 +385,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const Work<S::BL, BN, SWAP> work(a, pre, bound);
+    const WorkOf work(a, pre, bound);
     // parts > 1: one unit per cluster of `parts` CTAs, each with its part of K; else units round robin over the CTAs, or
     // over the pairs, of which CTA 0 issues the MMAs
     const int rank = PAIR ? (int)cluster_ctarank() : 0;
@@ -398,7 +402,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t aL = smem_addr(sL), aR = smem_addr(sR), aSL = smem_addr(sSL), aSR = smem_addr(sSR);
         for (long long u = u0; ok && u < work.units; u += du) {
             const Unit w = work.at(u);
-            const int l0 = w.lt * S::BL + rank * BM, r0 = w.rt * BN + rank * S::RN;
+            const int l0 = w.l0 + rank * BM, r0 = w.r0 + rank * S::RN;
             for (int kb = kb0; kb < kb1; kb++) {
                 ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS);
                 if (!ok) break;
@@ -413,12 +417,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                         tma_load_3d_pair(dl, &tmL, kc, l0, w.lg, bar);
                         tma_load_3d_pair(dr, &tmR, kc, r0, w.rg, bar);
                         tma_load_4d_pair(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, w.lg, bar);
-                        tma_load_4d_pair(dsr, &tmSR, 0, kb * S::KT, w.rt * BN / TILE, w.rg, bar);
+                        tma_load_4d_pair(dsr, &tmSR, 0, kb * S::KT, w.r0 / TILE, w.rg, bar);
                     } else {
                         tma_load_3d(dl, &tmL, kc, l0, w.lg, bar);
                         tma_load_3d(dr, &tmR, kc, r0, w.rg, bar);
                         tma_load_4d(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, w.lg, bar);
-                        tma_load_4d(dsr, &tmSR, 0, kb * S::KT, w.rt * BN / TILE, w.rg, bar);
+                        tma_load_4d(dsr, &tmSR, 0, kb * S::KT, w.r0 / TILE, w.rg, bar);
                     }
                 }
                 __syncwarp();
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint32_t d_tmem = tmem + (uint32_t)(b * S::ACC_STRIDE);
                 // the second tile of 64 right rows in a scale tile starts two columns on (32 rows a column; an MMA takes
                 // its scales from an even column, so tiles of 32 rows exist for a first tile only)
-                const uint32_t r_col = BN == 64 ? (uint32_t)(w.rt & 1) * 2u : 0u;
+                const uint32_t r_col = BN == 64 ? (uint32_t)(w.r0 / BN & 1) * 2u : 0u;
                 auto columns = [&](uint32_t st) { return tmem + (uint32_t)(S::SCALE_BASE + (int)(st & 1u) * S::SCALE_COLS); };
                 // the four instructions of a stage: 32 bytes along K inside the swizzle atom each (+2 in the >> 4 address
                 // field); the last stage of an odd number of scale tiles has half of them
@@ -560,9 +564,9 @@ __global__ void __launch_bounds__(THREADS, 1)
             }
             __syncwarp();
             tc_fence_after();
-            const int l = w.lt * S::BL + rank * BM + quarter * 32 + lane;
+            const int l = w.l0 + rank * BM + quarter * 32 + lane;
             const uint32_t acc = tmem_base + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(b * S::ACC_STRIDE + half * S::HALF);
-            const int r = w.rt * BN + half * S::HALF;
+            const int r = w.r0 + half * S::HALF;
             if (!PAIR && parts > 1) {
                 float* mine = reinterpret_cast<float*>(smem);
 #pragma unroll 1
@@ -647,7 +651,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             for (int q = QUADS * part / parts + (int)threadIdx.x - 64; q < QUADS * (part + 1) / parts; q += EPI_WARPS * 32) {
                 const int line = q / (LINE / 4), at = q % (LINE / 4) * 4;
                 const uint32_t addr = base + 4u * (uint32_t)(line * PITCH + at);
-                const int token = (SWAP ? w.rt * BN : w.lt * BM) + line, col = (SWAP ? w.lt * BM : w.rt * BN) + at;
+                const int token = (SWAP ? w.r0 : w.l0) + line, col = (SWAP ? w.l0 : w.r0) + at;
                 if (token < w.first || token >= w.last || col >= a.n) continue;
                 float4 f[8];
 #pragma unroll
