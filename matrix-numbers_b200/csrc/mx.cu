@@ -893,16 +893,14 @@ extern "C" int ozk_mx_rms_norm(const void* x, const void* residual, const void* 
     if (!x || !weight || !codes || !scales || !fmt_ok(fmt) || rows < 1 || d < 1 || d > OZK_MX_KMAX) return OZK_ERR_ARG;
     if (!(eps > 0.0f) || !(eps < INFINITY) || x_stride < 0 || residual_stride < 0) return OZK_ERR_ARG;
     if (!aligned16(codes) || !aligned16(scales)) return OZK_ERR_ARG;
+    if (dtype != OZK_F32 && dtype != OZK_F16 && dtype != OZK_BF16) return OZK_ERR_ARG;
     int sms = 0;
     const int rc = ozk_device_sm_count(&sms);
     if (rc != OZK_OK) return rc;
     const NormArgs a = {x,    residual,      weight, x_stride, residual_stride, rows,
                         d,    eps,           round_up != 0,    sum,  codes,  scales,
                         reinterpret_cast<cudaStream_t>(stream), sms};
-    switch (dtype) {
-        case OZK_F32: return dispatch_norm<float>(a, true, fmt);
-        case OZK_F16: return dispatch_norm<__half>(a, weight_f32 != 0, fmt);
-        case OZK_BF16: return dispatch_norm<__nv_bfloat16>(a, weight_f32 != 0, fmt);
-        default: return OZK_ERR_ARG;
-    }
+    if (dtype == OZK_F32) return dispatch_norm<float>(a, true, fmt);
+    if (dtype == OZK_F16) return dispatch_norm<__half>(a, weight_f32 != 0, fmt);
+    return dispatch_norm<__nv_bfloat16>(a, weight_f32 != 0, fmt);
 }

@@ -33,6 +33,7 @@ MAX_GROUPS = 1024
 KMAX = 1 << 28
 _INT_MAX = 2 ** 31 - 1
 
+_empty, _uint8, _Tensor = torch.empty, torch.uint8, torch.Tensor
 _current_device = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream    # handle of a device's current stream
 _error_words = {}                # device index -> int32 word that the products' launches OR their flags into
@@ -58,6 +59,14 @@ def _operand_bytes(code, groups, rows, k):
         raise ValueError(f"operand of {groups} x {rows} x {k} elements is too large")
     codes = groups * rows * kt * (TILE if code else TILE // 2)
     return codes, codes + groups * rt * kt * TILE_BYTES
+
+
+def _new_operand(fmt, code, groups, rows, k, device):
+    """MXMatrix(fmt, groups, rows, k, device) for a format whose code is known."""
+    code_bytes, total = _operand_bytes(code, 1 if groups is None else groups, rows, k)
+    out = object.__new__(MXMatrix)
+    out._take(fmt, code, groups, rows, k, device, code_bytes, _empty(total, dtype=_uint8, device=_DEVICES[device]))
+    return out
 
 
 def _padded(k: int) -> int:
@@ -111,9 +120,10 @@ def _dtype(dtype, what):
 
 
 def _tensor(t, what):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+    if not isinstance(t, _Tensor) or not t.is_cuda:
         raise ValueError(f"{what}: CUDA tensor required (there is no CPU path)")
-    return _dtype(t.dtype, what)
+    code = _DTYPES.get(t.dtype)
+    return _dtype(t.dtype, what) if code is None else code
 
 
 class MXMatrix:
@@ -126,21 +136,19 @@ class MXMatrix:
         """An operand with uninitialised contents."""
         code = _format(fmt)
         code_bytes, total = _operand_bytes(code, 1 if groups is None else groups, rows, k)
-        self._take(fmt, code, groups, rows, k, device, code_bytes,
-                   torch.empty(total, dtype=torch.uint8, device=_DEVICES[device]))
+        self._take(fmt, code, groups, rows, k, device, code_bytes, _empty(total, dtype=_uint8, device=_DEVICES[device]))
 
     def _take(self, fmt, code, groups, rows, k, device, code_bytes, buffer):
-        self.fmt, self._fmt, self.groups, self.rows, self.k, self.device = fmt, code, groups, rows, k, device
-        self._buffer, self._code_bytes = buffer, code_bytes
+        self.fmt = fmt
+        self._fmt = code
+        self.groups = groups
+        self.rows = rows
+        self.k = k
+        self.device = device
+        self._buffer = buffer
+        self._code_bytes = code_bytes
         self._code_ptr = p = buffer.data_ptr()               # one allocation: the codes, then the scales
         self._scale_ptr = p + code_bytes
-
-    @classmethod
-    def _over(cls, fmt, rows, k, device, buffer):
-        """The plain operand that ``buffer`` holds."""
-        out, code = object.__new__(cls), FORMATS[fmt]
-        out._take(fmt, code, None, rows, k, device, _operand_bytes(code, 1, rows, k)[0], buffer)
-        return out
 
     @property
     def shape(self):
@@ -210,7 +218,7 @@ class MXMatrix:
         if _current_device() != device:
             with torch.cuda.device(device):
                 return self.dequantize(dtype)
-        out = torch.empty(self.shape, dtype=dtype, device=_DEVICES[device])
+        out = _empty(self.shape, dtype=dtype, device=_DEVICES[device])
         if self.rows and self.groups != 0:
             rc = _lib.lib().ozk_mx_dequantize(self._code_ptr, self._scale_ptr, self._fmt, self.groups or 1, self.rows,
                                               self.k, out.data_ptr(), d, _stream_of(device))
@@ -231,24 +239,24 @@ def mx_quantize(x, fmt="e2m1", axis=-1, rule="floor"):
     code, up = _format(fmt), _rule(rule)
     shape, stride = x.shape, x.stride()
     dim = len(shape)
-    if dim not in (2, 3):
-        raise ValueError(f"x: 2 or 3 axes required, not {dim}")
-    if not -2 <= axis < dim:
-        raise ValueError(f"axis {axis} out of range for {dim} axes")
-    at = axis % dim
-    if at < dim - 2:
-        raise ValueError("the groups of x cannot be contracted: axis is one of the last two")
+    if dim == 2 and -2 <= axis < 2:
+        at, other, groups, group_stride = axis & 1, 1 - (axis & 1), None, 0
+    elif dim == 3 and axis in (-1, -2, 1, 2):
+        at = axis % 3
+        other, groups, group_stride = 3 - at, shape[0], stride[0]
+    else:
+        if dim not in (2, 3):
+            raise ValueError(f"x: 2 or 3 axes required, not {dim}")
+        raise ValueError(f"axis {axis} of {dim}: one of the last two is contracted")
     device = x.get_device()
     if _current_device() != device:
         with torch.cuda.device(device):
             return mx_quantize(x, fmt, axis, rule)
-    other = 2 * dim - 3 - at
     rows, k = shape[other], shape[at]
-    groups = shape[0] if dim == 3 else None
-    out = MXMatrix(fmt, groups, rows, k, device)
+    out = _new_operand(fmt, code, groups, rows, k, device)
     if rows and groups != 0:
-        rc = _lib.lib().ozk_mx_quantize(x.data_ptr(), d, groups or 1, rows, k, stride[0] if dim == 3 else 0,
-                                        stride[other], stride[at], code, up, out._code_ptr, out._scale_ptr,
+        rc = _lib.lib().ozk_mx_quantize(x.data_ptr(), d, groups or 1, rows, k, group_stride, stride[other],
+                                        stride[at], code, up, out._code_ptr, out._scale_ptr,
                                         _stream_of(device))
         if rc:
             check(rc, "ozk_mx_quantize")
@@ -269,7 +277,8 @@ def mx_quantize_both(x, fmt="e4m3", rule="floor"):
     rows, cols = x.shape
     if not rows or not cols:
         raise ValueError("x: both axes are contracted in turn and cannot be empty")
-    along_rows, along_cols = MXMatrix(fmt, None, rows, cols, device), MXMatrix(fmt, None, cols, rows, device)
+    along_rows = _new_operand(fmt, code, None, rows, cols, device)
+    along_cols = _new_operand(fmt, code, None, cols, rows, device)
     rc = _lib.lib().ozk_mx_quantize_both(x.data_ptr(), d, rows, cols, x.stride(0), x.stride(1), code, up,
                                          along_rows._code_ptr, along_cols._code_ptr, _stream_of(device))
     if rc:
@@ -291,8 +300,10 @@ def _operands(A, B):
 def _result(C, rows, cols, dtype, device):
     """The output tensor, its dtype code and row stride."""
     if C is None:
-        d = _dtype(dtype, "dtype")
-        return torch.empty((rows, cols), dtype=dtype, device=_DEVICES[device]), d, cols or 1
+        d = _DTYPES.get(dtype)
+        if d is None:
+            d = _dtype(dtype, "dtype")
+        return _empty((rows, cols), dtype=dtype, device=_DEVICES[device]), d, cols or 1
     d = _tensor(C, "C")
     if C.device.index != device or tuple(C.shape) != (rows, cols) or (cols > 1 and C.stride(1) != 1) \
             or (rows > 1 and C.stride(0) < cols):
@@ -358,27 +369,27 @@ def mx_rms_norm(x, weight, residual=None, eps=1e-6, fmt="e4m3", rule="floor"):
     if not shape:
         raise ValueError("x: at least one axis required")
     n = shape[-1]
-    if not isinstance(weight, torch.Tensor) or weight.device != x.device or weight.dim() != 1 or weight.shape[0] != n \
-            or not (weight.dtype == x.dtype or weight.dtype == torch.float32) or not weight.is_contiguous():
+    device, dtype = x.get_device(), x.dtype
+    if not isinstance(weight, _Tensor) or weight.get_device() != device or weight.shape != shape[-1:] \
+            or not (weight.dtype is dtype or weight.dtype is torch.float32) or not weight.is_contiguous():
         raise ValueError(f"weight: contiguous ({n},) tensor of x's type or float32 on its device required")
     if not 0.0 < eps < float("inf"):
         raise ValueError(f"eps {eps}: a positive number required")
-    if residual is not None and (not isinstance(residual, torch.Tensor) or residual.shape != shape
-                                 or residual.dtype != x.dtype or residual.device != x.device):
+    if residual is not None and (not isinstance(residual, _Tensor) or residual.shape != shape
+                                 or residual.dtype is not dtype or residual.get_device() != device):
         raise ValueError("residual: a tensor of x's shape, type and device required")
-    device = x.get_device()
     if _current_device() != device:
         with torch.cuda.device(device):
             return mx_rms_norm(x, weight, residual, eps, fmt, rule)
-    x2 = _rows(x, n)
+    x2 = x if len(shape) == 2 and x.stride(1) == 1 else _rows(x, n)
     rows = x2.shape[0]
-    out = MXMatrix(fmt, None, rows, n, device)
+    out = _new_operand(fmt, code, None, rows, n, device)
     r_ptr = r_stride = t_ptr = 0
     total = None
     if residual is not None:
-        r2 = _rows(residual, n)
+        r2 = residual if len(shape) == 2 and residual.stride(1) == 1 else _rows(residual, n)
         r_ptr, r_stride = r2.data_ptr(), r2.stride(0)
-        total = torch.empty(shape, dtype=x.dtype, device=_DEVICES[device])
+        total = _empty(shape, dtype=dtype, device=_DEVICES[device])
         t_ptr = total.data_ptr()
     if rows:
         rc = _lib.lib().ozk_mx_rms_norm(x2.data_ptr(), r_ptr, weight.data_ptr(), d, weight.dtype == torch.float32, rows,
@@ -393,62 +404,79 @@ def _rows(x, n):
     """x as a matrix of rows of length n >= 1 with contiguous elements: x itself or a view where it can be."""
     if x.dim() != 2:
         x = x.reshape(x.numel() // max(n, 1), n)
-    return x if n < 2 or x.stride(1) == 1 else x.contiguous()
+    return x if x.stride(1) == 1 or n < 2 else x.contiguous()
 
 
-def _linear_forward(x2, weight, fmt, rule, need_dx, need_dw):
+def _linear_forward(x2, weight, code, up, need_dx, need_dw):
     """y and the operands that the backward pass takes: x along its rows where dweight is wanted, weight along n where
     dx is."""
     device = x2.get_device()
     m, k = x2.shape
     n = weight.shape[0]
-    code = FORMATS[fmt]
     xk, wk = _operand_bytes(code, 1, m, k)[1], _operand_bytes(code, 1, n, k)[1]
     dev = _DEVICES[device]
-    y = torch.empty((m, n), dtype=x2.dtype, device=dev)
-    scratch = torch.empty(xk + wk, dtype=torch.uint8, device=dev)
-    xm = torch.empty(_operand_bytes(code, 1, k, m)[1], dtype=torch.uint8, device=dev) if need_dw else None
-    wn = torch.empty(_operand_bytes(code, 1, k, n)[1], dtype=torch.uint8, device=dev) if need_dx else None
+    xm = wn = None
+    xm_ptr = wn_ptr = 0
+    if need_dw:
+        xm = _empty(_operand_bytes(code, 1, k, m)[1], dtype=_uint8, device=dev)
+        xm_ptr = xm.data_ptr()
+    if need_dx:
+        wn = _empty(_operand_bytes(code, 1, k, n)[1], dtype=_uint8, device=dev)
+        wn_ptr = wn.data_ptr()
+    y = _empty((m, n), dtype=x2.dtype, device=dev)
+    scratch = _empty(xk + wk, dtype=_uint8, device=dev)
     p = scratch.data_ptr()
-    rc = _lib.lib().ozk_mx_linear_forward(x2.data_ptr(), _DTYPES[x2.dtype], *x2.stride(), weight.data_ptr(),
-                                          _DTYPES[weight.dtype], *weight.stride(), m, n, k, code, RULES[rule], p, p + xk,
-                                          xm.data_ptr() if need_dw else 0, wn.data_ptr() if need_dx else 0, y.data_ptr(),
-                                          _error_word(device), _stream_of(device))
+    x_row, x_col = x2.stride()
+    w_row, w_col = weight.stride()
+    rc = _lib.lib().ozk_mx_linear_forward(x2.data_ptr(), _DTYPES[x2.dtype], x_row, x_col, weight.data_ptr(),
+                                          _DTYPES[weight.dtype], w_row, w_col, m, n, k, code, up, p, p + xk, xm_ptr, wn_ptr,
+                                          y.data_ptr(), _error_word(device), _stream_of(device))
     if rc:
         check(rc, "ozk_mx_linear_forward")
     return y, xm, wn
 
 
+def _linear_backward(ctx, dy):
+    xm, wn = ctx.saved_tensors
+    code, up, x_code, w_code, w_dtype, n, k = ctx.how
+    device, m = dy.get_device(), dy.shape[0]
+    dev = _DEVICES[device]
+    along_n, along_m = _operand_bytes(code, 1, m, n)[1], _operand_bytes(code, 1, n, m)[1]
+    dx = dw = None
+    dx_ptr = dw_ptr = xm_ptr = wn_ptr = 0
+    if wn is not None:
+        dx = _empty((m, k), dtype=dy.dtype, device=dev)        # y, and so dy, has the type of x
+        dx_ptr, wn_ptr = dx.data_ptr(), wn.data_ptr()
+    if xm is not None:
+        dw = _empty((n, k), dtype=w_dtype, device=dev)
+        dw_ptr, xm_ptr = dw.data_ptr(), xm.data_ptr()
+    scratch = _empty(along_n + along_m, dtype=_uint8, device=dev)
+    p = scratch.data_ptr()
+    row_stride, col_stride = dy.stride()
+    rc = _lib.lib().ozk_mx_linear_backward(dy.data_ptr(), x_code, row_stride, col_stride, xm_ptr, wn_ptr, m, n, k, code, up,
+                                           p, p + along_n, dx_ptr, x_code, dw_ptr, w_code, _error_word(device),
+                                           _stream_of(device))
+    if rc:
+        check(rc, "ozk_mx_linear_backward")
+    return dx, dw, None, None
+
+
+_linear_backward_once = torch.autograd.function.once_differentiable(_linear_backward)
+
+
 class _MXLinear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, fmt, rule):
+    def forward(ctx, x, weight, code, up):
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        y, xm, wn = _linear_forward(x, weight, fmt, rule, need_dx, need_dw)
+        y, xm, wn = _linear_forward(x, weight, code, up, need_dx, need_dw)
         ctx.save_for_backward(xm, wn)
-        ctx.how = (fmt, rule, x.dtype, weight.dtype, weight.shape)
+        ctx.how = (code, up, _DTYPES[x.dtype], _DTYPES[weight.dtype], weight.dtype, *weight.shape)
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        xm, wn = ctx.saved_tensors
-        fmt, rule, x_dtype, w_dtype, (n, k) = ctx.how
-        need_dx, need_dw = ctx.needs_input_grad[:2]
-        device, m = dy.get_device(), dy.shape[0]
-        code, dev = FORMATS[fmt], _DEVICES[device]
-        dx = torch.empty((m, k), dtype=x_dtype, device=dev) if need_dx else None
-        dw = torch.empty((n, k), dtype=w_dtype, device=dev) if need_dw else None
-        along_n, along_m = _operand_bytes(code, 1, m, n)[1], _operand_bytes(code, 1, n, m)[1]
-        scratch = torch.empty(along_n + along_m, dtype=torch.uint8, device=dev)
-        p = scratch.data_ptr()
-        rc = _lib.lib().ozk_mx_linear_backward(dy.data_ptr(), _DTYPES[dy.dtype], *dy.stride(),
-                                               xm.data_ptr() if need_dw else 0, wn.data_ptr() if need_dx else 0, m, n, k,
-                                               code, RULES[rule], p, p + along_n, dx.data_ptr() if need_dx else 0,
-                                               _DTYPES[x_dtype], dw.data_ptr() if need_dw else 0, _DTYPES[w_dtype],
-                                               _error_word(device), _stream_of(device))
-        if rc:
-            check(rc, "ozk_mx_linear_backward")
-        return dx, dw, None, None
+        # under create_graph the gradients must say that they cannot be differentiated again
+        return _linear_backward_once(ctx, dy) if torch.is_grad_enabled() else _linear_backward(ctx, dy)
 
 
 def mx_linear(x, weight, fmt="e4m3", rule="floor"):
@@ -460,27 +488,26 @@ def mx_linear(x, weight, fmt="e4m3", rule="floor"):
     what torch needs of any: no eager graph of the same leaves alive on another stream."""
     _tensor(x, "x")
     _tensor(weight, "weight")
-    _format(fmt)
-    _rule(rule)
-    shape = x.shape
-    if weight.dim() != 2 or not shape or shape[-1] != weight.shape[1] or x.device != weight.device:
-        raise ValueError(f"x (..., k) and weight (n, k) on one device required, not {tuple(shape)} and "
-                         f"{tuple(weight.shape)}")
-    n, k = weight.shape
+    code, up = _format(fmt), _rule(rule)
+    shape, w_shape = x.shape, weight.shape
     device = x.get_device()
+    if len(w_shape) != 2 or not shape or shape[-1] != w_shape[1] or device != weight.get_device():
+        raise ValueError(f"x (..., k) and weight (n, k) on one device required, not {tuple(shape)} and {tuple(w_shape)}")
     if _current_device() != device:
         with torch.cuda.device(device):
             return mx_linear(x, weight, fmt, rule)
-    for rows, length in ((x.numel() // max(k, 1), k), (n, k)):
-        _operand_bytes(0, 1, rows, length)                    # refuses an empty k and sizes beyond the operands'
-    if x.numel() == 0 or n == 0:
+    n, k = w_shape
+    if k == 0:
+        raise ValueError("contracted axis of length 0: at least 1 required")
+    if n == 0 or x.numel() == 0:
         return torch.matmul(x, weight.t().to(x.dtype))        # nothing to multiply: empty, with its gradients of zero
-    x2 = x if len(shape) == 2 else x.reshape(-1, k)
-    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
-        y = _MXLinear.apply(x2, weight, fmt, rule)
+    plain = len(shape) == 2
+    x2 = x if plain else x.reshape(-1, k)
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+        y = _MXLinear.apply(x2, weight, code, up)
     else:
-        y = _linear_forward(x2, weight, fmt, rule, False, False)[0]
-    return y if len(shape) == 2 else y.view(*shape[:-1], n)
+        y = _linear_forward(x2, weight, code, up, False, False)[0]
+    return y if plain else y.view(*shape[:-1], n)
 
 
 __all__ = ["MXMatrix", "mx_quantize", "mx_quantize_both", "mx_matmul", "mx_grouped_matmul", "mx_rms_norm", "mx_linear", "mx_check_errors"]
