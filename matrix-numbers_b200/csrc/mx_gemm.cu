@@ -349,7 +349,10 @@ __global__ void __launch_bounds__(THREADS, 1)
     int* pre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 256);
     int* bound = pre + OZK_MX_MAX_GROUPS + 1;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // one value a warp, in a form that the compiler knows as such: the branches and loops that hang on it keep the operands
+    // of the issuing warps in uniform registers
+    auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const int warp = uniform((int)threadIdx.x >> 5), lane = threadIdx.x & 31;
     const uint32_t bar0 = smem_addr(bars);
     auto full_bar = [&](int s) { return bar0 + 8u * (uint32_t)s; };
     auto empty_bar = [&](int s) { return bar0 + 8u * (uint32_t)(STAGES + s); };
@@ -385,11 +388,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
-    const WorkOf work(a, pre, bound);
+    WorkOf work(a, pre, bound);
+    work.units = (long long)(uint32_t)uniform((int)work.units) | (long long)uniform((int)(work.units >> 32)) << 32;
     // parts > 1: one unit per cluster of `parts` CTAs, each with its part of K; else units round robin over the CTAs, or
     // over the pairs, of which CTA 0 issues the MMAs
-    const int rank = PAIR ? (int)cluster_ctarank() : 0;
-    const int part = !PAIR && parts > 1 ? (int)cluster_ctarank() : 0;
+    const int rank = PAIR ? uniform((int)cluster_ctarank()) : 0;
+    const int part = !PAIR && parts > 1 ? uniform((int)cluster_ctarank()) : 0;
     const long long u0 = blockIdx.x / (parts * S::CTAS), du = gridDim.x / (parts * S::CTAS);
     const int kb0 = (int)((long long)a.kblocks * part / parts), kb1 = (int)((long long)a.kblocks * (part + 1) / parts);
 
@@ -402,7 +406,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         const uint32_t aL = smem_addr(sL), aR = smem_addr(sR), aSL = smem_addr(sSL), aSR = smem_addr(sSR);
         for (long long u = u0; ok && u < work.units; u += du) {
             const Unit w = work.at(u);
-            const int l0 = w.l0 + rank * BM, r0 = w.r0 + rank * S::RN;
+            const int l0 = uniform(w.l0) + rank * BM, rt = uniform(w.r0), r0 = rt + rank * S::RN;
+            const int lg = uniform(w.lg), rg = uniform(w.rg);
             for (int kb = kb0; kb < kb1; kb++) {
                 ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS);
                 if (!ok) break;
@@ -414,15 +419,15 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const uint32_t dl = aL + stage * S::L_BYTES, dr = aR + stage * S::R_BYTES;
                     const uint32_t dsl = aSL + stage * S::SL_BYTES, dsr = aSR + stage * S::SR_BYTES;
                     if (PAIR) {
-                        tma_load_3d_pair(dl, &tmL, kc, l0, w.lg, bar);
-                        tma_load_3d_pair(dr, &tmR, kc, r0, w.rg, bar);
-                        tma_load_4d_pair(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, w.lg, bar);
-                        tma_load_4d_pair(dsr, &tmSR, 0, kb * S::KT, w.r0 / TILE, w.rg, bar);
+                        tma_load_3d_pair(dl, &tmL, kc, l0, lg, bar);
+                        tma_load_3d_pair(dr, &tmR, kc, r0, rg, bar);
+                        tma_load_4d_pair(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, lg, bar);
+                        tma_load_4d_pair(dsr, &tmSR, 0, kb * S::KT, rt / TILE, rg, bar);
                     } else {
-                        tma_load_3d(dl, &tmL, kc, l0, w.lg, bar);
-                        tma_load_3d(dr, &tmR, kc, r0, w.rg, bar);
-                        tma_load_4d(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, w.lg, bar);
-                        tma_load_4d(dsr, &tmSR, 0, kb * S::KT, w.r0 / TILE, w.rg, bar);
+                        tma_load_3d(dl, &tmL, kc, l0, lg, bar);
+                        tma_load_3d(dr, &tmR, kc, r0, rg, bar);
+                        tma_load_4d(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, lg, bar);
+                        tma_load_4d(dsr, &tmSR, 0, kb * S::KT, rt / TILE, rg, bar);
                     }
                 }
                 __syncwarp();
@@ -447,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             int stage = 0, before = 0;
             uint32_t phase = 0, it = 0, step = 0;
             bool ok = true;
-            const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_base, 0);
+            const uint32_t tmem = (uint32_t)uniform((int)tmem_base);
             // descriptors: the address part advances with the stage, the rest is constant
             const uint64_t dL = umma_desc_sw128(smem_addr(sL)), dR = umma_desc_sw128(smem_addr(sR));
             const uint64_t dSL = smem_desc_scales(smem_addr(sSL)), dSR = smem_desc_scales(smem_addr(sSR));
@@ -460,7 +465,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                 }
             };
             for (long long u = u0; ok && u < work.units; u += du) {
-                const Unit w = work.at(u);
                 const int b = (int)(it & 1u);
                 if (it >= (uint32_t)S::LAG) {
                     const uint32_t bar = S::LAG == 1 ? acce_bar(0) : acce_bar(b);
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const uint32_t d_tmem = tmem + (uint32_t)(b * S::ACC_STRIDE);
                 // the second tile of 64 right rows in a scale tile starts two columns on (32 rows a column; an MMA takes
                 // its scales from an even column, so tiles of 32 rows exist for a first tile only)
-                const uint32_t r_col = BN == 64 ? (uint32_t)(w.r0 / BN & 1) * 2u : 0u;
+                const uint32_t r_col = BN == 64 ? (uint32_t)uniform(work.at(u).r0 / BN & 1) * 2u : 0u;
                 auto columns = [&](uint32_t st) { return tmem + (uint32_t)(S::SCALE_BASE + (int)(st & 1u) * S::SCALE_COLS); };
                 // the four instructions of a stage: 32 bytes along K inside the swizzle atom each (+2 in the >> 4 address
                 // field); the last stage of an odd number of scale tiles has half of them
