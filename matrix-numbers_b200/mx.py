@@ -408,21 +408,21 @@ def _rows(x, n):
 
 
 def _linear_forward(x2, weight, code, up, need_dx, need_dw):
-    """y and the operands that the backward pass takes: x along its rows where dweight is wanted, weight along n where
-    dx is."""
+    """y and what the backward pass takes, or None: one buffer of the weight along n (where dx is wanted) and of x along
+    its rows (where dweight is)."""
     device = x2.get_device()
     m, k = x2.shape
     n = weight.shape[0]
     xk, wk = _operand_bytes(code, 1, m, k)[1], _operand_bytes(code, 1, n, k)[1]
     dev = _DEVICES[device]
-    xm = wn = None
-    xm_ptr = wn_ptr = 0
-    if need_dw:
-        xm = _empty(_operand_bytes(code, 1, k, m)[1], dtype=_uint8, device=dev)
-        xm_ptr = xm.data_ptr()
-    if need_dx:
-        wn = _empty(_operand_bytes(code, 1, k, n)[1], dtype=_uint8, device=dev)
-        wn_ptr = wn.data_ptr()
+    kept = None
+    wn_ptr = xm_ptr = 0
+    if need_dx or need_dw:
+        wn = _operand_bytes(code, 1, k, n)[1] if need_dx else 0
+        xm = _operand_bytes(code, 1, k, m)[1] if need_dw else 0
+        kept = _empty(wn + xm, dtype=_uint8, device=dev)
+        p = kept.data_ptr()
+        wn_ptr, xm_ptr = p if need_dx else 0, p + wn if need_dw else 0
     y = _empty((m, n), dtype=x2.dtype, device=dev)
     scratch = _empty(xk + wk, dtype=_uint8, device=dev)
     p = scratch.data_ptr()
@@ -433,23 +433,25 @@ def _linear_forward(x2, weight, code, up, need_dx, need_dw):
                                           y.data_ptr(), _error_word(device), _stream_of(device))
     if rc:
         check(rc, "ozk_mx_linear_forward")
-    return y, xm, wn
+    return y, kept
 
 
 def _linear_backward(ctx, dy):
-    xm, wn = ctx.saved_tensors
-    code, up, x_code, w_code, w_dtype, n, k = ctx.how
+    kept, = ctx.saved_tensors
+    code, up, need_dx, need_dw, x_code, w_code, w_dtype, n, k = ctx.how
     device, m = dy.get_device(), dy.shape[0]
     dev = _DEVICES[device]
     along_n, along_m = _operand_bytes(code, 1, m, n)[1], _operand_bytes(code, 1, n, m)[1]
     dx = dw = None
     dx_ptr = dw_ptr = xm_ptr = wn_ptr = 0
-    if wn is not None:
+    p = kept.data_ptr()
+    if need_dx:
         dx = _empty((m, k), dtype=dy.dtype, device=dev)        # y, and so dy, has the type of x
-        dx_ptr, wn_ptr = dx.data_ptr(), wn.data_ptr()
-    if xm is not None:
+        dx_ptr, wn_ptr = dx.data_ptr(), p
+        p += _operand_bytes(code, 1, k, n)[1]
+    if need_dw:
         dw = _empty((n, k), dtype=w_dtype, device=dev)
-        dw_ptr, xm_ptr = dw.data_ptr(), xm.data_ptr()
+        dw_ptr, xm_ptr = dw.data_ptr(), p
     scratch = _empty(along_n + along_m, dtype=_uint8, device=dev)
     p = scratch.data_ptr()
     row_stride, col_stride = dy.stride()
@@ -468,9 +470,9 @@ class _MXLinear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, code, up):
         need_dx, need_dw = ctx.needs_input_grad[:2]
-        y, xm, wn = _linear_forward(x, weight, code, up, need_dx, need_dw)
-        ctx.save_for_backward(xm, wn)
-        ctx.how = (code, up, _DTYPES[x.dtype], _DTYPES[weight.dtype], weight.dtype, *weight.shape)
+        y, kept = _linear_forward(x, weight, code, up, need_dx, need_dw)
+        ctx.save_for_backward(kept)
+        ctx.how = (code, up, need_dx, need_dw, _DTYPES[x.dtype], _DTYPES[weight.dtype], weight.dtype, *weight.shape)
         return y
 
     @staticmethod
