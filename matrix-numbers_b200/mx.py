@@ -14,7 +14,8 @@ and one scale byte s per block of 32 along the contracted axis (255: the block h
 everything it touches is NaN).  Any sizes; the operands are laid out for the tensor cores once, by the quantisation.
 
 All calls are enqueued on the current stream of the operand's device and may be captured in a CUDA graph (after one
-eager call on that device).  A product whose bounded waits ran out leaves a flag that ``mx_check_errors`` raises.
+eager product on that device).  A product whose bounded waits ran out leaves a flag that ``mx_check_errors`` raises.
+Only ``mx_linear`` has gradients; the other results carry none, whatever their inputs require.
 """
 from __future__ import annotations
 
@@ -160,6 +161,11 @@ class MXMatrix:
     @property
     def _g(self):
         return 1 if self.groups is None else self.groups
+
+    def record_stream(self, stream):
+        """As ``torch.Tensor.record_stream``: the operand is also used on ``stream``, so its memory is not handed out again
+        before the work there is done."""
+        self._buffer.record_stream(stream)
 
     def codes(self):
         """The element codes as uint8 (..., rows, ceil(k / 2)) for e2m1 (two a byte, the even one in the lower half)

@@ -595,6 +595,30 @@ def test_linear_shared_and_partial(pkg):
         g.sum().backward()
 
 
+@pytest.mark.gpu
+def test_linear_other_forms(pkg):
+    """A vector, a transposed and a wider weight, an input that needs no gradient: equal to the plain call or its parts."""
+    import torch
+    rng = np.random.default_rng(24)
+    x, w = _put(rng.standard_normal((30, 72)), "bfloat16"), _put(rng.standard_normal((40, 72)), "bfloat16")
+    y = pkg.mx_linear(x, w)
+    assert torch.equal(pkg.mx_linear(x[3], w), pkg.mx_linear(x[3:4], w)[0])
+    assert torch.equal(pkg.mx_linear(x, w.t().contiguous().t()), y) and torch.equal(pkg.mx_linear(x, w.float()), y)
+    assert torch.equal(pkg.mx_linear(x.t().contiguous().t(), w), y)
+    assert torch.equal(y, pkg.mx_matmul(pkg.mx_quantize(x, "e4m3"), pkg.mx_quantize(w, "e4m3")))
+    dy = _put(rng.standard_normal((30, 40)), "bfloat16")
+    grads = []
+    for need_x, need_w, weight in ((True, True, w), (True, False, w), (False, True, w), (True, True, w.float())):
+        xx, ww = x.clone().requires_grad_(need_x), weight.clone().requires_grad_(need_w)
+        pkg.mx_linear(xx, ww).backward(dy)
+        grads.append((xx.grad, ww.grad))
+    (dx, dw), (dx1, none), (none2, dw1), (dx2, dw2) = grads
+    assert none is None and none2 is None and torch.equal(dx, dx1) and torch.equal(dw, dw1) and torch.equal(dx, dx2)
+    assert dw2.dtype == torch.float32 and torch.equal(dw2.bfloat16(), dw)
+    with torch.no_grad():
+        assert not pkg.mx_linear(x.clone().requires_grad_(), w).requires_grad
+
+
 # ---- as they are used together --------------------------------------------------------------------------------------
 def _block(pkg, x, h, gain, W1, experts, ends):
     import torch
@@ -706,6 +730,123 @@ def test_linear_captured(pkg):
         with torch.no_grad():
             x.mul_(-1.5)
             dy.add_(0.25)
+
+
+@pytest.mark.gpu
+def test_threads(pkg):
+    """Calls from several host threads at once, each on its own stream."""
+    import threading
+    import torch
+    x, h, gain, W1, E, ends = _block_inputs(pkg, 70, 25)
+    want = _block(pkg, x, h, gain, W1, E, ends)
+    torch.cuda.synchronize()
+    bad = []
+
+    def work():
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            for _ in range(20):
+                got = _block(pkg, x, h, gain, W1, E, ends)
+                s.synchronize()
+                if not (torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])):
+                    bad.append(1)
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
+    pkg.mx_check_errors()
+
+
+@pytest.mark.gpu
+def test_stream_recorded(pkg):
+    """An operand used on another stream keeps its memory until that stream is done with it."""
+    import torch
+    A = pkg.mx_quantize(torch.ones(256, 256, device="cuda"))
+    want = pkg.mx_matmul(A, A)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(20_000_000)                            # about 10 ms
+        got = pkg.mx_matmul(A, A)
+    A.record_stream(s)
+    del A
+    junk = [pkg.mx_quantize(torch.full((256, 256), 3.0, device="cuda")) for _ in range(8)]
+    torch.cuda.synchronize()
+    assert torch.equal(got, want) and len(junk) == 8
+
+
+@pytest.mark.gpu
+def test_empty_operands(pkg):
+    import torch
+    for shape in ((0, 64), (3, 0, 64), (0, 5, 64)):
+        q = pkg.mx_quantize(torch.empty(shape, device="cuda"), "e2m1")
+        assert q.codes().shape == (*shape[:-1], 32) and q.scales().shape == (*shape[:-1], 2)
+        assert q.dequantize().shape == shape
+        r = pkg.MXMatrix.from_codes(q.codes(), q.scales(), "e2m1")
+        assert r.shape == shape
+    a, b = pkg.mx_quantize(torch.empty(0, 64, device="cuda")), pkg.mx_quantize(torch.ones(5, 64, device="cuda"))
+    assert pkg.mx_matmul(a, b).shape == (0, 5) and pkg.mx_matmul(b, a).shape == (5, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("axis", [0, 1])
+def test_quantize_beyond_32_bit_offsets(pkg, axis):
+    """More than 2^32 bytes and 2^31 elements: the last vectors, whose offsets pass 32 bits, against the definition."""
+    import torch
+    rows, k = 2 ** 15 + 3, 2 ** 16 + 64                          # 2.15e9 values
+    x = torch.zeros((rows, k) if axis == 1 else (k, rows), dtype=torch.bfloat16, device="cuda")
+    last = x[-3:] if axis == 1 else x[:, -3:]
+    rng = np.random.default_rng(26)
+    last.copy_(_put(rng.standard_normal(tuple(last.shape)), "bfloat16"))
+    q = pkg.mx_quantize(x, "e4m3", axis=axis)
+    want = _f64(last) if axis == 1 else _f64(last).T
+    del x
+    codes, scales = R.quantize(want, "e4m3")
+    pitch = -(-k // 128) * 128
+    got = q._buffer[:rows * pitch].view(rows, pitch)[-3:, :k]
+    np.testing.assert_array_equal(got.cpu().numpy(), codes)
+    np.testing.assert_array_equal(q.scales()[-3:].cpu().numpy(), scales)
+    del got, q
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_product_beyond_32_bit_offsets(pkg):
+    """A C of more than 2^32 bytes: its corners, and a grouped one's last rows."""
+    import torch
+    rng = np.random.default_rng(27)
+    m, n, k = 66000, 33000, 32
+    A, av = _exact_operand(pkg, rng, "e2m1", m, k)
+    B, bv = _exact_operand(pkg, rng, "e2m1", n, k)
+    C = pkg.mx_matmul(A, B)
+    for r, c in ((slice(0, 50), slice(0, 50)), (slice(m - 50, m), slice(n - 50, n)), (slice(m - 50, m), slice(0, 50)),
+                 (slice(m // 2, m // 2 + 50), slice(n // 2, n // 2 + 50))):
+        want = torch.from_numpy(av[r] @ bv[c].T).float().bfloat16()
+        assert torch.equal(C[r, c].cpu(), want)
+    B1 = pkg.MXMatrix.from_codes(B.codes()[None], B.scales()[None], "e2m1")
+    D = pkg.mx_grouped_matmul(A, B1, torch.tensor([m - 5], dtype=torch.int32, device="cuda"))
+    assert torch.equal(D[:m - 5], C[:m - 5]) and (D[m - 5:] == 0).all()
+    del C, D
+    torch.cuda.empty_cache()
+
+
+@pytest.mark.gpu
+def test_product_nan_codes(pkg):
+    """The NaN code of e4m3 makes its row or column NaN, and no other."""
+    import torch
+    rng = np.random.default_rng(28)
+    A, av = _exact_operand(pkg, rng, "e4m3", 40, 96)
+    B, bv = _exact_operand(pkg, rng, "e2m1", 50, 96)
+    c = A.codes()
+    c[7, 33] = 0x7f
+    c[9, 95] = 0xff
+    C = _f64(pkg.mx_matmul(pkg.MXMatrix.from_codes(c, A.scales(), "e4m3"), B, dtype=torch.float32))
+    want = av @ bv.T
+    want[[7, 9]] = np.nan
+    np.testing.assert_array_equal(C, want)
 
 
 @pytest.mark.gpu
