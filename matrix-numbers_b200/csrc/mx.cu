@@ -98,6 +98,40 @@ __device__ __forceinline__ uint4 load8_raw(const T* __restrict__ p, int count) {
     return w;
 }
 
+// A thread's eight rows (r0 + 16 i) of a tile of 16-bit values, eight values each from column col0 + 8 lane16 of rows that
+// have J; `first` is column 0 of the tile's first row, of `rows`; zeros outside
+template <typename T, bool ALIGNED>
+__device__ __forceinline__ void load_rows_raw(const T* __restrict__ first, long long row_stride, int rows, int col0, int J,
+                                              int r0, int lane16, uint4 (&raw)[8]) {
+    const int col = col0 + lane16 * 8;
+    if constexpr (ALIGNED) {
+#pragma unroll
+        for (int i = 0; i < 8; i++)
+            raw[i] = load8_raw(first + (long long)(r0 + 16 * i) * row_stride + col, r0 + 16 * i < rows ? J - col : 0);
+    } else {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+            uint4 tail[4];                                      // the granule behind a row's last lane
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int r = r0 + 16 * (h + i);
+                const uintptr_t begin = reinterpret_cast<uintptr_t>(first + (long long)r * row_stride);
+                const uintptr_t end = r < rows ? begin + 2 * (uintptr_t)J : begin;
+                const uintptr_t at = (begin & ~(uintptr_t)15) + 2 * (uintptr_t)col;
+                raw[h + i] = load_granule(at, begin, end);
+                tail[i] = make_uint4(0u, 0u, 0u, 0u);
+                if (lane16 == 15) tail[i] = load_granule(at + 16, begin, end);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(first + (long long)(r0 + 16 * (h + i)) * row_stride) & 15);
+                const uint4 n = next_lane(raw[h + i]);
+                raw[h + i] = shift_granules(raw[h + i], lane16 == 15 ? tail[i] : n, sh);
+            }
+        }
+    }
+}
+
 template <typename T, int FMT>
 __device__ __forceinline__ void emit_raw(uint4 raw, bool up, int r, int here, int lane16, uint8_t* __restrict__ ct,
                                          long long pitch, uint8_t* sc) {
@@ -118,7 +152,7 @@ __device__ __forceinline__ void emit_raw(uint4 raw, bool up, int r, int here, in
 // The row operand, rows contiguous.  One CTA per scale tile; all of a thread's eight loads are issued before the first is
 // used, and the tile's 512 scale bytes leave as one contiguous store.  ALIGNED: rows start on 16-byte boundaries.
 template <typename T, int FMT, bool ALIGNED>
-__global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const __grid_constant__ QuantJob q, bool up) {
+__global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && ALIGNED ? 4 : 3) quantize_rows_kernel(const __grid_constant__ QuantJob q, bool up) {
     __shared__ __align__(16) uint8_t sc[TILE_BYTES];
     const int ktiles = padded_k(q.J) / TILE, rtiles = row_tiles(q.I);
     const int kt = (int)(blockIdx.x % (unsigned)ktiles);
@@ -132,11 +166,10 @@ __global__ void __launch_bounds__(THREADS) quantize_rows_kernel(const __grid_con
 
     const long long pitch = code_pitch(FMT, q.J);
     uint8_t* ct = q.row_codes + ((long long)g * q.I + (long long)rt * TILE) * pitch + kt * (FMT == OZK_MX_E2M1 ? 64 : 128);
-    if constexpr (ALIGNED && sizeof(T) == 2) {
+    if constexpr (sizeof(T) == 2) {
         // the words as they are until they are encoded: half the registers, and magnitudes ordered like their bits
         uint4 raw[8];
-#pragma unroll
-        for (int i = 0; i < 8; i++) raw[i] = load8_raw(xt + (long long)(r0 + 16 * i) * q.si, r0 + 16 * i < here ? count : 0);
+        load_rows_raw<T, ALIGNED>(xt - col, q.si, here, kt * TILE, q.J, r0, lane16, raw);
 #pragma unroll
         for (int i = 0; i < 8; i++) emit_raw<T, FMT>(raw[i], up, r0 + 16 * i, here, lane16, ct, pitch, sc);
     } else {
@@ -173,13 +206,12 @@ __device__ __forceinline__ int encode_block(uint32_t m, bool up, uint4 (&c)[2], 
     return s;
 }
 
-// The column operand, or (FP32) both operands, of one or two jobs in one launch.  A thread owns a block of 32
-// values down a column (FP32) or a pair of columns (16-bit types, one 32-bit word a row), which it reads straight into
-// registers: a warp reads 128 contiguous bytes a row, nothing is transposed in memory, and a block's largest magnitude
-// needs no exchange.  Only the codes go through shared memory, to leave as whole segments of the operand's vectors.
-// The row operand of FP32 values reads the tile again.  WORDS: the pairs are aligned 32-bit words (else element by element,
-// any strides, and no row operand).
-template <typename T, int FMT, bool WORDS>
+// The column operand, or (FP32, rows aligned) both operands, of one or two jobs in one launch; any strides.  A thread owns
+// a block of 32 values down a column (FP32) or a pair of columns (16-bit types), which it reads straight into registers: a
+// warp reads a row's neighbouring values, nothing is transposed in memory, and a block's largest magnitude needs no
+// exchange.  Only the codes go through shared memory, to leave as whole segments of the operand's vectors.  The row operand
+// reads the tile again.  FP32 5001 x 4095 down the columns to e2m1: 18 us, 5.1 TB/s.
+template <typename T, int FMT>
 __global__ void __launch_bounds__(THREADS)
     quantize_dual_kernel(const __grid_constant__ QuantJob q0, const __grid_constant__ QuantJob q1, unsigned tiles0, bool up) {
     constexpr int SEG = FMT == OZK_MX_E2M1 ? TILE / 2 : TILE;   // code bytes of a vector of the tile
@@ -223,12 +255,8 @@ __global__ void __launch_bounds__(THREADS)
             for (int j = 0; j < BLOCK; j++) {
                 v[j] = 0u;
                 if (b * BLOCK + j < rows) {
-                    if (WORDS && c + 1 < cols) {
-                        v[j] = __ldg(reinterpret_cast<const uint32_t*>(p + j * q.si));
-                    } else if (c < cols) {
-                        v[j] = __ldg(reinterpret_cast<const unsigned short*>(p + j * q.si));
-                        if (c + 1 < cols) v[j] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p + j * q.si + q.sj)) << 16;
-                    }
+                    if (c < cols) v[j] = __ldg(reinterpret_cast<const unsigned short*>(p + j * q.si));
+                    if (c + 1 < cols) v[j] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short*>(p + j * q.si + q.sj)) << 16;
                 }
             }
             uint32_t m = 0;                                      // magnitudes of 16-bit types are ordered like their bits
@@ -248,7 +276,7 @@ __global__ void __launch_bounds__(THREADS)
             if (FMT != OZK_MX_E2M1) d[1] = o[1];
         }
     }
-    if (sizeof(T) == 4 && WORDS && q.row_codes) {
+    if (sizeof(T) == 4 && q.row_codes) {
         const int lane16 = threadIdx.x & 15, r0 = threadIdx.x >> 4;
         const long long pitch = code_pitch(FMT, q.J);
         uint8_t* ct = q.row_codes + ((long long)g * q.I + (long long)it * TILE) * pitch + (long long)jt * SEG;
@@ -279,16 +307,16 @@ __global__ void __launch_bounds__(THREADS)
         }
         copy_scale_tile(q.col_scales + (((long long)g * jtiles + jt) * itiles + it) * TILE_BYTES, sc[0]);
     }
-    if (sizeof(T) == 4 && WORDS && q.row_codes)
+    if (sizeof(T) == 4 && q.row_codes)
         copy_scale_tile(q.row_scales + (((long long)g * itiles + it) * jtiles + jt) * TILE_BYTES, sc[1]);
 }
 
-// Column operands, both operands, or several jobs, of 16-bit matrices with aligned rows, from one read: 16 lanes load a row's 128 values, the
+// Column operands, both operands, or several jobs, of 16-bit matrices with contiguous rows, from one read: 16 lanes load a row's 128 values, the
 // row operand is encoded from those registers, and the tile goes to shared memory (rows 16 bytes apart from a multiple of
 // 128: neither its rows nor its columns meet in a bank), from which the column operand is encoded as above.  bf16
 // 16384 x 8192 to e4m3: 102 us, 5.3 TB/s (134 us when the tile was read from global memory twice).
-template <typename T, int FMT>
-__global__ void __launch_bounds__(THREADS, 4)
+template <typename T, int FMT, bool ALIGNED>
+__global__ void __launch_bounds__(THREADS, ALIGNED ? 4 : 3)
     quantize_shared_kernel(const __grid_constant__ QuantJob q0, const __grid_constant__ QuantJob q1, unsigned tiles0, bool up) {
     constexpr int SEG = FMT == OZK_MX_E2M1 ? TILE / 2 : TILE, CP = SEG + 16, PITCH = TILE * 2 + 16;
     __shared__ __align__(16) uint8_t tile_mem[TILE * PITCH];
@@ -307,8 +335,7 @@ __global__ void __launch_bounds__(THREADS, 4)
     const T* const type = nullptr;
 
     uint4 raw[8];
-#pragma unroll
-    for (int i = 0; i < 8; i++) raw[i] = load8_raw(xt + (long long)(r0 + 16 * i) * q.si + lane16 * 8, r0 + 16 * i < rows ? cols - lane16 * 8 : 0);
+    load_rows_raw<T, ALIGNED>(xt - jt * TILE, q.si, rows, jt * TILE, q.J, r0, lane16, raw);
     if (q.col_codes) {
 #pragma unroll
         for (int i = 0; i < 8; i++) *reinterpret_cast<uint4*>(tile_mem + (r0 + 16 * i) * PITCH + lane16 * 16) = raw[i];
@@ -681,20 +708,10 @@ int launch_rows(const QuantJob& q, bool aligned, bool up, cudaStream_t st) {
 }
 
 template <typename T, int FMT>
-int launch_dual(const QuantJob& a, const QuantJob& b, bool words, bool up, cudaStream_t st) {
+int launch_dual(const QuantJob& a, const QuantJob& b, bool up, cudaStream_t st) {
     const unsigned t0 = (unsigned)tile_count(a.groups, a.I, a.J);
     const unsigned t1 = b.x ? (unsigned)tile_count(b.groups, b.I, b.J) : 0u;
-    if (words) quantize_dual_kernel<T, FMT, true><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
-    else quantize_dual_kernel<T, FMT, false><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
-    OZK_CHECK_LAUNCH();
-    return OZK_OK;
-}
-
-template <typename T, int FMT>
-int launch_shared(const QuantJob& a, const QuantJob& b, bool up, cudaStream_t st) {
-    const unsigned t0 = (unsigned)tile_count(a.groups, a.I, a.J);
-    const unsigned t1 = b.x ? (unsigned)tile_count(b.groups, b.I, b.J) : 0u;
-    quantize_shared_kernel<T, FMT><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
+    quantize_dual_kernel<T, FMT><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
     OZK_CHECK_LAUNCH();
     return OZK_OK;
 }
@@ -703,6 +720,18 @@ int launch_shared(const QuantJob& a, const QuantJob& b, bool up, cudaStream_t st
 bool rows_aligned(const QuantJob& q, long long size, uintptr_t unit) {
     return q.sj == 1 && reinterpret_cast<uintptr_t>(q.x) % unit == 0 && (q.I == 1 || q.si * size % (long long)unit == 0) &&
            (q.groups == 1 || q.gs * size % (long long)unit == 0);
+}
+
+template <typename T, int FMT>
+int launch_shared(const QuantJob& a, const QuantJob& b, bool up, cudaStream_t st) {
+    const unsigned t0 = (unsigned)tile_count(a.groups, a.I, a.J);
+    const unsigned t1 = b.x ? (unsigned)tile_count(b.groups, b.I, b.J) : 0u;
+    if (rows_aligned(a, 2, 16) && (!b.x || rows_aligned(b, 2, 16)))
+        quantize_shared_kernel<T, FMT, true><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
+    else
+        quantize_shared_kernel<T, FMT, false><<<t0 + t1, THREADS, 0, st>>>(a, b, t0, up);
+    OZK_CHECK_LAUNCH();
+    return OZK_OK;
 }
 
 QuantJob swapped(const QuantJob& q) {
@@ -725,8 +754,8 @@ int quantize_one(QuantJob q, bool up, cudaStream_t st) {
     }
     const QuantJob t = swapped(q);
     if constexpr (sizeof(T) == 2)
-        if (rows_aligned(t, size, 16)) return launch_shared<T, FMT>(t, QuantJob{}, up, st);
-    return launch_dual<T, FMT>(t, QuantJob{}, sizeof(T) == 4 || rows_aligned(t, size, 4), up, st);
+        if (t.sj == 1) return launch_shared<T, FMT>(t, QuantJob{}, up, st);
+    return launch_dual<T, FMT>(t, QuantJob{}, up, st);
 }
 
 // Jobs of one type: in one launch where a row operand has to be written beside a column operand or there are two jobs,
@@ -736,7 +765,8 @@ int quantize_jobs(const QuantJob* jobs, int count, bool up, cudaStream_t st) {
     bool joint = true;
     for (int i = 0; i < count; i++) {
         const bool both = jobs[i].row_codes && jobs[i].col_codes;
-        if (!rows_aligned(jobs[i], (long long)sizeof(T), 16)) joint = false;
+        // (FP32 rows that are not aligned are read by the rows kernel, whose loads are vectors all the same)
+        if (sizeof(T) == 2 ? jobs[i].sj != 1 : !rows_aligned(jobs[i], 4, 16)) joint = false;
         if (count == 1 && !both) joint = false;
     }
     long long tiles = 0;
@@ -744,7 +774,7 @@ int quantize_jobs(const QuantJob* jobs, int count, bool up, cudaStream_t st) {
     if (joint && tiles <= 0x7fffffffLL) {
         const QuantJob second = count > 1 ? jobs[1] : QuantJob{};
         if constexpr (sizeof(T) == 2) return launch_shared<T, FMT>(jobs[0], second, up, st);
-        else return launch_dual<T, FMT>(jobs[0], second, true, up, st);
+        else return launch_dual<T, FMT>(jobs[0], second, up, st);
     }
     for (int i = 0; i < count; i++) {
         int rc = OZK_OK;

@@ -164,6 +164,43 @@ __device__ __forceinline__ void store8(T* __restrict__ p, bool whole, int count,
     }
 }
 
+// ---- rows that start anywhere ----
+// The lanes of a row read the aligned 16 bytes ("granules") that cover it, each its own, get the next one from their
+// neighbour and shift the two into place; bytes outside [begin, end) are never read and count as zero.
+__device__ __forceinline__ uint4 load_granule(uintptr_t at, uintptr_t begin, uintptr_t end) {
+    if (at >= begin && at + 16 <= end) return __ldg(reinterpret_cast<const uint4*>(at));
+    if (at >= end) return make_uint4(0u, 0u, 0u, 0u);
+    uint16_t e[8];
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const uintptr_t p = at + 2 * j;
+        e[j] = p >= begin && p < end ? __ldg(reinterpret_cast<const unsigned short*>(p)) : (uint16_t)0;
+    }
+    return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
+                      e[6] | (uint32_t)e[7] << 16);
+}
+__device__ __forceinline__ uint4 next_lane(uint4 g) {
+    return make_uint4(__shfl_down_sync(0xffffffffu, g.x, 1), __shfl_down_sync(0xffffffffu, g.y, 1),
+                      __shfl_down_sync(0xffffffffu, g.z, 1), __shfl_down_sync(0xffffffffu, g.w, 1));
+}
+// the 16 bytes from byte `sh` (0, 2 .. 14) of the 32 that g and n hold
+__device__ __forceinline__ uint4 shift_granules(uint4 g, uint4 n, uint32_t sh) {
+    uint32_t w[8] = {g.x, g.y, g.z, g.w, n.x, n.y, n.z, n.w};
+    if (sh & 8u) {
+#pragma unroll
+        for (int j = 0; j < 6; j++) w[j] = w[j + 2];
+    }
+    if (sh & 4u) {
+#pragma unroll
+        for (int j = 0; j < 5; j++) w[j] = w[j + 1];
+    }
+    if (sh & 2u) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // the larger magnitude, NaN if either is
 __device__ __forceinline__ float max_magnitude(float a, float b) {
     float m;
