@@ -19,7 +19,7 @@ struct QuantJob {
     long long gs, si, sj;
     int groups, I, J;
     uint8_t *row_codes, *row_scales, *col_codes, *col_scales;
-    const void *begin, *end;                 // the bytes that the matrix occupies (rows kernel)
+    uintptr_t begin, end;                    // the bytes between its first and last element
 };
 
 __device__ __forceinline__ void copy_scale_tile(uint8_t* __restrict__ to, const uint8_t* sc) {
@@ -30,12 +30,12 @@ __device__ __forceinline__ void copy_scale_tile(uint8_t* __restrict__ to, const 
 // Eight consecutive values of which 16 bytes need not be aligned: the aligned vectors around them, shifted into place,
 // where those lie within [begin, end); one by one otherwise.
 template <typename T>
-__device__ __forceinline__ void load8_any(const T* __restrict__ p, int count, const void* begin, const void* end,
+__device__ __forceinline__ void load8_any(const T* __restrict__ p, int count, uintptr_t begin, uintptr_t end,
                                           float (&v)[8]) {
     constexpr int NV = sizeof(T) == 4 ? 3 : 2, NW = 4 * NV;
     const uintptr_t at = reinterpret_cast<uintptr_t>(p), a0 = at & ~(uintptr_t)15;
     const uint32_t sh = (uint32_t)(at & 15);
-    if (count < 8 || a0 < reinterpret_cast<uintptr_t>(begin) || a0 + 16 * NV > reinterpret_cast<uintptr_t>(end)) {
+    if (count < 8 || a0 < begin || a0 + 16 * NV > end) {
         load8(p, false, count, v);
         return;
     }
@@ -101,8 +101,10 @@ __device__ __forceinline__ uint4 load8_raw(const T* __restrict__ p, int count) {
 // A thread's eight rows (r0 + 16 i) of a tile of 16-bit values, eight values each from column col0 + 8 lane16 of rows that
 // have J; `first` is column 0 of the tile's first row, of `rows`; zeros outside
 template <typename T, bool ALIGNED>
-__device__ __forceinline__ void load_rows_raw(const T* __restrict__ first, long long row_stride, int rows, int col0, int J,
-                                              int r0, int lane16, uint4 (&raw)[8]) {
+__device__ __forceinline__ void load_rows_raw(const QuantJob& q, const T* __restrict__ first, int rows, int col0, int r0,
+                                              int lane16, uint4 (&raw)[8]) {
+    const long long row_stride = q.si;
+    const int J = q.J;
     const int col = col0 + lane16 * 8;
     if constexpr (ALIGNED) {
 #pragma unroll
@@ -115,18 +117,18 @@ __device__ __forceinline__ void load_rows_raw(const T* __restrict__ first, long 
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const int r = r0 + 16 * (h + i);
-                const uintptr_t begin = reinterpret_cast<uintptr_t>(first + (long long)r * row_stride);
-                const uintptr_t end = r < rows ? begin + 2 * (uintptr_t)J : begin;
-                const uintptr_t at = (begin & ~(uintptr_t)15) + 2 * (uintptr_t)col;
-                raw[h + i] = load_granule(at, begin, end);
+                const uintptr_t row = reinterpret_cast<uintptr_t>(first + (long long)r * row_stride);
+                const uintptr_t end = r < rows ? row + 2 * (uintptr_t)J : 0;
+                const uintptr_t at = (row & ~(uintptr_t)15) + 2 * (uintptr_t)col;
+                raw[h + i] = load_granule(at, end, q.begin, q.end);
                 tail[i] = make_uint4(0u, 0u, 0u, 0u);
-                if (lane16 == 15) tail[i] = load_granule(at + 16, begin, end);
+                if (lane16 == 15) tail[i] = load_granule(at + 16, end, q.begin, q.end);
             }
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(first + (long long)(r0 + 16 * (h + i)) * row_stride) & 15);
                 const uint4 n = next_lane(raw[h + i]);
-                raw[h + i] = shift_granules(raw[h + i], lane16 == 15 ? tail[i] : n, sh);
+                raw[h + i] = keep8(shift_granules(raw[h + i], lane16 == 15 ? tail[i] : n, sh), J - col);
             }
         }
     }
@@ -169,7 +171,7 @@ __global__ void __launch_bounds__(THREADS, sizeof(T) == 2 && ALIGNED ? 4 : 3) qu
     if constexpr (sizeof(T) == 2) {
         // the words as they are until they are encoded: half the registers, and magnitudes ordered like their bits
         uint4 raw[8];
-        load_rows_raw<T, ALIGNED>(xt - col, q.si, here, kt * TILE, q.J, r0, lane16, raw);
+        load_rows_raw<T, ALIGNED>(q, xt - col, here, kt * TILE, r0, lane16, raw);
 #pragma unroll
         for (int i = 0; i < 8; i++) emit_raw<T, FMT>(raw[i], up, r0 + 16 * i, here, lane16, ct, pitch, sc);
     } else {
@@ -335,7 +337,7 @@ __global__ void __launch_bounds__(THREADS, ALIGNED ? 4 : 3)
     const T* const type = nullptr;
 
     uint4 raw[8];
-    load_rows_raw<T, ALIGNED>(xt - jt * TILE, q.si, rows, jt * TILE, q.J, r0, lane16, raw);
+    load_rows_raw<T, ALIGNED>(q, xt - jt * TILE, rows, jt * TILE, r0, lane16, raw);
     if (q.col_codes) {
 #pragma unroll
         for (int i = 0; i < 8; i++) *reinterpret_cast<uint4*>(tile_mem + (r0 + 16 * i) * PITCH + lane16 * 16) = raw[i];
@@ -504,60 +506,132 @@ __device__ __forceinline__ void emit_chunk(float (&o)[8], bool up, int c, bool i
     if (in && (c & 15) == 0) *reinterpret_cast<uint32_t*>(tr + (long long)(c / 16) * TILE_BYTES) = four;
 }
 
-// Eight values as they lie in memory
-template <typename T>
+// Eight values of a row as they lie in memory.  Rows that do not start on 16 bytes: the aligned granules from the one that
+// holds the first value, and in a warp's last lane the one behind; `get` shifts them into place (called by whole warps).
+template <typename T, bool ALIGNED>
 struct Raw8 {
-    uint4 w[sizeof(T) / 2];
-    __device__ __forceinline__ void load(const T* p) {
+    static constexpr int NG = sizeof(T) / 2;
+    uint4 w[NG], tail;
+    __device__ __forceinline__ void clear() {
 #pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
+        for (int i = 0; i < NG; i++) w[i] = make_uint4(0u, 0u, 0u, 0u);
+        tail = make_uint4(0u, 0u, 0u, 0u);
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
-        if constexpr (sizeof(T) == 4) {
+    // values 8 c .. 8 c + 7 of a row of d; zeros behind its end
+    __device__ __forceinline__ void load(const T* row, int c, int d, uintptr_t begin, uintptr_t end) {
+        if constexpr (ALIGNED) {
+            if (c < d / 8) {
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                v[4 * i] = __uint_as_float(w[i].x); v[4 * i + 1] = __uint_as_float(w[i].y);
-                v[4 * i + 2] = __uint_as_float(w[i].z); v[4 * i + 3] = __uint_as_float(w[i].w);
+                for (int i = 0; i < NG; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(row + c * 8) + i);
             }
         } else {
-            const uint32_t u[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
+            const uintptr_t at0 = reinterpret_cast<uintptr_t>(row), row_end = at0 + (uintptr_t)d * sizeof(T);
+            const uintptr_t at = (at0 & ~(uintptr_t)15) + (uintptr_t)c * (8 * sizeof(T));
+#pragma unroll
+            for (int i = 0; i < NG; i++) w[i] = load_granule(at + 16 * i, row_end, begin, end);
+            if ((threadIdx.x & 31) == 31) tail = load_granule(at + 16 * NG, row_end, begin, end);
+        }
+    }
+    __device__ __forceinline__ void get(const T* row, int c, int d, float (&v)[8]) const {
+        uint4 u[NG];
+#pragma unroll
+        for (int i = 0; i < NG; i++) u[i] = w[i];
+        if constexpr (!ALIGNED) {
+            const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15);
+            uint4 n = next_lane(w[0]);
+            if ((threadIdx.x & 31) == 31) n = tail;
+#pragma unroll
+            for (int i = 0; i < NG; i++) u[i] = shift_granules(w[i], i + 1 < NG ? w[i + 1] : n, sh);
+        }
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < NG; i++) {
+                v[4 * i] = __uint_as_float(u[i].x); v[4 * i + 1] = __uint_as_float(u[i].y);
+                v[4 * i + 2] = __uint_as_float(u[i].z); v[4 * i + 3] = __uint_as_float(u[i].w);
+            }
+        } else {
+            const uint32_t e[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
-                const float2 f = unpack2(u[j], (const T*)nullptr);
+                const float2 f = unpack2(e[j], (const T*)nullptr);
                 v[2 * j] = f.x;
                 v[2 * j + 1] = f.y;
             }
         }
+        if (!ALIGNED && c * 8 + 8 > d) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (c * 8 + j >= d) v[j] = 0.0f;
+        }
     }
 };
 
-// Many aligned rows that fit into the registers of TPR threads (d a multiple of 8, at most 8 TPR NC): CTAs stay and take
-// rows in turn, with the next row's loads under way while a row is summed and encoded, and the weights in registers.
-template <typename T, typename W, int FMT, int TPR, int NC, bool RES>
-__global__ void __launch_bounds__(TPR, 1024 / TPR)
+// Values 8 c .. 8 c + 7 of a row of d to memory that need not be aligned (called by whole warps): each lane stores the
+// granule that ends its neighbour's values and begins its own; a warp's two ends, a row's end and FP32 go one by one.
+template <typename T>
+__device__ __forceinline__ void store8_any(T* row, int c, int d, const float (&v)[8]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (c * 8 + j < d) row[c * 8 + j] = v[j];
+    } else {
+        const T* const type = nullptr;
+        const int lane = threadIdx.x & 31, lead = (int)(reinterpret_cast<uintptr_t>(row) & 15) / 2;   // values of the granule
+        const uint4 own = make_uint4(pack2(v[0], v[1], type), pack2(v[2], v[3], type), pack2(v[4], v[5], type),   // before the row
+                                     pack2(v[6], v[7], type));
+        const uint4 before = make_uint4(__shfl_up_sync(0xffffffffu, own.x, 1), __shfl_up_sync(0xffffffffu, own.y, 1),
+                                        __shfl_up_sync(0xffffffffu, own.z, 1), __shfl_up_sync(0xffffffffu, own.w, 1));
+        const uint4 g = lead ? shift_granules(before, own, (uint32_t)(16 - 2 * lead)) : own;
+        const int first = c * 8 - lead;                         // the row's value at the granule's start
+        if ((lane > 0 || lead == 0) && first >= 0 && first + 8 <= d) {
+            *reinterpret_cast<uint4*>(row + first) = g;
+        } else {
+            // the granule's values that are this lane's own (lane 0) or anyone's, and inside the row
+            const uint32_t e[4] = {g.x, g.y, g.z, g.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int k = first + j;
+                if (k >= 0 && k < d && (lane > 0 || j >= lead))
+                    reinterpret_cast<uint16_t*>(row)[k] = (uint16_t)(e[j / 2] >> (16 * (j & 1)));
+            }
+        }
+        if (lane == 31) {                                       // its last values are in the next warp's first granule
+            const uint32_t e[4] = {own.x, own.y, own.z, own.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (j >= 8 - lead && c * 8 + j < d)
+                    reinterpret_cast<uint16_t*>(row)[c * 8 + j] = (uint16_t)(e[j / 2] >> (16 * (j & 1)));
+        }
+    }
+}
+
+// Many rows that fit into the registers of TPR threads (d at most 8 TPR NC): CTAs stay and take rows in turn, with the
+// next row's loads under way while a row is summed and encoded, and the weights in registers.  bf16 16384 x 8192 with the
+// residual to e4m3: 168 us, 5.6 TB/s (264 us with a CTA a row).
+template <typename T, typename W, int FMT, int TPR, int NC, bool RES, bool ALIGNED>
+__global__ void __launch_bounds__(TPR, ALIGNED || TPR == 1024 ? 1024 / TPR : 768 / TPR)
     rms_norm_stream_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ residual, long long res_stride,
-                           const W* __restrict__ weight, int rows, int d, double inv_d, float eps, bool up,
+                           const W* __restrict__ weight, int rows, int d, double inv_d, float eps, bool weight_aligned, bool up,
                            T* __restrict__ sum, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     __shared__ double part[2][32];
-    const int t = threadIdx.x, full = d / 8, chunks = padded_k(d) / 8;
-    Raw8<T> rx[NC], rr[RES ? NC : 1];
-    Raw8<W> rw[NC];
+    const int t = threadIdx.x, chunks = padded_k(d) / 8;
+    Raw8<T, ALIGNED> rx[NC], rr[RES ? NC : 1];
+    float w[NC][8];
+    const uintptr_t x_begin = reinterpret_cast<uintptr_t>(x), x_end = reinterpret_cast<uintptr_t>(x + (rows - 1) * x_stride + d);
+    const uintptr_t r_begin = reinterpret_cast<uintptr_t>(residual), r_end = reinterpret_cast<uintptr_t>(residual + (rows - 1) * res_stride + d);
     auto fetch = [&](int row) {
 #pragma unroll
         for (int i = 0; i < NC; i++) {
-            const int c = t + i * TPR;
-            if (c < full) {
-                rx[i].load(x + row * x_stride + c * 8);
-                if (RES) rr[i].load(residual + row * res_stride + c * 8);
-            }
+            rx[i].load(x + row * x_stride, t + i * TPR, d, x_begin, x_end);
+            if (RES) rr[i].load(residual + row * res_stride, t + i * TPR, d, r_begin, r_end);
         }
     };
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-        rx[i] = {};
-        if (RES) rr[i] = {};
-        rw[i] = {};
-        if (t + i * TPR < full) rw[i].load(weight + (t + i * TPR) * 8);
+        rx[i].clear();
+        if (RES) rr[i].clear();
+        const int col = (t + i * TPR) * 8;
+        load8(weight + col, weight_aligned && col + 8 <= d, max(0, d - col), w[i]);
     }
     fetch(blockIdx.x);
     const long long pitch = code_pitch(FMT, d);
@@ -567,10 +641,10 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR)
         float sq = 0.0f;
 #pragma unroll
         for (int i = 0; i < NC; i++) {
-            rx[i].get(v[i]);
+            rx[i].get(x + row * x_stride, t + i * TPR, d, v[i]);
             if (RES) {
                 float q[8];
-                rr[i].get(q);
+                rr[i].get(residual + row * res_stride, t + i * TPR, d, q);
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[i][j] += q[j];
             }
@@ -580,8 +654,11 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR)
         if (row + (int)gridDim.x < rows) fetch(row + (int)gridDim.x);
         if (sum) {
 #pragma unroll
-            for (int i = 0; i < NC; i++)
-                if (t + i * TPR < full) store8(sum + row * (long long)d + (t + i * TPR) * 8, true, 8, v[i]);
+            for (int i = 0; i < NC; i++) {
+                T* to = sum + row * (long long)d;
+                if (!ALIGNED) store8_any(to, t + i * TPR, d, v[i]);
+                else if (t + i * TPR < d / 8) store8(to + (t + i * TPR) * 8, true, 8, v[i]);
+            }
         }
         double total = row_sum<TPR>(sq, part[turn]);
         if (!(total < 3.0e38)) {                                // squares beyond FP32: once more, scaled
@@ -601,10 +678,8 @@ __global__ void __launch_bounds__(TPR, 1024 / TPR)
         uint8_t* tr = scales + (row / TILE) * (long long)(chunks / 16) * TILE_BYTES + scale_slot(row % TILE, 0);
 #pragma unroll
         for (int i = 0; i < NC; i++) {
-            float w[8];
-            rw[i].get(w);
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * w[j] * rstd;
+            for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * w[i][j] * rstd;
             emit_chunk<FMT>(v[i], up, t + i * TPR, t + i * TPR < chunks, cr, tr);
         }
     }
@@ -748,8 +823,6 @@ int quantize_one(QuantJob q, bool up, cudaStream_t st) {
     const long long size = (long long)sizeof(T);
     q.col_codes = q.col_scales = nullptr;
     if (q.sj == 1) {
-        q.begin = q.x;
-        q.end = static_cast<const T*>(q.x) + (q.groups - 1) * q.gs + (q.I - 1) * q.si + q.J;
         return launch_rows<T, FMT>(q, rows_aligned(q, size, 16), up, st);
     }
     const QuantJob t = swapped(q);
@@ -785,7 +858,13 @@ int quantize_jobs(const QuantJob* jobs, int count, bool up, cudaStream_t st) {
     return OZK_OK;
 }
 
-int quantize(const QuantJob* jobs, int count, int dtype, int fmt, bool up, cudaStream_t st) {
+int quantize(QuantJob* jobs, int count, int dtype, int fmt, bool up, cudaStream_t st) {
+    for (int i = 0; i < count; i++) {
+        QuantJob& q = jobs[i];
+        const long long last = (q.groups - 1) * q.gs + (q.I - 1) * q.si + (q.J - 1) * q.sj;
+        q.begin = reinterpret_cast<uintptr_t>(q.x);
+        q.end = q.begin + (uintptr_t)(last + 1) * (dtype == OZK_F32 ? 4 : 2);
+    }
     switch (dtype) {
         case OZK_F32:
             return fmt == OZK_MX_E2M1 ? quantize_jobs<float, OZK_MX_E2M1>(jobs, count, up, st)
@@ -852,15 +931,21 @@ int launch_norm(const NormArgs& a) {
             static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps, aligned, a.up, static_cast<T*>(a.sum), a.codes, a.scales)
 #define OZK_STREAM(TPR, NC)                                                                                          \
     {                                                                                                                \
-        const int grid = a.rows < a.sms * (1024 / TPR) ? a.rows : a.sms * (1024 / TPR);                              \
-        auto kern = a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true> : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false>; \
-        kern<<<(unsigned)grid, TPR, 0, a.st>>>(static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), \
-                                               a.res_stride, static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps,  \
-                                               a.up, static_cast<T*>(a.sum), a.codes, a.scales);                     \
+        auto kern = aligned8 ? (a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true, true>                  \
+                                           : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false, true>)                \
+                             : (a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true, false>                 \
+                                           : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false, false>);              \
+        const int grid = a.sms * (aligned8 || TPR == 1024 ? 1024 / TPR : 768 / TPR);                                 \
+        kern<<<(unsigned)(a.rows < grid ? a.rows : grid), TPR, 0, a.st>>>(                                           \
+            static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), a.res_stride,                 \
+            static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps, aligned16(a.weight), a.up,                   \
+            static_cast<T*>(a.sum), a.codes, a.scales);                                                              \
     }
     // rows enough for every CTA to take several: the streaming kernel
-    if (aligned && d % 8 == 0 && d > 1024 && d <= 16384 && a.rows >= 4 * a.sms) {
-        if (d <= 2048) OZK_STREAM(256, 1)
+    const bool aligned8 = aligned && d % 8 == 0;
+    if (d > 256 && d <= 16384 && a.rows >= 4 * a.sms) {
+        if (d <= 1024) OZK_STREAM(128, 1)
+        else if (d <= 2048) OZK_STREAM(256, 1)
         else if (d <= 4096) OZK_STREAM(256, 2)
         else if (d <= 8192) OZK_STREAM(512, 2)
         else OZK_STREAM(1024, 2)
@@ -954,7 +1039,7 @@ extern "C" int ozk_mx_quantize_both(const void* x, int dtype, int rows, int cols
                                     ozk_stream_t stream) {
     if (!matrix_ok(x, dtype, rows, cols, row_stride, col_stride) || !fmt_ok(fmt)) return OZK_ERR_ARG;
     if (!operand_ok(along_rows) || !operand_ok(along_cols)) return OZK_ERR_ARG;
-    const QuantJob q = job_of(x, rows, cols, row_stride, col_stride, fmt, along_rows, along_cols);
+    QuantJob q = job_of(x, rows, cols, row_stride, col_stride, fmt, along_rows, along_cols);
     return quantize(&q, 1, dtype, fmt, round_up != 0, reinterpret_cast<cudaStream_t>(stream));
 }
 
@@ -966,7 +1051,7 @@ extern "C" int ozk_mx_linear_forward(const void* x, int x_dtype, int64_t x_row_s
         return OZK_ERR_ARG;
     if (!fmt_ok(fmt) || !operand_ok(x_along_k) || !operand_ok(w_along_k) || !y || !err) return OZK_ERR_ARG;
     if ((x_along_m && !operand_ok(x_along_m)) || (w_along_n && !operand_ok(w_along_n))) return OZK_ERR_ARG;
-    const QuantJob q[2] = {job_of(x, m, k, x_row_stride, x_col_stride, fmt, x_along_k, x_along_m),
+    QuantJob q[2] = {job_of(x, m, k, x_row_stride, x_col_stride, fmt, x_along_k, x_along_m),
                            job_of(w, n, k, w_row_stride, w_col_stride, fmt, w_along_k, w_along_n)};
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     int rc;
@@ -988,7 +1073,7 @@ extern "C" int ozk_mx_linear_backward(const void* dy, int dy_dtype, int64_t dy_r
     if (!dx && !dw) return OZK_ERR_ARG;
     if (dx && (!operand_ok(w_along_n) || !operand_ok(dy_along_n))) return OZK_ERR_ARG;
     if (dw && (!operand_ok(x_along_m) || !operand_ok(dy_along_m))) return OZK_ERR_ARG;
-    const QuantJob q = job_of(dy, m, n, dy_row_stride, dy_col_stride, fmt, dx ? dy_along_n : nullptr, dw ? dy_along_m : nullptr);
+    QuantJob q = job_of(dy, m, n, dy_row_stride, dy_col_stride, fmt, dx ? dy_along_n : nullptr, dw ? dy_along_m : nullptr);
     int rc = quantize(&q, 1, dy_dtype, fmt, round_up != 0, reinterpret_cast<cudaStream_t>(stream));
     if (rc == OZK_OK && dx) rc = product(dy_along_n, w_along_n, fmt, m, k, n, dx, dx_dtype, err, stream);
     if (rc == OZK_OK && dw) rc = product(dy_along_m, x_along_m, fmt, n, k, m, dw, dw_dtype, err, stream);

@@ -166,10 +166,11 @@ __device__ __forceinline__ void store8(T* __restrict__ p, bool whole, int count,
 
 // ---- rows that start anywhere ----
 // The lanes of a row read the aligned 16 bytes ("granules") that cover it, each its own, get the next one from their
-// neighbour and shift the two into place; bytes outside [begin, end) are never read and count as zero.
-__device__ __forceinline__ uint4 load_granule(uintptr_t at, uintptr_t begin, uintptr_t end) {
+// neighbour and shift the two into place.  Granules from a row's end on are not read; of the others the matrix's first and
+// last may reach out of it, and are read value by value: bytes outside [begin, end) never are.
+__device__ __forceinline__ uint4 load_granule(uintptr_t at, uintptr_t row_end, uintptr_t begin, uintptr_t end) {
+    if (at >= row_end) return make_uint4(0u, 0u, 0u, 0u);
     if (at >= begin && at + 16 <= end) return __ldg(reinterpret_cast<const uint4*>(at));
-    if (at >= end) return make_uint4(0u, 0u, 0u, 0u);
     uint16_t e[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
@@ -178,6 +179,14 @@ __device__ __forceinline__ uint4 load_granule(uintptr_t at, uintptr_t begin, uin
     }
     return make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16, e[4] | (uint32_t)e[5] << 16,
                       e[6] | (uint32_t)e[7] << 16);
+}
+// the first `count` of eight 16-bit values, zeros behind
+__device__ __forceinline__ uint4 keep8(uint4 w, int count) {
+    if (count >= 8) return w;
+    uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int j = 0; j < 4; j++) u[j] = count >= 2 * j + 2 ? u[j] : count == 2 * j + 1 ? u[j] & 0xffffu : 0u;
+    return make_uint4(u[0], u[1], u[2], u[3]);
 }
 __device__ __forceinline__ uint4 next_lane(uint4 g) {
     return make_uint4(__shfl_down_sync(0xffffffffu, g.x, 1), __shfl_down_sync(0xffffffffu, g.y, 1),

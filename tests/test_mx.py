@@ -464,7 +464,7 @@ def test_rms_norm(pkg, name, fmt):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("d", [1032, 2056, 4104, 8200])
+@pytest.mark.parametrize("d", [264, 777, 1032, 1999, 2056, 3001, 4104, 4098, 8191, 8200, 8201])
 def test_rms_norm_many_rows(pkg, d):
     """Rows enough for the kernel that streams them: the last ones against the definition, a row of NaN, one of squares
     beyond FP32, and all of them against the same rows in small batches (another kernel, other orders of the sum)."""
@@ -479,8 +479,13 @@ def test_rms_norm_many_rows(pkg, d):
         q, s = pkg.mx_rms_norm(x, w, residual=r, fmt=fmt)
         got = q.dequantize(torch.float32)
         assert np.isnan(_f64(got[rows - 3])).all()
-        if with_res:
+        if r is not None:
             assert torch.equal(s.nan_to_num(), (x.float() + r.float()).to(x.dtype).nan_to_num())
+        off, base = 3, _put(rng.standard_normal((rows, d + 7)), name)   # strided rows that start anywhere
+        v = base[:, off:off + d]
+        a, b = pkg.mx_rms_norm(v, w, residual=v, fmt=fmt), pkg.mx_rms_norm(v.contiguous(), w, residual=v.contiguous(), fmt=fmt)
+        assert torch.equal(a[1], (2 * v.float()).to(x.dtype)) and torch.equal(a[1], b[1])
+        assert (a[0].dequantize() != b[0].dequantize()).sum() <= 64 + rows * d * 2.0 ** -16
         keep = [0, 1, rows // 2, rows - 2, rows - 1]
         _, y = _norm_want(_f64(x[keep]), _f64(w), None if r is None else _f64(r[keep]), 1e-6)
         sub = pkg.MXMatrix.from_codes(q.codes()[keep].contiguous(), q.scales()[keep].contiguous(), fmt, d)
