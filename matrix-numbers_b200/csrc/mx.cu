@@ -506,51 +506,26 @@ __device__ __forceinline__ void emit_chunk(float (&o)[8], bool up, int c, bool i
     if (in && (c & 15) == 0) *reinterpret_cast<uint32_t*>(tr + (long long)(c / 16) * TILE_BYTES) = four;
 }
 
-// Eight values of a row as they lie in memory.  Rows that do not start on 16 bytes: the aligned granules from the one that
-// holds the first value, and in a warp's last lane the one behind; `get` shifts them into place (called by whole warps).
-template <typename T, bool ALIGNED>
+// Eight neighbouring values as they lie in memory: unit c of a row, the 8 sizeof(T) bytes x c behind the 16-byte boundary at
+// or before its first value, holds the values from 8 c - lead on (lead: the values between the boundary and the row).
+template <typename T>
 struct Raw8 {
     static constexpr int NG = sizeof(T) / 2;
-    uint4 w[NG], tail;
-    __device__ __forceinline__ void clear() {
+    uint4 w[NG];
+    // vectors from the row's end on are zero; those that pass the matrix's end are read value by value
+    __device__ __forceinline__ void load(uintptr_t unit, uintptr_t row_end, uintptr_t end) {
 #pragma unroll
-        for (int i = 0; i < NG; i++) w[i] = make_uint4(0u, 0u, 0u, 0u);
-        tail = make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < NG; i++) w[i] = load_granule(unit + 16 * i, row_end, 0, end);
     }
-    // values 8 c .. 8 c + 7 of a row of d; zeros behind its end
-    __device__ __forceinline__ void load(const T* row, int c, int d, uintptr_t begin, uintptr_t end) {
-        if constexpr (ALIGNED) {
-            if (c < d / 8) {
-#pragma unroll
-                for (int i = 0; i < NG; i++) w[i] = __ldg(reinterpret_cast<const uint4*>(row + c * 8) + i);
-            }
-        } else {
-            const uintptr_t at0 = reinterpret_cast<uintptr_t>(row), row_end = at0 + (uintptr_t)d * sizeof(T);
-            const uintptr_t at = (at0 & ~(uintptr_t)15) + (uintptr_t)c * (8 * sizeof(T));
-#pragma unroll
-            for (int i = 0; i < NG; i++) w[i] = load_granule(at + 16 * i, row_end, begin, end);
-            if ((threadIdx.x & 31) == 31) tail = load_granule(at + 16 * NG, row_end, begin, end);
-        }
-    }
-    __device__ __forceinline__ void get(const T* row, int c, int d, float (&v)[8]) const {
-        uint4 u[NG];
-#pragma unroll
-        for (int i = 0; i < NG; i++) u[i] = w[i];
-        if constexpr (!ALIGNED) {
-            const uint32_t sh = (uint32_t)(reinterpret_cast<uintptr_t>(row) & 15);
-            uint4 n = next_lane(w[0]);
-            if ((threadIdx.x & 31) == 31) n = tail;
-#pragma unroll
-            for (int i = 0; i < NG; i++) u[i] = shift_granules(w[i], i + 1 < NG ? w[i + 1] : n, sh);
-        }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
             for (int i = 0; i < NG; i++) {
-                v[4 * i] = __uint_as_float(u[i].x); v[4 * i + 1] = __uint_as_float(u[i].y);
-                v[4 * i + 2] = __uint_as_float(u[i].z); v[4 * i + 3] = __uint_as_float(u[i].w);
+                v[4 * i] = __uint_as_float(w[i].x); v[4 * i + 1] = __uint_as_float(w[i].y);
+                v[4 * i + 2] = __uint_as_float(w[i].z); v[4 * i + 3] = __uint_as_float(w[i].w);
             }
         } else {
-            const uint32_t e[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+            const uint32_t e[4] = {w[0].x, w[0].y, w[0].z, w[0].w};
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 const float2 f = unpack2(e[j], (const T*)nullptr);
@@ -558,106 +533,134 @@ struct Raw8 {
                 v[2 * j + 1] = f.y;
             }
         }
-        if (!ALIGNED && c * 8 + 8 > d) {
+    }
+};
+
+// The eight values of a chunk (from 8 c on) out of the units c (`v`) and c + 1: the next lane's, or for a warp's last lane
+// the ones that the next warp left in `edge`
+template <int LEAD>
+__device__ __forceinline__ void take_chunk(float (&v)[8], const float* edge, bool last) {
+    float o[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (c * 8 + j >= d) v[j] = 0.0f;
+    for (int j = 0; j < 8; j++) {
+        if (j + LEAD < 8) {
+            o[j] = v[(j + LEAD) & 7];
+        } else {
+            const float n = __shfl_down_sync(0xffffffffu, v[(j + LEAD) & 7], 1);
+            o[j] = last ? edge[(j + LEAD) & 7] : n;
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 8; j++) v[j] = o[j];
+}
+
+// Eight values of type T kept in as few registers as they need
+template <typename T>
+struct Kept8 {
+    uint32_t w[2 * sizeof(T)];
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int j = 0; j < 2 * (int)sizeof(T); j++) {
+            if constexpr (sizeof(T) == 4) w[j] = __float_as_uint(v[j]);
+            else w[j] = pack2(v[2 * j], v[2 * j + 1], (const T*)nullptr);
+        }
+    }
+    __device__ __forceinline__ float get(int j) const {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[j]);
+        } else {
+            const float2 f = unpack2(w[j / 2], (const T*)nullptr);
+            return j & 1 ? f.y : f.x;
         }
     }
 };
 
-// Values 8 c .. 8 c + 7 of a row of d to memory that need not be aligned (called by whole warps): each lane stores the
-// granule that ends its neighbour's values and begins its own; a warp's two ends, a row's end and FP32 go one by one.
-template <typename T>
-__device__ __forceinline__ void store8_any(T* row, int c, int d, const float (&v)[8]) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int j = 0; j < 8; j++)
-            if (c * 8 + j < d) row[c * 8 + j] = v[j];
-    } else {
-        const T* const type = nullptr;
-        const int lane = threadIdx.x & 31, lead = (int)(reinterpret_cast<uintptr_t>(row) & 15) / 2;   // values of the granule
-        const uint4 own = make_uint4(pack2(v[0], v[1], type), pack2(v[2], v[3], type), pack2(v[4], v[5], type),   // before the row
-                                     pack2(v[6], v[7], type));
-        const uint4 before = make_uint4(__shfl_up_sync(0xffffffffu, own.x, 1), __shfl_up_sync(0xffffffffu, own.y, 1),
-                                        __shfl_up_sync(0xffffffffu, own.z, 1), __shfl_up_sync(0xffffffffu, own.w, 1));
-        const uint4 g = lead ? shift_granules(before, own, (uint32_t)(16 - 2 * lead)) : own;
-        const int first = c * 8 - lead;                         // the row's value at the granule's start
-        if ((lane > 0 || lead == 0) && first >= 0 && first + 8 <= d) {
-            *reinterpret_cast<uint4*>(row + first) = g;
-        } else {
-            // the granule's values that are this lane's own (lane 0) or anyone's, and inside the row
-            const uint32_t e[4] = {g.x, g.y, g.z, g.w};
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int k = first + j;
-                if (k >= 0 && k < d && (lane > 0 || j >= lead))
-                    reinterpret_cast<uint16_t*>(row)[k] = (uint16_t)(e[j / 2] >> (16 * (j & 1)));
-            }
-        }
-        if (lane == 31) {                                       // its last values are in the next warp's first granule
-            const uint32_t e[4] = {own.x, own.y, own.z, own.w};
-#pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (j >= 8 - lead && c * 8 + j < d)
-                    reinterpret_cast<uint16_t*>(row)[c * 8 + j] = (uint16_t)(e[j / 2] >> (16 * (j & 1)));
-        }
-    }
-}
+// Many rows that fit into the registers of TPR threads (NC units of eight values each): CTAs stay and take rows in turn, with
+// the next row's loads under way while a row is summed and encoded, and the weights in registers.  Rows need not start on
+// 16 bytes (`SHIFTED`), as long as those of x, residual and sum do so alike: everything up to the sum of squares and the
+// new residual happens in units of memory, and only then do the values move by `lead` places to where their blocks of 32
+// begin.  bf16 16384 x 8192 with the residual to e4m3: 166 us, 5.7 TB/s (264 us with a CTA a row).
+// CTAs an SM: 1024 threads with 64 registers, 768 with 85 for three units a thread
+constexpr int stream_blocks(int tpr, int nc) { return (nc > 2 ? 768 : 1024) / tpr; }
 
-// Many rows that fit into the registers of TPR threads (d at most 8 TPR NC): CTAs stay and take rows in turn, with the
-// next row's loads under way while a row is summed and encoded, and the weights in registers.  bf16 16384 x 8192 with the
-// residual to e4m3: 168 us, 5.6 TB/s (264 us with a CTA a row).
-template <typename T, typename W, int FMT, int TPR, int NC, bool RES, bool ALIGNED>
-__global__ void __launch_bounds__(TPR, ALIGNED || TPR == 1024 ? 1024 / TPR : 768 / TPR)
+template <typename T, typename W, int FMT, int TPR, int NC, bool RES, bool SHIFTED>
+__global__ void __launch_bounds__(TPR, stream_blocks(TPR, NC))
     rms_norm_stream_kernel(const T* __restrict__ x, long long x_stride, const T* __restrict__ residual, long long res_stride,
                            const W* __restrict__ weight, int rows, int d, double inv_d, float eps, bool weight_aligned, bool up,
                            T* __restrict__ sum, uint8_t* __restrict__ codes, uint8_t* __restrict__ scales) {
     __shared__ double part[2][32];
-    const int t = threadIdx.x, chunks = padded_k(d) / 8;
-    Raw8<T, ALIGNED> rx[NC], rr[RES ? NC : 1];
-    float w[NC][8];
-    const uintptr_t x_begin = reinterpret_cast<uintptr_t>(x), x_end = reinterpret_cast<uintptr_t>(x + (rows - 1) * x_stride + d);
-    const uintptr_t r_begin = reinterpret_cast<uintptr_t>(residual), r_end = reinterpret_cast<uintptr_t>(residual + (rows - 1) * res_stride + d);
+    __shared__ __align__(16) float edge[SHIFTED ? 2 : 1][SHIFTED ? NC : 1][SHIFTED ? TPR / 32 + 1 : 1][8];
+    const int t = threadIdx.x, warp = t >> 5, lane = t & 31, chunks = padded_k(d) / 8;
+    Raw8<T> rx[NC], rr[RES ? NC : 1];
+    Kept8<W> w[NC];
+    const uintptr_t x_end = reinterpret_cast<uintptr_t>(x + (rows - 1) * x_stride + d);
+    const uintptr_t r_end = reinterpret_cast<uintptr_t>(residual + (rows - 1) * res_stride + d);
     auto fetch = [&](int row) {
+        const uintptr_t px = reinterpret_cast<uintptr_t>(x + row * x_stride), pr = reinterpret_cast<uintptr_t>(residual + row * res_stride);
+        const uintptr_t bytes = (uintptr_t)d * sizeof(T);
 #pragma unroll
         for (int i = 0; i < NC; i++) {
-            rx[i].load(x + row * x_stride, t + i * TPR, d, x_begin, x_end);
-            if (RES) rr[i].load(residual + row * res_stride, t + i * TPR, d, r_begin, r_end);
+            const uintptr_t at = (uintptr_t)(t + i * TPR) * (8 * sizeof(T));
+            rx[i].load((px & ~(uintptr_t)15) + at, px + bytes, x_end);
+            if (RES) rr[i].load((pr & ~(uintptr_t)15) + at, pr + bytes, r_end);
         }
     };
 #pragma unroll
     for (int i = 0; i < NC; i++) {
-        rx[i].clear();
-        if (RES) rr[i].clear();
         const int col = (t + i * TPR) * 8;
-        load8(weight + col, weight_aligned && col + 8 <= d, max(0, d - col), w[i]);
+        float u[8];
+        load8(weight + col, weight_aligned && col + 8 <= d, max(0, d - col), u);
+        w[i].set(u);
     }
+    if (SHIFTED && t < NC * 16) edge[t / 8 & 1][t / 16][TPR / 32][t & 7] = 0.0f;   // behind the last unit
     fetch(blockIdx.x);
     const long long pitch = code_pitch(FMT, d);
     int turn = 0;
     for (int row = blockIdx.x; row < rows; row += gridDim.x, turn ^= 1) {
+        const int lead = SHIFTED ? (int)((reinterpret_cast<uintptr_t>(x + row * x_stride) & 15) / sizeof(T)) : 0;
         float v[NC][8];
         float sq = 0.0f;
 #pragma unroll
         for (int i = 0; i < NC; i++) {
-            rx[i].get(x + row * x_stride, t + i * TPR, d, v[i]);
+            rx[i].get(v[i]);
             if (RES) {
                 float q[8];
-                rr[i].get(residual + row * res_stride, t + i * TPR, d, q);
+                rr[i].get(q);
 #pragma unroll
                 for (int j = 0; j < 8; j++) v[i][j] += q[j];
+            }
+            const int k = (t + i * TPR) * 8 - lead;             // the row's value that the unit begins with
+            if (k < 0 || k + 8 > d) {
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (k + j < 0 || k + j >= d) v[i][j] = 0.0f;
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) sq = fmaf(v[i][j], v[i][j], sq);
         }
         if (row + (int)gridDim.x < rows) fetch(row + (int)gridDim.x);
         if (sum) {
+            T* to = sum + row * (long long)d;
 #pragma unroll
             for (int i = 0; i < NC; i++) {
-                T* to = sum + row * (long long)d;
-                if (!ALIGNED) store8_any(to, t + i * TPR, d, v[i]);
-                else if (t + i * TPR < d / 8) store8(to + (t + i * TPR) * 8, true, 8, v[i]);
+                const int k = (t + i * TPR) * 8 - lead;
+                if (k >= 0 && k + 8 <= d) {
+                    store8(to + k, true, 8, v[i]);
+                } else if (k + 8 > 0 && k < d) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++)
+                        if (k + j >= 0 && k + j < d) to[k + j] = from_f32<T>(v[i][j]);
+                }
+            }
+        }
+        if (SHIFTED && lane == 0) {                             // for the last lane of the warp before
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const int slot = warp > 0 ? i : i - 1;
+                if (slot < 0) continue;
+                float4* e = reinterpret_cast<float4*>(edge[turn][slot][warp > 0 ? warp : TPR / 32]);
+                e[0] = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                e[1] = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
             }
         }
         double total = row_sum<TPR>(sq, part[turn]);
@@ -674,12 +677,28 @@ __global__ void __launch_bounds__(TPR, ALIGNED || TPR == 1024 ? 1024 / TPR : 768
             total = row_sum<TPR>(sq, part[turn]) * 0x1p140;
         }
         const float rstd = inverse_root(total * inv_d + (double)eps);
+        if (SHIFTED) {
+            auto shift = [&](auto take) {
+#pragma unroll
+                for (int i = 0; i < NC; i++) take(v[i], edge[turn][i][warp + 1], lane == 31);
+            };
+            switch (lead) {
+                case 1: shift(take_chunk<1>); break;
+                case 2: shift(take_chunk<2>); break;
+                case 3: shift(take_chunk<3>); break;
+                case 4: shift(take_chunk<4>); break;
+                case 5: shift(take_chunk<5>); break;
+                case 6: shift(take_chunk<6>); break;
+                case 7: shift(take_chunk<7>); break;
+                default: break;
+            }
+        }
         uint8_t* cr = codes + row * pitch;
         uint8_t* tr = scales + (row / TILE) * (long long)(chunks / 16) * TILE_BYTES + scale_slot(row % TILE, 0);
 #pragma unroll
         for (int i = 0; i < NC; i++) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * w[i][j] * rstd;
+            for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * w[i].get(j) * rstd;
             emit_chunk<FMT>(v[i], up, t + i * TPR, t + i * TPR < chunks, cr, tr);
         }
     }
@@ -931,23 +950,29 @@ int launch_norm(const NormArgs& a) {
             static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps, aligned, a.up, static_cast<T*>(a.sum), a.codes, a.scales)
 #define OZK_STREAM(TPR, NC)                                                                                          \
     {                                                                                                                \
-        auto kern = aligned8 ? (a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true, true>                  \
-                                           : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false, true>)                \
-                             : (a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true, false>                 \
-                                           : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false, false>);              \
-        const int grid = a.sms * (aligned8 || TPR == 1024 ? 1024 / TPR : 768 / TPR);                                 \
+        auto kern = whole ? (a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true, false>                    \
+                                        : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false, false>)                  \
+                          : (a.residual ? rms_norm_stream_kernel<T, W, FMT, TPR, NC, true, true>                     \
+                                        : rms_norm_stream_kernel<T, W, FMT, TPR, NC, false, true>);                  \
+        const int grid = a.sms * stream_blocks(TPR, NC);                                                             \
         kern<<<(unsigned)(a.rows < grid ? a.rows : grid), TPR, 0, a.st>>>(                                           \
             static_cast<const T*>(a.x), a.x_stride, static_cast<const T*>(a.residual), a.res_stride,                 \
             static_cast<const W*>(a.weight), a.rows, d, 1.0 / d, a.eps, aligned16(a.weight), a.up,                   \
             static_cast<T*>(a.sum), a.codes, a.scales);                                                              \
     }
-    // rows enough for every CTA to take several: the streaming kernel
-    const bool aligned8 = aligned && d % 8 == 0;
-    if (d > 256 && d <= 16384 && a.rows >= 4 * a.sms) {
-        if (d <= 1024) OZK_STREAM(128, 1)
-        else if (d <= 2048) OZK_STREAM(256, 1)
-        else if (d <= 4096) OZK_STREAM(256, 2)
-        else if (d <= 8192) OZK_STREAM(512, 2)
+    // rows enough for every CTA to take several, and all three tensors' rows at the same place of their 16 bytes: the
+    // streaming kernel (with rows that start anywhere, one unit more than the chunks of eight may be needed)
+    const bool whole = aligned;
+    const bool alike = aligned16(a.x) && aligned16(a.residual) && aligned16(a.sum) &&
+                       (!a.residual || (a.res_stride - a.x_stride) * size % 16 == 0) &&
+                       (!a.sum || (d - a.x_stride) * size % 16 == 0);
+    const int need = d + (whole ? 0 : 8);
+    if ((whole || alike) && d > 256 && need <= 16384 && a.rows >= 4 * a.sms) {
+        if (need <= 1024) OZK_STREAM(128, 1)
+        else if (need <= 2048) OZK_STREAM(256, 1)
+        else if (need <= 4096) OZK_STREAM(256, 2)
+        else if (need <= 6144) OZK_STREAM(256, 3)
+        else if (need <= 8192) OZK_STREAM(512, 2)
         else OZK_STREAM(1024, 2)
     }
     else if (d <= 1024) OZK_NORM(32, 4);
