@@ -10,6 +10,7 @@ import os
 import shutil
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -19,7 +20,7 @@ OBJ_DIR = os.path.join(ROOT, "_build", "ozaki_b200")
 LIB = os.path.join(OUT_DIR, "libozaki_b200.so")
 
 SOURCES = ["capi.cu", "stats.cu", "rule.cu", "split.cu", "split_tc.cu", "gemm_tc.cu", "recon.cu", "certificate.cu", "chain.cu",
-           "mx.cu", "mx_gemm.cu"]
+           "mx.cu", "mx_norm.cu", "mx_gemm.cu"]
 HEADERS = ["ozk_common.cuh", "tc_ptx.cuh", "mx_common.cuh"]
 
 
@@ -45,7 +46,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(OUT_DIR, exist_ok=True)
     os.makedirs(OBJ_DIR, exist_ok=True)
     hdrs = [os.path.join(HERE, h) for h in HEADERS] + [os.path.join(ROOT, "include", "ozaki_b200.h")]
-    objs = []
+    objs, stale = [], []
     for src in SOURCES:
         s = os.path.join(HERE, src)
         o = os.path.join(OBJ_DIR, src.replace(".cu", ".o"))
@@ -54,7 +55,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
             cmd = [nvcc()] + FLAGS + ["-c", s, "-o", o]
             if verbose:
                 print(" ".join(cmd), flush=True)
-            subprocess.run(cmd, check=True)
+            stale.append(cmd)
+    with ThreadPoolExecutor(max_workers=min(8, os.cpu_count() or 1)) as pool:   # one nvcc per stale source
+        for done in [pool.submit(subprocess.run, cmd, check=True) for cmd in stale]:
+            done.result()
     if force or _stale(LIB, objs):
         cmd = [nvcc(), "-shared", "-gencode", "arch=compute_100a,code=sm_100a", "-o", LIB] + objs
         if verbose:

@@ -230,4 +230,7 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t m) {
     return max(m, __shfl_xor_sync(0xffffffffu, m, 2));
 }
 
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool fmt_ok(int fmt) { return fmt == OZK_MX_E2M1 || fmt == OZK_MX_E4M3; }
+
 }  // namespace ozk_mx

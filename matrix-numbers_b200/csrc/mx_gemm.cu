@@ -864,8 +864,6 @@ int choose(const Call& c) {
     return launch<KIND, 128, false>(c, parts_for(((m + BM - 1) / BM) * nt, kblocks, c.sms));
 }
 
-bool fmt_ok(int fmt) { return fmt == OZK_MX_E2M1 || fmt == OZK_MX_E4M3; }
-
 int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const uint8_t* Bs, int Bf, int m, int n, int k,
         int groups, const int32_t* ends, int fill, void* C, int64_t ldc, int dtype, int32_t* err, ozk_stream_t stream) {
     if (!Ac || !As || !Bc || !Bs || !C || !err || !fmt_ok(Af) || !fmt_ok(Bf)) return OZK_ERR_ARG;
