@@ -20,8 +20,8 @@
 // in its shared memory, and every CTA adds one slice of the tile over the cluster in a fixed order (no workspace, no
 // atomics, one launch).
 // Grouped: `ends` is read on the device; a group's rows are covered by windows of A (of a tile's rows, from the multiple of
-// 128 or of the tile's rows at or before the group's first), and each window is multiplied with the group's B and stored
-// for the group's rows only.  So A's rows and scales stay where the quantisation put them, whatever the routing, for at
+// 128 at or before the group's first), and each window is multiplied with the group's B and stored for the group's rows
+// only.  So A's rows and scales stay where the quantisation put them, whatever the routing, for at
 // most one more tile per group than packing would need.
 // Every mbarrier wait is bounded; on a timeout the CTA records a flag in *err, stops, waits (bounded) for its own copies
 // and MMAs in flight, frees TMEM and exits.  No multicast is used.
@@ -58,7 +58,10 @@ struct Shape {
     static constexpr uint32_t L_BYTES = BM * ROW_BYTES, R_BYTES = RN * ROW_BYTES;
     static constexpr uint32_t SL_BYTES = KT * TILE_BYTES, SR_BYTES = SUBS * KT * TILE_BYTES;
     static constexpr uint32_t STAGE_BYTES = L_BYTES + R_BYTES + SL_BYTES + SR_BYTES;
-    static constexpr uint32_t OUT_BYTES = SWAP ? 0 : EPI_WARPS * OUT_WARP_BYTES;   // where C leaves by TMA
+    // where C leaves by TMA; not for B on the left (C^T), nor for groups of few rows (128 x 256 alone), whose rows seldom fill
+    // a box: there the room is a fourth stage
+    static constexpr bool BOXES = !SWAP && (PAIR || BN < 256);
+    static constexpr uint32_t OUT_BYTES = BOXES ? EPI_WARPS * OUT_WARP_BYTES : 0;
     static constexpr int FIT = (int)((SMEM_MAX - 1024 - 256 - TABLE_BYTES - OUT_BYTES) / STAGE_BYTES);
     static constexpr int STAGES = FIT < 8 ? FIT : 8;
     static constexpr size_t SMEM = (size_t)STAGES * STAGE_BYTES + OUT_BYTES + 1024 + 256 + TABLE_BYTES;
@@ -96,16 +99,13 @@ struct Args {
 };
 
 struct Unit {
-    int lg, rg;                              // group coordinates
+    int rg;                                  // group of the right operand
     int l0, r0;                              // first left and right row of the tile
     int first, last;                         // rows of A (and C) that belong to this unit's group: [first, last)
 };
 
-template <int BL, int BN, bool SWAP>
+template <int BL, int BN>
 struct Work {
-    // rows of A are taken in windows of WIN, the first of a group from a multiple of ALIGN (their scales come in tiles of
-    // 128 rows, of which a smaller window is an even part)
-    static constexpr int WIN = SWAP ? BN : BL, ALIGN = WIN < TILE ? WIN : TILE;
     const Args& a;
     const int *pre, *bound;                  // grouped: windows before group g, first row of group g
     int ltiles, rtiles;
@@ -114,13 +114,12 @@ struct Work {
     __device__ Work(const Args& a_, const int* pre_, const int* bound_) : a(a_), pre(pre_), bound(bound_) {
         ltiles = (a.l_rows + BL - 1) / BL;
         rtiles = (a.r_rows + BN - 1) / BN;
-        units = a.groups ? (long long)pre[a.groups] * (SWAP ? ltiles : rtiles) : (long long)ltiles * rtiles;
+        units = (long long)(a.groups ? pre[a.groups] : ltiles) * rtiles;
     }
     __device__ __forceinline__ Unit at(long long u) const {
         Unit w;
-        if (a.groups) {
-            const int other = SWAP ? ltiles : rtiles;
-            const int q = (int)(u / other);
+        if (a.groups) {                      // A is on the left; a group's windows next to each other, for B's columns in L2
+            const int q = (int)(u / rtiles);
             int lo = 0, hi = a.groups - 1;                  // the last group with pre[g] <= q: it has windows
             while (lo < hi) {
                 const int mid = (lo + hi + 1) >> 1;
@@ -128,20 +127,18 @@ struct Work {
             }
             w.first = bound[lo];
             w.last = bound[lo + 1];
-            const long long in = u - (long long)pre[lo] * other;
+            const long long in = u - (long long)pre[lo] * rtiles;
             const int nw = pre[lo + 1] - pre[lo];
-            const int row = w.first / ALIGN * ALIGN + (int)(in % nw) * WIN, o = (int)(in / nw);
-            w.l0 = SWAP ? o * BL : row;
-            w.r0 = SWAP ? row : o * BN;
-            w.lg = SWAP ? lo : 0;
-            w.rg = SWAP ? 0 : lo;
+            w.l0 = w.first / TILE * TILE + (int)(in % nw) * BL;
+            w.r0 = (int)(in / nw) * BN;
+            w.rg = lo;
         } else {
             const int per = GROUP_L * rtiles;
             const int g = (int)(u / per), l0 = g * GROUP_L, gl = min(ltiles - l0, GROUP_L);
             const int in = (int)(u - (long long)g * per);
             w.l0 = (l0 + in % gl) * BL;
             w.r0 = in / gl * BN;
-            w.lg = w.rg = 0;
+            w.rg = 0;
             w.first = 0;
             w.last = a.tokens;
         }
@@ -233,11 +230,12 @@ __device__ __forceinline__ void store_chunk(const Args& a, const Unit& w, int l,
 // with direct stores of 32 bytes a row, which were slower than the MMAs of K < 4096.  The edge rows of a group, and a C
 // whose rows are not aligned, take the direct stores; so do the last columns where a row of C does not end on 16 bytes (a
 // clipped box writes zeros up to there).
+template <bool BOXES>
 __device__ __forceinline__ void store_block(const Args& a, const CUtensorMap* tmC, const Unit& w, int l0, int r, int lane,
                                             uint32_t out, const uint32_t (&v0)[32], const uint32_t (&v1)[32]) {
     if (r >= a.n || l0 >= w.last || l0 + 32 <= w.first) return;
     const bool ends_inside = r + 64 > a.n && a.n * (a.dtype == OZK_F32 ? 4 : 2) % 16 != 0;
-    if (!a.vec || ends_inside || l0 < w.first || (l0 + 32 > w.last && w.last < a.tokens)) {
+    if (!BOXES || !a.vec || ends_inside || l0 < w.first || (l0 + 32 > w.last && w.last < a.tokens)) {
         store_chunk<32, false>(a, w, l0 + lane, r, v0);
         store_chunk<32, false>(a, w, l0 + lane, r + 32, v1);
         return;
@@ -294,7 +292,7 @@ __device__ __forceinline__ void store4(const Args& a, int token, int col, float4
 }
 
 // Grouped: clamp `ends` to an ascending sequence within [0, rows] and count the windows each group touches (one warp)
-template <int WIN, int ALIGN>
+template <int WIN>
 __device__ __forceinline__ void group_tables(const Args& a, int* pre, int* bound, int lane) {
     int end_before = 0, windows_before = 0;
     if (lane == 0) { pre[0] = 0; bound[0] = 0; }
@@ -309,7 +307,7 @@ __device__ __forceinline__ void group_tables(const Args& a, int* pre, int* bound
         }
         int s = __shfl_up_sync(0xffffffffu, e, 1);
         if (lane == 0) s = end_before;
-        int w = e > s ? (e - s / ALIGN * ALIGN + WIN - 1) / WIN : 0;
+        int w = e > s ? (e - s / TILE * TILE + WIN - 1) / WIN : 0;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int p = __shfl_up_sync(0xffffffffu, w, o);
@@ -334,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                    const __grid_constant__ CUtensorMap tmSL, const __grid_constant__ CUtensorMap tmSR,
                    const __grid_constant__ CUtensorMap tmC, const __grid_constant__ Args a, int parts) {
     using S = Shape<KIND, BN, SWAP, PAIR>;
-    using WorkOf = Work<S::BL, BN, SWAP>;
+    using WorkOf = Work<S::BL, BN>;
     constexpr int STAGES = S::STAGES, CHUNK = S::CHUNK;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
@@ -380,7 +378,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             tmem_relinquish();
         }
     }
-    if (warp == 2 && a.groups) group_tables<WorkOf::WIN, WorkOf::ALIGN>(a, pre, bound, lane);
+    if (!SWAP && warp == 2 && a.groups) group_tables<S::BL>(a, pre, bound, lane);
     __syncwarp();
     tc_fence_before();
     __syncthreads();
@@ -407,7 +405,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (long long u = u0; ok && u < work.units; u += du) {
             const Unit w = work.at(u);
             const int l0 = uniform(w.l0) + rank * BM, rt = uniform(w.r0), r0 = rt + rank * S::RN;
-            const int lg = uniform(w.lg), rg = uniform(w.rg);
+            const int rg = uniform(w.rg);
             for (int kb = kb0; kb < kb1; kb++) {
                 ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS);
                 if (!ok) break;
@@ -419,14 +417,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const uint32_t dl = aL + stage * S::L_BYTES, dr = aR + stage * S::R_BYTES;
                     const uint32_t dsl = aSL + stage * S::SL_BYTES, dsr = aSR + stage * S::SR_BYTES;
                     if (PAIR) {
-                        tma_load_3d_pair(dl, &tmL, kc, l0, lg, bar);
+                        tma_load_3d_pair(dl, &tmL, kc, l0, 0, bar);
                         tma_load_3d_pair(dr, &tmR, kc, r0, rg, bar);
-                        tma_load_4d_pair(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, lg, bar);
+                        tma_load_4d_pair(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, 0, bar);
                         tma_load_4d_pair(dsr, &tmSR, 0, kb * S::KT, rt / TILE, rg, bar);
                     } else {
-                        tma_load_3d(dl, &tmL, kc, l0, lg, bar);
+                        tma_load_3d(dl, &tmL, kc, l0, 0, bar);
                         tma_load_3d(dr, &tmR, kc, r0, rg, bar);
-                        tma_load_4d(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, lg, bar);
+                        tma_load_4d(dsl, &tmSL, 0, kb * S::KT, l0 / TILE, 0, bar);
                         tma_load_4d(dsr, &tmSR, 0, kb * S::KT, rt / TILE, rg, bar);
                     }
                 }
@@ -474,9 +472,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                     tc_fence_after();
                 }
                 const uint32_t d_tmem = tmem + (uint32_t)(b * S::ACC_STRIDE);
-                // the second tile of 64 right rows in a scale tile starts two columns on (32 rows a column; an MMA takes
-                // its scales from an even column, so tiles of 32 rows exist for a first tile only)
-                const uint32_t r_col = BN == 64 ? (uint32_t)uniform(work.at(u).r0 / BN & 1) * 2u : 0u;
                 auto columns = [&](uint32_t st) { return tmem + (uint32_t)(S::SCALE_BASE + (int)(st & 1u) * S::SCALE_COLS); };
                 // the four instructions of a stage: 32 bytes along K inside the swizzle atom each (+2 in the >> 4 address
                 // field); the last stage of an odd number of scale tiles has half of them
@@ -490,7 +485,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                         if (t >= tiles) break;
                         const uint32_t idesc = a.idesc | umma_idesc_scale_id(KIND == MXF4 ? 2u * (kk & 1) : (uint32_t)kk);
                         const uint32_t acc = (kb > kb0 || kk > 0) ? 1u : 0u;
-                        const uint32_t ca = tl + 4u * t, cb = tr + 4u * (uint32_t)(t * S::SUBS) + r_col;
+                        const uint32_t ca = tl + 4u * t, cb = tr + 4u * (uint32_t)(t * S::SUBS);
                         if (KIND == MXF4 && PAIR) umma_mxf4_pair(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
                         else if (KIND == MXF4) umma_mxf4(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
                         else if (PAIR) umma_mxf8f6f4_pair(d_tmem, ld + 2u * kk, rd + 2u * kk, idesc, ca, cb, acc);
@@ -620,14 +615,14 @@ __global__ void __launch_bounds__(THREADS, 1)
                         __syncwarp();
                         if (lane == 0) drained(S::LAG == 1 ? 0 : b);
                     }
-                    store_block(a, &tmC, w, l - lane, r + at, lane, smem_addr(sOut + ew * OUT_WARP_BYTES), v0, v1);
+                    store_block<S::BOXES>(a, &tmC, w, l - lane, r + at, lane, smem_addr(sOut + ew * OUT_WARP_BYTES), v0, v1);
                 }
                 tc_fence_before();
                 __syncwarp();
             }
             it++;
         }
-        if (!SWAP && lane == 0) bulk_wait_all();
+        if (S::BOXES && lane == 0) bulk_wait_all();
         // rows of C behind the last group
         if (a.groups && a.fill) {
             const int size = a.dtype == OZK_F32 ? 4 : 2;
@@ -780,7 +775,7 @@ struct Call {
 
 uint32_t format_bits(int kind, int fmt) { return kind == MXF4 ? 1u : fmt == OZK_MX_E2M1 ? 5u : 0u; }
 
-template <int KIND, int BN, bool SWAP, bool PAIR = false>
+template <int KIND, int BN, bool SWAP, bool PAIR>
 int launch(const Call& c, int parts) {
     using S = Shape<KIND, BN, SWAP, PAIR>;
     auto kern = mx_gemm_kernel<KIND, BN, SWAP, PAIR>;
@@ -799,9 +794,9 @@ int launch(const Call& c, int parts) {
     if ((rc = make_map(&tr, R, c.k, S::RN, KIND)) != OZK_OK) return rc;
     if ((rc = make_scale_map(&tsl, L, c.k, S::KT, 1)) != OZK_OK) return rc;
     if ((rc = make_scale_map(&tsr, R, c.k, S::KT, S::SUBS)) != OZK_OK) return rc;
-    if (!SWAP && parts == 1 && a.vec && (rc = make_out_map(&tc, a)) != OZK_OK) return rc;
+    if (S::BOXES && parts == 1 && a.vec && (rc = make_out_map(&tc, a)) != OZK_OK) return rc;
     const long long lt = (L.rows + S::BL - 1) / S::BL, rt = (R.rows + BN - 1) / BN;
-    if (lt * rt > 0x7fffffffLL || (BN == 32 && rt > 1)) return OZK_ERR_ARG;
+    if (lt * rt > 0x7fffffffLL || (SWAP && rt > 1)) return OZK_ERR_ARG;
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute cluster[1];
     cluster[0].id = cudaLaunchAttributeClusterDimension;
@@ -838,30 +833,39 @@ int launch(const Call& c, int parts) {
     return OZK_OK;
 }
 
-// CTAs that share one tile along K: as many as keep the grid within the SMs and leave each at least two stages
-int parts_for(long long units, int kblocks, int sms) {
+// CTAs that share one tile along K: as many as keep the grid within the SMs, with at least `least` stages each
+int parts_for(long long units, int kblocks, int sms, int least) {
     int p = 1;
-    while (p < 8 && units * p * 2 <= sms && kblocks >= 4 * p) p *= 2;
+    while (p < 8 && units * p * 2 <= sms && kblocks >= 2 * p * least) p *= 2;
     return p;
 }
 
+// Which tile.  Every stage costs about 0.25 us whatever the tile's width, so wide tiles win as soon as they fill the SMs,
+// and where they do not, K is split.  Measured, us (e4m3 x e4m3, n = k = 4096; in brackets e2m1 x e2m1):
+//   m = 16:   B left, 32 rows of A, K in four 7.7 (6.8); 64 rows 8.9 (7.5); 128 x 128 in four 10.8 (8.8); pair 15.0 (10.4)
+//   m = 64:   B left, 64 rows, K in four 8.8 (7.5); 128 x 128 in four 9.7 (8.1)
+//   m = 128:  128 x 128 in four 10.1 (8.7), unsplit 15.0 (10.1); B left, 64 rows, in two 11.6 (9.1); pair 15.6 (11.2)
+//   m = 512:  128 x 128 16.5 (10.8); pair 16.1 (11.4)
+//   m = 768:  pair 16.5 (11.7); 128 x 128 (192 tiles, more than SMs) 26.3 (16.1)
+// and with n = k = 1024, where the split's exchange costs more than it saves: m = 512 unsplit 7.3 (6.3), in four 8.0 (7.6).
+// Grouped, 16 experts of 4096 x 2048 in e2m1, A in e4m3 (in brackets e2m1), by the rows of an average group:
+//   8: 128 x 256 22.6 (15.6), pair 31.8 (23.9); 32: 30.0 (19.3), 32.3 (23.7); 64: 35.8 (21.6), 33.6 (23.7);
+//   100: 46.0 (26.8), 35.3 (24.4); 256: 73.1 (44.6), 53.6 (37.8); 1024: 181 (107), 138 (90).
+// (The 4-bit kind stays with 128 x 128 a little longer; the difference is at most 6 % and has no rule of its own.)
 template <int KIND>
 int choose(const Call& c) {
     const int kblocks = (padded_k(c.k) / TILE + (KIND == MXF4 ? 1 : 0)) / (KIND == MXF4 ? 2 : 1);
     if (c.args.groups) {
-        const int per = c.args.tokens / c.args.groups;            // rows of an average group
-        if (per <= 64) return launch<KIND, 64, true>(c, 1);
-        if (per <= 128) return launch<KIND, 128, true>(c, 1);
-        if (per <= 512) return launch<KIND, 256, false>(c, 1);
+        if (c.args.tokens / c.args.groups < 64) return launch<KIND, 256, false, false>(c, 1);
         return launch<KIND, 256, false, true>(c, 1);
     }
-    const long long m = c.A.rows, nt = (c.n + BM - 1) / BM;
-    if (m <= 32) return launch<KIND, 32, true>(c, parts_for(nt, kblocks, c.sms));
-    if (m <= 64) return launch<KIND, 64, true>(c, parts_for(nt, kblocks, c.sms));
-    const long long wide = ((m + BM - 1) / BM) * ((c.n + 255) / 256);
-    if (((m + 255) / 256) * ((c.n + 255) / 256) * 2 > c.sms) return launch<KIND, 256, false, true>(c, 1);
-    if (wide * 2 > c.sms) return launch<KIND, 256, false>(c, 1);
-    return launch<KIND, 128, false>(c, parts_for(((m + BM - 1) / BM) * nt, kblocks, c.sms));
+    const long long m = c.A.rows, nt = (c.n + BM - 1) / BM, squares = ((m + BM - 1) / BM) * nt;
+    if (m <= 64 && kblocks >= 8) {
+        const int parts = parts_for(nt, kblocks, c.sms, 2);
+        return m <= 32 ? launch<KIND, 32, true, false>(c, parts) : launch<KIND, 64, true, false>(c, parts);
+    }
+    if (squares <= c.sms) return launch<KIND, 128, false, false>(c, kblocks >= 16 ? parts_for(squares, kblocks, c.sms, 4) : 1);
+    return launch<KIND, 256, false, true>(c, 1);
 }
 
 int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const uint8_t* Bs, int Bf, int m, int n, int k,
