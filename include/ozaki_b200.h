@@ -286,8 +286,8 @@ int ozk_mx_linear_backward(const void* dy, int dy_dtype, int64_t dy_row_stride, 
                            int32_t* err, ozk_stream_t stream);
 /* Root-mean-square norm with an MX output: t = x + residual (residual may be NULL), y = t / sqrt(mean(t^2) + eps)
  * weight over rows of d values, all in FP32; y quantised as ozk_mx_quantize does, into an operand of `rows` vectors of
- * length d; t rounded to dtype into sum (rows x d, contiguous; may be NULL).  x, residual: contiguous rows, row strides
- * in elements; weight[d] of dtype, or FP32 with weight_f32.                                                   */
+ * length d; t rounded to dtype into sum (rows x d, contiguous; may be NULL; not overlapping the inputs).  x, residual:
+ * contiguous rows, row strides in elements; weight[d] of dtype, or FP32 with weight_f32.                      */
 int ozk_mx_rms_norm(const void* x, const void* residual, const void* weight, int dtype, int weight_f32, int rows, int d,
                     int64_t x_stride, int64_t residual_stride, float eps, int fmt, int round_up, void* sum,
                     uint8_t* codes, uint8_t* scales, ozk_stream_t stream);

@@ -6,6 +6,10 @@ Python entry point:
     from matrix_numbers_b200 import OzakiCRT
     C, info = OzakiCRT().run(A, B)            # A (m, k), B (k, n): float64 CUDA tensors
 
+and of the microscaled (MX) low-bit products of language models beside it:
+
+    from matrix_numbers_b200 import mx_quantize, mx_matmul, mx_grouped_matmul, mx_rms_norm, mx_linear
+
 The package directory is named ``matrix-numbers_b200``; ``__graft_entry__.load_package()`` (repository root)
 registers it under the importable name ``matrix_numbers_b200``.  The compute path is libozaki_b200.so (hand-written
 sm_100a kernels behind the C ABI in include/ozaki_b200.h); there is no CPU path.

@@ -14,8 +14,8 @@
 // instruction has at least are then rows of B, which there are plenty of, and A's tile is as small as 32 rows; C^T comes
 // out of TMEM, whose lanes are then neighbours in a row of C.
 // `PAIR`: two CTAs on neighbouring SMs share a 256 x 256 tile (cta_group::2): each holds 128 left rows and 128 right rows,
-// so a stage of the same work brings 32 KB of codes to an SM instead of 48 KB.  One CTA alone is bound by its shared
-// memory: 48 KB written and read at 128 bytes a clock is 768 clocks a stage, the MMAs need 512.
+// so a stage of the same work brings 32 KB of codes to an SM instead of 48 KB, which its shared memory would take 768 clocks
+// to write and read at 128 bytes a clock; the MMAs need 512 (2048 x 4096 x 4096 in e4m3: 28.7 us against 37.6).
 // Where there are fewer tiles than SMs, a cluster of CTAs shares one tile: each takes a part of K, leaves its FP32 sums
 // in its shared memory, and every CTA adds one slice of the tile over the cluster in a fixed order (no workspace, no
 // atomics, one launch).
@@ -23,6 +23,11 @@
 // 128 at or before the group's first), and each window is multiplied with the group's B and stored for the group's rows
 // only.  So A's rows and scales stay where the quantisation put them, whatever the routing, for at
 // most one more tile per group than packing would need.
+// The producer and the issuing warp run their loops as whole warps and let one elected lane issue: with the loops in one
+// lane alone each operand of a tcgen05 instruction was moved to a uniform register on its way, and the issue bound the
+// kernel (8192 x 4096 x 8192 in e2m1: 163 us, tensor pipe 41 % active; elected: 99 us, 75 %).
+// Measured on one B200 at its power cap (1.4 - 1.5 GHz): e2m1 16384 x 8192 x 8192 in 394 us, 5.6 PFLOP/s; e4m3 8192 x 8192 x
+// 8192 in 396 us, 2.8 PFLOP/s: four and two times the rate that the card sustains in bf16, and bound by the same cap.
 // Every mbarrier wait is bounded; on a timeout the CTA records a flag in *err, stops, waits (bounded) for its own copies
 // and MMAs in flight, frees TMEM and exits.  No multicast is used.
 #include <cuda.h>
@@ -847,6 +852,7 @@ int parts_for(long long units, int kblocks, int sms, int least) {
 //   m = 128:  128 x 128 in four 10.1 (8.7), unsplit 15.0 (10.1); B left, 64 rows, in two 11.6 (9.1); pair 15.6 (11.2)
 //   m = 512:  128 x 128 16.5 (10.8); pair 16.1 (11.4)
 //   m = 768:  pair 16.5 (11.7); 128 x 128 (192 tiles, more than SMs) 26.3 (16.1)
+// with n = 65536 (e4m3 x e2m1): m = 16: B left 45, 128 x 256 50; m = 64: 47, 42; m = 128: 128 x 128 or pair 64, 128 x 256 45;
 // and with n = k = 1024, where the split's exchange costs more than it saves: m = 512 unsplit 7.3 (6.3), in four 8.0 (7.6).
 // Grouped, 16 experts of 4096 x 2048 in e2m1, A in e4m3 (in brackets e2m1), by the rows of an average group:
 //   8: 128 x 256 22.6 (15.6), pair 31.8 (23.9); 32: 30.0 (19.3), 32.3 (23.7); 64: 35.8 (21.6), 33.6 (23.7);
@@ -860,6 +866,7 @@ int choose(const Call& c) {
         return launch<KIND, 256, false, true>(c, 1);
     }
     const long long m = c.A.rows, nt = (c.n + BM - 1) / BM, squares = ((m + BM - 1) / BM) * nt;
+    if (m > 32 && m <= 128 && c.n >= 384LL * c.sms) return launch<KIND, 256, false, false>(c, 1);
     if (m <= 64 && kblocks >= 8) {
         const int parts = parts_for(nt, kblocks, c.sms, 2);
         return m <= 32 ? launch<KIND, 32, true, false>(c, parts) : launch<KIND, 64, true, false>(c, parts);

@@ -131,7 +131,7 @@ struct Kept8 {
 // the next row's loads under way while a row is summed and encoded, and the weights in registers.  Rows need not start on
 // 16 bytes (`SHIFTED`), as long as those of x, residual and sum do so alike: everything up to the sum of squares and the
 // new residual happens in units of memory, and only then do the values move by `lead` places to where their blocks of 32
-// begin.  bf16 16384 x 8192 with the residual to e4m3: 166 us, 5.7 TB/s (264 us with a CTA a row).
+// begin.  bf16 16384 x 8192 with the residual to e4m3: 149 - 168 us, 5.6 - 6.3 TB/s (264 us with a CTA a row); bf16 8192 x 4097: 76 us (153).
 // CTAs an SM: 1024 threads with 64 registers, 768 with 85 for three units a thread
 constexpr int stream_blocks(int tpr, int nc) { return (nc > 2 ? 768 : 1024) / tpr; }
 
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(TPR, stream_blocks(TPR, NC))
         load8(weight + col, weight_aligned && col + 8 <= d, max(0, d - col), u);
         w[i].set(u);
     }
-    if (SHIFTED && t < NC * 16) edge[t / 8 & 1][t / 16][TPR / 32][t & 7] = 0.0f;   // behind the last unit
+    if (SHIFTED && t < 16) edge[t / 8][NC - 1][TPR / 32][t & 7] = 0.0f;   // behind the last unit, which no warp writes
     fetch(blockIdx.x);
     const long long pitch = code_pitch(FMT, d);
     int turn = 0;

@@ -19,6 +19,8 @@ Only ``mx_linear`` has gradients; the other results carry none, whatever their i
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import _lib
@@ -37,6 +39,7 @@ _INT_MAX = 2 ** 31 - 1
 _empty, _uint8, _Tensor = torch.empty, torch.uint8, torch.Tensor
 _current_device = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream    # handle of a device's current stream
+_error_lock = threading.Lock()
 _error_words = {}                # device index -> int32 word that the products' launches OR their flags into
 
 
@@ -79,8 +82,12 @@ def _error_word(device: int):
     if w is None:
         if torch.cuda.is_current_stream_capturing():
             raise OzkError("the first MX product on a device allocates its error word: make one call before capturing")
-        w = _error_words[device] = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
-        torch.cuda.synchronize(device)               # products on any stream may use it from here on
+        with _error_lock:
+            w = _error_words.get(device)
+            if w is None:
+                w = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+                torch.cuda.synchronize(device)       # products on any stream may use it from here on
+                _error_words[device] = w
     return w.data_ptr()
 
 
@@ -203,13 +210,18 @@ class MXMatrix:
         rows = codes.shape[-2]
         out = cls(fmt, groups, rows, k, codes.device.index)
         g = out._g
-        c = out._buffer[:out._code_bytes].view(g, rows, _padded(k) // (2 if code == 0 else 1))
+        pitch = _padded(k) // (2 if code == 0 else 1)
+        c = out._buffer[:out._code_bytes].view(g, rows, pitch)
         c[..., :per] = codes.reshape(g, rows, per)
         if code == 0 and k % 2:
             c[..., per - 1] &= 15
-        c[..., per:] = 0
+        if per < pitch:
+            c[..., per:] = 0
         rt, kt = -(-rows // TILE), _padded(k) // TILE
-        s = torch.nn.functional.pad(scales.reshape(g, rows, scales.shape[-1]), (0, 4 * kt - scales.shape[-1], 0, rt * TILE - rows))
+        s = scales.reshape(g, rows, scales.shape[-1])
+        if s.shape[1:] != (rt * TILE, 4 * kt):
+            s = torch.nn.functional.pad(s, (0, 4 * kt - s.shape[-1], 0, rt * TILE - rows))
+        s = s.contiguous()
         out._buffer[out._code_bytes:].view(g, rt, kt, 32, 4, 4).copy_(
             s.view(g, rt, 4, 32, kt, 4).permute(0, 1, 4, 3, 2, 5))
         return out
