@@ -233,13 +233,14 @@ int ozk_rule_certified(const double* nA, const double* nB, const int32_t* flag, 
  *           in the lower half;
  *   scales: [group][ceil(rows / 128)][kp / 128][512]; row r and block b of a 128 x 128 tile at 16 (r % 32) +
  *           4 (r / 32) + b.
- * No shape rule: any rows, k >= 1.  dtype: OZK_F32, OZK_F16 or OZK_BF16.                                      */
+ * No shape rule: any rows, k from 1 up to the limits below.  dtype: OZK_F32, OZK_F16 or OZK_BF16.                                      */
 #define OZK_MX_E2M1 0
 #define OZK_MX_E4M3 1
 #define OZK_F32 0
 #define OZK_F16 1
 #define OZK_BF16 2
 #define OZK_MX_KMAX (1 << 28)     /* longest contracted axis               */
+#define OZK_MX_ROWS_MAX 0x7fffff00 /* most rows of an operand               */
 #define OZK_MX_MAX_GROUPS 1024    /* most experts of one grouped product   */
 /* bytes of an operand's codes and scales; 0 for an invalid format or size */
 size_t ozk_mx_code_bytes(int fmt, int groups, int rows, int k);

@@ -231,6 +231,9 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t m) {
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+inline bool dtype_ok(int dtype) { return dtype == OZK_F32 || dtype == OZK_F16 || dtype == OZK_BF16; }
+// p points at values of that (valid) type: a null pointer does too
+inline bool on_elements(const void* p, int dtype) { return (reinterpret_cast<uintptr_t>(p) & (dtype == OZK_F32 ? 3 : 1)) == 0; }
 inline bool fmt_ok(int fmt) { return fmt == OZK_MX_E2M1 || fmt == OZK_MX_E4M3; }
 
 }  // namespace ozk_mx

@@ -878,8 +878,8 @@ int choose(const Call& c) {
 int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const uint8_t* Bs, int Bf, int m, int n, int k,
         int groups, const int32_t* ends, int fill, void* C, int64_t ldc, int dtype, int32_t* err, ozk_stream_t stream) {
     if (!Ac || !As || !Bc || !Bs || !C || !err || !fmt_ok(Af) || !fmt_ok(Bf)) return OZK_ERR_ARG;
-    if (m < 1 || n < 1 || k < 1 || k > OZK_MX_KMAX || ldc < n) return OZK_ERR_ARG;
-    if (dtype != OZK_F32 && dtype != OZK_F16 && dtype != OZK_BF16) return OZK_ERR_ARG;
+    if (m < 1 || n < 1 || m > OZK_MX_ROWS_MAX || n > OZK_MX_ROWS_MAX || k < 1 || k > OZK_MX_KMAX || ldc < n) return OZK_ERR_ARG;
+    if (!dtype_ok(dtype)) return OZK_ERR_ARG;
     const uintptr_t align = reinterpret_cast<uintptr_t>(Ac) | reinterpret_cast<uintptr_t>(Bc);
     const uintptr_t align_s = reinterpret_cast<uintptr_t>(As) | reinterpret_cast<uintptr_t>(Bs);
     const uintptr_t size = dtype == OZK_F32 ? 4 : 2;

@@ -407,10 +407,14 @@ int dispatch_norm(const NormArgs& a, bool weight_f32, int fmt) {
 extern "C" int ozk_mx_rms_norm(const void* x, const void* residual, const void* weight, int dtype, int weight_f32,
                                int rows, int d, int64_t x_stride, int64_t residual_stride, float eps, int fmt,
                                int round_up, void* sum, uint8_t* codes, uint8_t* scales, ozk_stream_t stream) {
-    if (!x || !weight || !codes || !scales || !fmt_ok(fmt) || rows < 1 || d < 1 || d > OZK_MX_KMAX) return OZK_ERR_ARG;
+    if (!x || !weight || !codes || !scales || !fmt_ok(fmt) || rows < 1 || rows > OZK_MX_ROWS_MAX || d < 1 ||
+        d > OZK_MX_KMAX)
+        return OZK_ERR_ARG;
     if (!(eps > 0.0f) || !(eps < INFINITY) || x_stride < 0 || residual_stride < 0) return OZK_ERR_ARG;
     if (!aligned16(codes) || !aligned16(scales)) return OZK_ERR_ARG;
-    if (dtype != OZK_F32 && dtype != OZK_F16 && dtype != OZK_BF16) return OZK_ERR_ARG;
+    if (!dtype_ok(dtype) || !on_elements(x, dtype) || !on_elements(residual, dtype) || !on_elements(sum, dtype) ||
+        !on_elements(weight, weight_f32 ? OZK_F32 : dtype))
+        return OZK_ERR_ARG;
     int sms = 0;
     const int rc = ozk_device_sm_count(&sms);
     if (rc != OZK_OK) return rc;

@@ -34,6 +34,7 @@ TILE = 128
 TILE_BYTES = 512
 MAX_GROUPS = 1024
 KMAX = 1 << 28
+ROWS_MAX = 0x7fffff00
 _INT_MAX = 2 ** 31 - 1
 
 _empty, _uint8, _Tensor = torch.empty, torch.uint8, torch.Tensor
@@ -59,7 +60,7 @@ def _operand_bytes(code, groups, rows, k):
     if not 1 <= k <= KMAX:
         raise ValueError(f"contracted axis of length {k}: 1 to {KMAX} required")
     kt, rt = -(-k // TILE), -(-rows // TILE)
-    if rows > _INT_MAX or groups * rt * kt > _INT_MAX:
+    if rows > ROWS_MAX or groups * rt * kt > _INT_MAX:
         raise ValueError(f"operand of {groups} x {rows} x {k} elements is too large")
     codes = groups * rows * kt * (TILE if code else TILE // 2)
     return codes, codes + groups * rt * kt * TILE_BYTES

@@ -38,11 +38,38 @@ def test_c_abi_refusals(pkg):
     L = pkg._lib.lib()
     p = 4096                                                     # an aligned address that nothing reads
     quant = [p, 0, 1, 4, 64, 0, 64, 1, 0, 0, p, p, None]
-    for at, v in [(0, None), (1, 3), (1, -1), (2, 0), (3, 0), (4, 0), (4, 2 ** 28 + 1), (5, -1), (6, -1), (7, -1),
+    for at, v in [(0, None), (0, p + 2), (1, 3), (1, -1), (2, 0), (3, 0), (4, 0), (4, 2 ** 28 + 1), (5, -1), (6, -1), (7, -1),
                   (8, 2), (10, None), (10, p + 8), (11, None), (11, p + 4)]:
         a = list(quant)
         a[at] = v
         assert L.ozk_mx_quantize(*a) == -1, (at, v)
+    for f, a, at in ((L.ozk_mx_quantize, quant, 3), (L.ozk_mx_dequantize, [p, p, 0, 1, 4, 64, p, 0, None], 4),
+                     (L.ozk_mx_gemm, [p, p, 0, p, p, 1, 4, 8, 64, p, 8, 2, p, None], 6),
+                     (L.ozk_mx_rms_norm, [p, None, p, 2, 0, 4, 64, 64, 0, 1e-6, 1, 0, None, p, p, None], 5)):
+        a = list(a)
+        a[at] = 2 ** 31 - 1                                      # rows whose tiles would not count in 32 bits
+        assert f(*a) == -1
+    both = [p, 0, 4, 64, 64, 1, 0, 0, p, p, None]
+    for at, v in [(0, None), (1, 3), (2, 0), (2, 2 ** 28 + 1), (3, 0), (4, -1), (5, -1), (6, 2), (8, None), (8, p + 16),
+                  (9, None)]:
+        a = list(both)
+        a[at] = v
+        assert L.ozk_mx_quantize_both(*a) == -1, (at, v)
+    fwd = [p, 2, 64, 1, p, 2, 64, 1, 4, 8, 64, 1, 0, p, p, None, None, p, p, None]
+    for at, v in [(0, None), (1, 4), (2, -1), (4, None), (5, -1), (7, -1), (8, 0), (9, 0), (10, 0), (11, 3), (13, None),
+                  (14, p + 8), (15, p + 8), (16, p + 4), (17, None), (18, None)]:
+        a = list(fwd)
+        a[at] = v
+        assert L.ozk_mx_linear_forward(*a) == -1, (at, v)
+    bwd = [p, 2, 8, 1, p, p, 4, 8, 64, 1, 0, p, p, p, 2, p, 2, p, None]
+    for at, v in [(0, None), (0, p + 1), (1, 3), (2, -1), (4, None), (5, None), (6, 0), (7, 0), (8, 0), (9, 2), (11, None),
+                  (12, None), (13, p + 1), (14, 3), (15, p + 1), (16, -1), (17, None)]:
+        a = list(bwd)
+        a[at] = v
+        assert L.ozk_mx_linear_backward(*a) == -1, (at, v)
+    a = list(bwd)
+    a[13] = a[15] = None
+    assert L.ozk_mx_linear_backward(*a) == -1                    # no gradient wanted
     assert L.ozk_mx_quantize(p, 0, 2 ** 16, 2 ** 30, 2 ** 20, 0, 64, 1, 0, 0, p, p, None) == -1   # more tiles than a grid
     deq = [p, p, 0, 1, 4, 64, p, 0, None]
     for at, v in [(0, None), (0, p + 8), (1, None), (2, 5), (3, 0), (4, 0), (5, 0), (6, None), (6, p + 2), (7, 3)]:
@@ -61,7 +88,7 @@ def test_c_abi_refusals(pkg):
         a[at] = v
         assert L.ozk_mx_grouped_gemm(*a) == -1, (at, v)
     norm = [p, None, p, 2, 0, 4, 64, 64, 0, 1e-6, 1, 0, None, p, p, None]
-    for at, v in [(0, None), (2, None), (3, 7), (5, 0), (6, 0), (7, -1), (8, -1), (9, 0.0), (9, float("nan")),
+    for at, v in [(0, None), (0, p + 1), (1, p + 1), (2, None), (2, p + 1), (12, p + 1), (3, 7), (5, 0), (6, 0), (7, -1), (8, -1), (9, 0.0), (9, float("nan")),
                   (9, float("inf")), (10, 2), (13, None), (13, p + 8), (14, None)]:
         a = list(norm)
         a[at] = v
