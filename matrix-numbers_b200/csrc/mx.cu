@@ -25,40 +25,33 @@ __device__ __forceinline__ void copy_scale_tile(uint8_t* __restrict__ to, const 
         reinterpret_cast<uint4*>(to)[threadIdx.x] = reinterpret_cast<const uint4*>(sc)[threadIdx.x];
 }
 
-// Eight consecutive values of which 16 bytes need not be aligned: the aligned vectors around them, shifted into place,
-// where those lie within [begin, end); one by one otherwise.
-template <typename T>
-__device__ __forceinline__ void load8_any(const T* __restrict__ p, int count, uintptr_t begin, uintptr_t end,
+// Eight consecutive FP32 values that need not be aligned to 16 bytes: the three aligned vectors around them, shifted into
+// place, where those lie within [begin, end); one by one otherwise.
+__device__ __forceinline__ void load8_any(const float* __restrict__ p, int count, uintptr_t begin, uintptr_t end,
                                           float (&v)[8]) {
-    constexpr int NV = sizeof(T) == 4 ? 3 : 2, NW = 4 * NV;
     const uintptr_t at = reinterpret_cast<uintptr_t>(p), a0 = at & ~(uintptr_t)15;
     const uint32_t sh = (uint32_t)(at & 15);
-    if (count < 8 || a0 < begin || a0 + 16 * NV > end) {
+    if (count < 8 || a0 < begin || a0 + 48 > end) {
         load8(p, false, count, v);
         return;
     }
-    uint32_t w[NW + 2];
+    float w[14];
 #pragma unroll
-    for (int q = 0; q < NV; q++) {
-        const uint4 u = __ldg(reinterpret_cast<const uint4*>(a0) + q);
+    for (int q = 0; q < 3; q++) {
+        const float4 u = __ldg(reinterpret_cast<const float4*>(a0) + q);
         w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
     }
-    w[NW] = w[NW + 1] = 0u;
+    w[12] = w[13] = 0.0f;
     if (sh & 8u) {
 #pragma unroll
-        for (int j = 0; j < NW; j++) w[j] = w[j + 2];
+        for (int j = 0; j < 12; j++) w[j] = w[j + 2];
     }
     if (sh & 4u) {
 #pragma unroll
-        for (int j = 0; j < NW; j++) w[j] = w[j + 1];
+        for (int j = 0; j < 12; j++) w[j] = w[j + 1];
     }
-    if (sizeof(T) == 2 && (sh & 2u)) {
 #pragma unroll
-        for (int j = 0; j < NW; j++) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
-    }
-    const T* e = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int j = 0; j < 8; j++) v[j] = to_f32(e[j]);
+    for (int j = 0; j < 8; j++) v[j] = w[j];
 }
 
 // One row's eight values per lane (16 lanes a row of the tile) to codes in global memory and the scale byte in `sc`: a
