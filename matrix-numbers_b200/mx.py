@@ -59,6 +59,8 @@ def _operand_bytes(code, groups, rows, k):
     """(bytes of the codes, a multiple of 64; bytes of codes and scales) of an operand."""
     if not 1 <= k <= KMAX:
         raise ValueError(f"contracted axis of length {k}: 1 to {KMAX} required")
+    if rows < 0 or groups < 0:
+        raise ValueError(f"operand of {groups} x {rows} x {k} elements: negative sizes")
     kt, rt = -(-k // TILE), -(-rows // TILE)
     if rows > ROWS_MAX or groups * rt * kt > _INT_MAX:
         raise ValueError(f"operand of {groups} x {rows} x {k} elements is too large")
@@ -71,6 +73,18 @@ def _new_operand(fmt, code, groups, rows, k, device):
     code_bytes, total = _operand_bytes(code, 1 if groups is None else groups, rows, k)
     out = object.__new__(MXMatrix)
     out._take(fmt, code, groups, rows, k, device, code_bytes, _empty(total, dtype=_uint8, device=_DEVICES[device]))
+    return out
+
+
+def _from_buffer(fmt, groups, rows, k, buffer):
+    """The operand whose codes and scales are ``buffer``."""
+    code = _format(fmt)
+    code_bytes, total = _operand_bytes(code, 1 if groups is None else groups, rows, k)
+    if not isinstance(buffer, _Tensor) or not buffer.is_cuda or buffer.dtype != _uint8 or not buffer.is_contiguous() \
+            or tuple(buffer.shape) != (total,):
+        raise ValueError(f"an operand's {total} bytes as a contiguous uint8 CUDA tensor required")
+    out = object.__new__(MXMatrix)
+    out._take(fmt, code, groups, rows, k, buffer.get_device(), code_bytes, buffer)
     return out
 
 
@@ -169,6 +183,10 @@ class MXMatrix:
     @property
     def _g(self):
         return 1 if self.groups is None else self.groups
+
+    def __reduce__(self):
+        """Copies and pickles hold the buffer, and take their addresses from their own."""
+        return _from_buffer, (self.fmt, self.groups, self.rows, self.k, self._buffer)
 
     def record_stream(self, stream):
         """As ``torch.Tensor.record_stream``: the operand is also used on ``stream``, so its memory is not handed out again

@@ -810,6 +810,46 @@ def test_stream_recorded(pkg):
     assert torch.equal(got, want) and len(junk) == 8
 
 
+def test_operand_from_a_pickle_is_checked(pkg):
+    import torch
+    for args in [("e2m1", None, 4, 64, torch.zeros(768, dtype=torch.uint8)), ("e2m1", None, 4, 64, None),
+                 ("e2m1", None, -4, 64, None), ("e2m1", -1, -4, 64, None)]:
+        with pytest.raises(ValueError):
+            pkg.mx._from_buffer(*args)
+    for groups, rows in ((None, -4), (-1, 4), (-1, -4)):
+        with pytest.raises(ValueError):
+            pkg.MXMatrix("e2m1", groups, rows, 64, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+def test_copies_stand_alone(pkg, fmt):
+    """A deep copy, a shallow one and a pickle outlive the operand they were taken from, and a deep one is another memory."""
+    import copy
+    import io
+    import torch
+    rng = np.random.default_rng(31)
+    x = _put(rng.standard_normal((3, 37, 100)), "float32")
+    for of in (x, x[1]):
+        q = pkg.mx_quantize(of, fmt)
+        want = q.dequantize(torch.float32)
+        stored = io.BytesIO()
+        torch.save(q, stored)
+        stored.seek(0)
+        copies = [copy.deepcopy(q), copy.copy(q), torch.load(stored, weights_only=False)]
+        assert copies[1]._code_ptr == q._code_ptr
+        assert len({c._code_ptr for c in (*copies, q)}) == 3
+        for c in copies:
+            assert (c._code_ptr, c._scale_ptr - c._code_ptr) == (c._buffer.data_ptr(), q._scale_ptr - q._code_ptr)
+        q._buffer.fill_(1)                                       # reaches the shallow copy alone
+        for c, same in zip(copies, (True, False, True)):
+            assert c.shape == q.shape and c.fmt == fmt and torch.equal(c.dequantize(torch.float32), want) == same
+        del q
+        for c in (copies[0], copies[2]):
+            if c.groups is None:
+                assert torch.equal(pkg.mx_matmul(c, copies[0]), pkg.mx_matmul(pkg.mx_quantize(of, fmt), copies[0]))
+
+
 @pytest.mark.gpu
 def test_empty_operands(pkg):
     import torch
