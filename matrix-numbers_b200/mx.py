@@ -22,6 +22,7 @@ from __future__ import annotations
 import threading
 
 import torch
+from torch.autograd import forward_ad as _forward_ad
 
 from . import _lib
 from ._lib import OzkError, check
@@ -40,6 +41,7 @@ _INT_MAX = 2 ** 31 - 1
 _empty, _uint8, _Tensor = torch.empty, torch.uint8, torch.Tensor
 _current_device = torch._C._cuda_getDevice
 _stream_of = torch._C._cuda_getCurrentRawStream    # handle of a device's current stream
+_increment_version = torch.autograd.graph.increment_version
 _error_lock = threading.Lock()
 _error_words = {}                # device index -> int32 word that the products' launches OR their flags into
 
@@ -145,6 +147,8 @@ def _dtype(dtype, what):
 def _tensor(t, what):
     if not isinstance(t, _Tensor) or not t.is_cuda:
         raise ValueError(f"{what}: CUDA tensor required (there is no CPU path)")
+    if t.is_neg():
+        raise ValueError(f"{what}: a view whose sign is still to be turned (see torch.Tensor.resolve_neg)")
     code = _DTYPES.get(t.dtype)
     return _dtype(t.dtype, what) if code is None else code
 
@@ -345,6 +349,10 @@ def _result(C, rows, cols, dtype, device):
     if C.device.index != device or tuple(C.shape) != (rows, cols) or (cols > 1 and C.stride(1) != 1) \
             or (rows > 1 and C.stride(0) < cols):
         raise ValueError(f"C: ({rows}, {cols}) on cuda:{device} with contiguous, separate rows required")
+    if C.requires_grad and torch.is_grad_enabled():
+        raise ValueError("C: requires a gradient, which the product does not give")
+    if not C.is_inference():
+        _increment_version(C)                   # a backward pass that kept the old C has to notice
     return C, d, C.stride(0) if rows > 1 else max(cols, 1)
 
 
@@ -408,12 +416,13 @@ def mx_rms_norm(x, weight, residual=None, eps=1e-6, fmt="e4m3", rule="floor"):
     n = shape[-1]
     device, dtype = x.get_device(), x.dtype
     if not isinstance(weight, _Tensor) or weight.get_device() != device or weight.shape != shape[-1:] \
-            or not (weight.dtype is dtype or weight.dtype is torch.float32) or not weight.is_contiguous():
+            or not (weight.dtype is dtype or weight.dtype is torch.float32) or not weight.is_contiguous() \
+            or weight.is_neg():
         raise ValueError(f"weight: contiguous ({n},) tensor of x's type or float32 on its device required")
     if not 0.0 < eps < float("inf"):
         raise ValueError(f"eps {eps}: a positive number required")
     if residual is not None and (not isinstance(residual, _Tensor) or residual.shape != shape
-                                 or residual.dtype is not dtype or residual.get_device() != device):
+                                 or residual.dtype is not dtype or residual.get_device() != device or residual.is_neg()):
         raise ValueError("residual: a tensor of x's shape, type and device required")
     if _current_device() != device:
         with torch.cuda.device(device):
@@ -475,6 +484,8 @@ def _linear_forward(x2, weight, code, up, need_dx, need_dw):
 
 def _linear_backward(ctx, dy):
     kept, = ctx.saved_tensors
+    if dy.is_neg():                             # of y in a conjugate's imaginary part
+        dy = dy.resolve_neg()
     code, up, need_dx, need_dw, x_code, w_code, w_dtype, n, k = ctx.how
     device, m = dy.get_device(), dy.shape[0]
     dev = _DEVICES[device]
@@ -523,7 +534,7 @@ def mx_linear(x, weight, fmt="e4m3", rule="floor"):
 
     Every operand is quantised along the axis its product contracts: y from x and weight along k, dx = dy weight from
     both along n, dweight = dy^T x from both along the rows of x.  The roundings themselves are passed over in the
-    backward pass (their derivative is taken as one).  A second derivative is refused.  A captured backward pass needs
+    backward pass (their derivative is taken as one).  A second derivative and forward-mode differentiation are refused.  A captured backward pass needs
     what torch needs of any: no eager graph of the same leaves alive on another stream."""
     _tensor(x, "x")
     _tensor(weight, "weight")
@@ -542,7 +553,7 @@ def mx_linear(x, weight, fmt="e4m3", rule="floor"):
         return torch.matmul(x, weight.t().to(x.dtype))        # nothing to multiply: empty, with its gradients of zero
     plain = len(shape) == 2
     x2 = x if plain else x.reshape(-1, k)
-    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled():
+    if (x.requires_grad or weight.requires_grad) and torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         y = _MXLinear.apply(x2, weight, code, up)
     else:
         y = _linear_forward(x2, weight, code, up, False, False)[0]

@@ -851,6 +851,58 @@ def test_copies_stand_alone(pkg, fmt):
 
 
 @pytest.mark.gpu
+def test_negated_views(pkg):
+    """A view whose elements are stored with the other sign is refused as an operand, and followed as a gradient."""
+    import torch
+    z = torch.randn(64, 64, dtype=torch.complex64, device="cuda")
+    neg, plain = z.conj().imag, -z.imag
+    assert neg.is_neg() and torch.equal(neg, plain)
+    w = torch.ones(64, device="cuda")
+    q = pkg.mx_quantize(plain)
+    for call in [lambda: pkg.mx_quantize(neg), lambda: pkg.mx_quantize_both(neg), lambda: pkg.mx_matmul(q, q, C=neg),
+                 lambda: pkg.mx_rms_norm(neg, w), lambda: pkg.mx_linear(neg, plain),
+                 lambda: pkg.mx_rms_norm(plain, torch._neg_view(w)), lambda: pkg.mx_rms_norm(plain, w, residual=neg),
+                 lambda: pkg.mx_linear(plain, neg)]:
+        with pytest.raises(ValueError):
+            call()
+    x = plain.clone().requires_grad_()
+    y = pkg.mx_linear(x, plain)
+    want, = torch.autograd.grad(y, x, plain, retain_graph=True)
+    got, = torch.autograd.grad(y, x, neg)
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_given_output_and_autograd(pkg):
+    """A C that a backward pass kept counts as changed, one that requires a gradient is refused; so is a dual number."""
+    import torch
+    q = pkg.mx_quantize(torch.ones(8, 64, device="cuda"))
+    q3 = pkg.mx_quantize(torch.ones(1, 8, 64, device="cuda"))
+    ends = torch.tensor([8], dtype=torch.int32, device="cuda")
+    for run in (lambda C: pkg.mx_matmul(q, q, C=C), lambda C: pkg.mx_grouped_matmul(q, q3, ends, C=C)):
+        C = torch.zeros(8, 8, device="cuda")
+        w = torch.ones(8, 8, device="cuda", requires_grad=True)
+        y = (w * C).sum()
+        assert run(C) is C and (C == 64).all()
+        with pytest.raises(RuntimeError):
+            y.backward()
+        with pytest.raises(ValueError):
+            run(w)
+        with torch.no_grad():
+            assert (run(w) == 64).all()
+        with torch.inference_mode():
+            C = torch.zeros(8, 8, device="cuda")
+        assert (run(C) == 64).all()
+    x = torch.ones(8, 64, device="cuda")
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, x)
+        for args in ((dual, x), (x, dual)):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                pkg.mx_linear(*args)
+        assert (pkg.mx_linear(x, x) == 64).all()
+
+
+@pytest.mark.gpu
 def test_empty_operands(pkg):
     import torch
     for shape in ((0, 64), (3, 0, 64), (0, 5, 64)):
