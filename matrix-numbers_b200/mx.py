@@ -111,7 +111,13 @@ def _error_word(device: int):
 def mx_check_errors(device=None) -> None:
     """Raise OzkError if a product launched on ``device`` (default: the current one) gave up a wait since the last
     check; synchronises the device."""
-    device = torch.cuda.current_device() if device is None else torch.device(device).index
+    if device is not None:
+        device = torch.device(device)
+        if device.type != "cuda":
+            raise ValueError(f"{device}: a CUDA device required")
+        device = device.index
+    if device is None:                          # or "cuda", which names the current one
+        device = torch.cuda.current_device()
     w = _error_words.get(device)
     if w is None:
         return

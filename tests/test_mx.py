@@ -903,6 +903,23 @@ def test_given_output_and_autograd(pkg):
 
 
 @pytest.mark.gpu
+def test_error_word(pkg):
+    """A flag in the device's error word is raised once, under every name of the device."""
+    import torch
+    q = pkg.mx_quantize(torch.ones(8, 64, device="cuda"))
+    pkg.mx_matmul(q, q)
+    pkg.mx_check_errors()
+    at = torch.cuda.current_device()
+    for name in (None, "cuda", at, f"cuda:{at}", torch.device("cuda"), torch.device("cuda", at)):
+        pkg.mx._error_words[at].fill_(5)
+        with pytest.raises(pkg._lib.OzkError):
+            pkg.mx_check_errors(name)
+        pkg.mx_check_errors(name)
+    with pytest.raises(ValueError):
+        pkg.mx_check_errors("cpu")
+
+
+@pytest.mark.gpu
 def test_empty_operands(pkg):
     import torch
     for shape in ((0, 64), (3, 0, 64), (0, 5, 64)):
