@@ -11,7 +11,8 @@ namespace {
 // t = x (+ residual), y = t / sqrt(mean(t^2) + eps) weight, y quantised; t, rounded to the type of x, is the next
 // residual.  Everything between the loads and the codes stays in registers: one pass over x and the residual, TPR threads
 // a row with NC chunks of eight values each (longer rows read the rest a second time).  The sums are taken in a fixed
-// order; the inverse root is rounded once, t weight and its product with the root once each.
+// order; the inverse root is rounded once, t times the root (at most sqrt(d), so it never overflows) and its product with
+// the weight once each.
 // Sum over the threads of a row: a warp's in FP32, the warps' in FP64.  `part` is free again after the block's next barrier.
 template <int TPR>
 __device__ __forceinline__ double row_sum(float share, double* part) {
@@ -26,9 +27,13 @@ __device__ __forceinline__ double row_sum(float share, double* part) {
     return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// 1 / sqrt(a) to the nearest FP32 number or its neighbour: FP32's root and one Newton step with an exact residual 1 - a r^2
+// Rows whose sum of squares and eps are beyond FP32 (or NaN) take their squares again of t 2^-70, and are normed as t / 16 and
+// 16 / sqrt(mean t^2 + eps): the root itself would be subnormal for the largest t.
+__device__ __forceinline__ bool beyond_f32(double total, float eps) { return !(total + (double)eps < 3.0e38); }
+
+// 1 / sqrt(a) to the nearest FP32 number or its neighbour, for a below 3e38: FP32's root and one Newton step with an exact
+// residual 1 - a r^2
 __device__ __forceinline__ float inverse_root(double a) {
-    if (!(a < 3.0e38)) return (float)(1.0 / sqrt(a));           // beyond FP32 (or NaN)
     const float ah = (float)a, al = (float)(a - (double)ah);
     const float r = rsqrtf(ah);
     const float q = ah * r, qe = fmaf(ah, r, -q);
@@ -205,18 +210,23 @@ __global__ void __launch_bounds__(TPR, stream_blocks(TPR, NC))
                 }
             }
         }
-        if (SHIFTED && lane == 0) {                             // for the last lane of the warp before
+        auto leave_edges = [&] {                                // for the last lane of the warp before
+            if constexpr (SHIFTED) {
+                if (lane != 0) return;
 #pragma unroll
-            for (int i = 0; i < NC; i++) {
-                const int slot = warp > 0 ? i : i - 1;
-                if (slot < 0) continue;
-                float4* e = reinterpret_cast<float4*>(edge[turn][slot][warp > 0 ? warp : TPR / 32]);
-                e[0] = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
-                e[1] = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
+                for (int i = 0; i < NC; i++) {
+                    const int slot = warp > 0 ? i : i - 1;
+                    if (slot < 0) continue;
+                    float4* e = reinterpret_cast<float4*>(edge[turn][slot][warp > 0 ? warp : TPR / 32]);
+                    e[0] = make_float4(v[i][0], v[i][1], v[i][2], v[i][3]);
+                    e[1] = make_float4(v[i][4], v[i][5], v[i][6], v[i][7]);
+                }
             }
-        }
+        };
+        leave_edges();
         double total = row_sum<TPR>(sq, part[turn]);
-        if (!(total < 3.0e38)) {                                // squares beyond FP32: once more, scaled
+        float rstd;
+        if (beyond_f32(total, eps)) {
             sq = 0.0f;
 #pragma unroll
             for (int i = 0; i < NC; i++)
@@ -224,11 +234,15 @@ __global__ void __launch_bounds__(TPR, stream_blocks(TPR, NC))
                 for (int j = 0; j < 8; j++) {
                     const float u = v[i][j] * 0x1p-70f;
                     sq = fmaf(u, u, sq);
+                    v[i][j] *= 0.0625f;
                 }
+            leave_edges();
             __syncthreads();
             total = row_sum<TPR>(sq, part[turn]) * 0x1p140;
+            rstd = (float)(16.0 / sqrt(total * inv_d + (double)eps));
+        } else {
+            rstd = inverse_root(total * inv_d + (double)eps);
         }
-        const float rstd = inverse_root(total * inv_d + (double)eps);
         if (SHIFTED) {
             auto shift = [&](auto take) {
 #pragma unroll
@@ -250,7 +264,7 @@ __global__ void __launch_bounds__(TPR, stream_blocks(TPR, NC))
 #pragma unroll
         for (int i = 0; i < NC; i++) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * w[i].get(j) * rstd;
+            for (int j = 0; j < 8; j++) v[i][j] = v[i][j] * rstd * w[i].get(j);
             emit_chunk<FMT>(v[i], up, t + i * TPR, t + i * TPR < chunks, cr, tr);
         }
     }
@@ -310,8 +324,18 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / 
     for (int i = 0; i < NC; i++)
         if (t + i * TPR < chunks) fetch(t + i * TPR, v[i]);
     double total = squares([](float x) { return x; }, true);
-    if (!(total < 3.0e38)) total = squares([](float x) { return x * 0x1p-70f; }, false) * 0x1p140;   // beyond FP32: scaled
-    const float rstd = inverse_root(total * inv_d + (double)eps);
+    float rstd, down = 1.0f;
+    if (beyond_f32(total, eps)) {
+        total = squares([](float x) { return x * 0x1p-70f; }, false) * 0x1p140;
+        rstd = (float)(16.0 / sqrt(total * inv_d + (double)eps));
+        down = 0.0625f;
+#pragma unroll
+        for (int i = 0; i < NC; i++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[i][j] *= down;
+    } else {
+        rstd = inverse_root(total * inv_d + (double)eps);
+    }
 
     const long long pitch = code_pitch(FMT, d);
     uint8_t* cr = codes + row * pitch;
@@ -320,7 +344,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / 
         float w[8];
         load8(weight + c * 8, in && aligned && c * 8 + 8 <= d, in ? max(0, d - c * 8) : 0, w);
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = in ? o[j] * w[j] * rstd : 0.0f;
+        for (int j = 0; j < 8; j++) o[j] = in ? o[j] * rstd * w[j] : 0.0f;
         emit_chunk<FMT>(o, up, c, in, cr, tr);
     };
 #pragma unroll
@@ -329,6 +353,8 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / 
         const int c = c0 + t;
         float o[8] = {};
         if (c < chunks) fetch(c, o);
+#pragma unroll
+        for (int j = 0; j < 8; j++) o[j] *= down;
         emit(c, o, c < chunks);
     }
 }

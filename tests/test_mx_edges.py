@@ -1,0 +1,61 @@
+"""The microscaled (MX) operators at the ends of their ranges: values near FP32's largest, long rows, blocks that end inside
+their 32 with a NaN in them, modes of torch in which a call is the first one, waits that run out, and the products' tiles
+over sizes that only one rule reaches.  Definitions in 64 bits: tests/mx_reference.py."""
+import numpy as np
+import pytest
+
+import mx_reference as R
+from test_mx import FMTS, _f64, _norm_want, _put
+
+
+def _near(q, y, fmt):
+    """The operand's numbers against the 64-bit norm y: the code of y or, where y is within the kernel's error of a rounding
+    border, its neighbour; any scale where the block's largest value is that near to a border between scales.  The error: a
+    thread adds at most max(32, d / 1024) squares one after another, and ten levels join the threads' sums, each step off
+    by half a step of FP32 (2^-24 of the sum); a root halves that; then the root itself (one step at most), its product with
+    the value and the one with the weight, half a step each: 4 half steps in all, and one to spare.  Below FP32's normal numbers
+    y is off by 2^-149, which no grid here sees: the finest has steps of 2^-136."""
+    band = ((max(32, y.shape[-1] / 1024) + 10) / 2 + 5) * 2.0 ** -24
+    got = q.dequantize(__import__("torch").float32).double().cpu().numpy()
+    codes, scales = R.quantize(y, fmt)
+    off = q.scales().cpu().numpy().astype(int) != scales
+    top = np.abs(R.blocks(y)).max(-1)
+    frac = np.frexp(np.where(top == 0, 1.0, top))[0] * 2
+    assert not (off & ~(np.minimum(np.abs(frac - 1), np.abs(frac - 2)) < 2 * band)).any()
+    ok = (got == R.rounded(y, fmt)) | (got == R.rounded(y * (1 - band), fmt)) | (got == R.rounded(y * (1 + band), fmt))
+    ok |= np.repeat(off, 32, -1)[..., :y.shape[-1]]
+    assert ok.all(), (int((~ok).sum()), got[~ok][:4], y[~ok][:4])
+
+
+# ---- norm: the whole range of FP32 ---------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [6, 600])
+@pytest.mark.parametrize("name", ["float32", "bfloat16"])
+def test_norm_of_the_largest_values(pkg, rows, name):
+    """t weight is beyond FP32 and y is not: rows of the largest values, uneven ones, ones with small values beside them,
+    in the kernels for few and for many rows."""
+    rng = np.random.default_rng(41)
+    for d in (96, 777, 1024, 4096):
+        x = rng.standard_normal((rows, d))
+        x[0] = 3e38
+        x[1] *= 6e37
+        x[2] = 1e-6
+        x[2, :8] = 3e38
+        x[3] *= 1e20
+        x, w = _put(x, name), _put(1.5 + 0.1 * rng.standard_normal(d), "float32")
+        keep = [0, 1, 2, 3, 4, rows - 1]
+        _, y = _norm_want(_f64(x[keep]), _f64(w), None, 1e-6)
+        for fmt in FMTS:
+            q, _ = pkg.mx_rms_norm(x, w, fmt=fmt)
+            _near(pkg.MXMatrix.from_codes(q.codes()[keep].contiguous(), q.scales()[keep].contiguous(), fmt, d), y, fmt)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [3, 600])
+def test_norm_of_a_large_gain(pkg, rows):
+    """The gain may be as large as its product with a normed value allows."""
+    rng = np.random.default_rng(42)
+    x, w = _put(rng.standard_normal((rows, 300)) * 1e18, "float32"), _put(rng.uniform(1e24, 1e25, 300), "float32")
+    q, _ = pkg.mx_rms_norm(x, w)
+    y = _norm_want(_f64(x), _f64(w), None, 1e-6)[1]
+    _near(q, y, "e4m3")
