@@ -27,8 +27,9 @@ __device__ __forceinline__ double row_sum(float share, double* part) {
     return __shfl_sync(0xffffffffu, v, 0);
 }
 
-// Rows whose sum of squares and eps are beyond FP32 (or NaN) take their squares again of t 2^-70, and are normed as t / 16 and
-// 16 / sqrt(mean t^2 + eps): the root itself would be subnormal for the largest t.
+// Rows whose sum of squares and eps are beyond FP32 (or NaN) take their squares again of t 2^-80 (a warp adds up to 2^23 of
+// them, each up to 2^96), and are normed as t / 16 and 16 / sqrt(mean t^2 + eps): the root itself would be subnormal for the
+// largest t.
 __device__ __forceinline__ bool beyond_f32(double total, float eps) { return !(total + (double)eps < 3.0e38); }
 
 // 1 / sqrt(a) to the nearest FP32 number or its neighbour, for a below 3e38: FP32's root and one Newton step with an exact
@@ -232,13 +233,13 @@ __global__ void __launch_bounds__(TPR, stream_blocks(TPR, NC))
             for (int i = 0; i < NC; i++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float u = v[i][j] * 0x1p-70f;
+                    const float u = v[i][j] * 0x1p-80f;
                     sq = fmaf(u, u, sq);
                     v[i][j] *= 0.0625f;
                 }
             leave_edges();
             __syncthreads();
-            total = row_sum<TPR>(sq, part[turn]) * 0x1p140;
+            total = row_sum<TPR>(sq, part[turn]) * 0x1p160;
             rstd = (float)(16.0 / sqrt(total * inv_d + (double)eps));
         } else {
             rstd = inverse_root(total * inv_d + (double)eps);
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, TPR == 32 ? 6 : 1024 / 
     double total = squares([](float x) { return x; }, true);
     float rstd, down = 1.0f;
     if (beyond_f32(total, eps)) {
-        total = squares([](float x) { return x * 0x1p-70f; }, false) * 0x1p140;
+        total = squares([](float x) { return x * 0x1p-80f; }, false) * 0x1p160;
         rstd = (float)(16.0 / sqrt(total * inv_d + (double)eps));
         down = 0.0625f;
 #pragma unroll

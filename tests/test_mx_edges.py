@@ -59,3 +59,16 @@ def test_norm_of_a_large_gain(pkg, rows):
     q, _ = pkg.mx_rms_norm(x, w)
     y = _norm_want(_f64(x), _f64(w), None, 1e-6)[1]
     _near(q, y, "e4m3")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [2 ** 17, 2 ** 18 + 5, 2 ** 21])
+def test_norm_of_long_rows_of_the_largest_values(pkg, d):
+    """However many squares beyond FP32 a row adds."""
+    import torch
+    rng = np.random.default_rng(43)
+    x = torch.full((2, d), 3.3e38, device="cuda")
+    x[1, ::3] = -1e37
+    w = _put(1.3 + 0.1 * rng.standard_normal(d), "float32")
+    q, _ = pkg.mx_rms_norm(x, w)
+    _near(q, _norm_want(_f64(x), _f64(w), None, 1e-6)[1], "e4m3")
