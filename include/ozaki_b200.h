@@ -229,8 +229,9 @@ int ozk_rule_certified(const double* nA, const double* nB, const int32_t* flag, 
  * number is code x 2^(s - 127): an element of 4 bits (e2m1) or 8 bits (e4m3) and one scale byte s (e8m0; 255 = NaN)
  * for each block of 32 along the contracted axis.  An operand is `groups` x `rows` vectors of length k, laid out for
  * the tensor cores (ozk_mx_code_bytes / ozk_mx_scale_bytes; both buffers 16-byte aligned, codes 32-byte):
- *   codes:  [group][row][kp], kp = k rounded up to 128, zero from k to kp; e2m1 holds two codes a byte, the even one
- *           in the lower half;
+ *   codes:  [group][row][kp], kp = k rounded up to 128, zero from k to kp (but unspecified in the rest of a block with
+ *           the NaN scale, and behind a row of NaN that the norm wrote, whose scales behind k are unspecified too); e2m1
+ *           holds two codes a byte, the even one in the lower half;
  *   scales: [group][ceil(rows / 128)][kp / 128][512]; row r and block b of a 128 x 128 tile at 16 (r % 32) +
  *           4 (r / 32) + b.
  * No shape rule: any rows, k from 1 up to the limits below.  dtype: OZK_F32, OZK_F16 or OZK_BF16.                                      */

@@ -4,7 +4,8 @@
 // for each block of 32 along the contracted axis.  An operand of `rows` vectors of length k (times `groups`, for
 // experts) is laid out once for the tensor cores:
 //   codes   [group][row][kp] with kp = k rounded up to 128, contiguous along k (e2m1: two codes a byte, the even one
-//           in the lower half); the codes from k to kp are zero.  One TMA box row is 128 bytes.
+//           in the lower half); the codes from k to kp are zero, but for those behind NaN (a block with the NaN scale
+//           ends with its 32 codes, a row of NaN from the norm with kp), which nothing reads.  One TMA box row is 128 bytes.
 //   scales  [group][row tile of 128][k tile of 128][512]: the byte of row r and block b of a tile sits at
 //           16 (r % 32) + 4 (r / 32) + b, which is what one tcgen05.cp 32x128b.warpx4 lays into TMEM as the scales of
 //           128 rows; a k step of the product reads its scales as one contiguous copy per row tile.

@@ -205,10 +205,14 @@ class MXMatrix:
 
     def codes(self):
         """The element codes as uint8 (..., rows, ceil(k / 2)) for e2m1 (two a byte, the even one in the lower half)
-        or (..., rows, k) for e4m3: a copy in the order in which checkpoints store them."""
+        or (..., rows, k) for e4m3: a copy in the order in which checkpoints store them.  The half of a byte behind an odd
+        number of 4-bit codes is zero."""
         per = (self.k + 1) // 2 if self._fmt == 0 else self.k
         pitch = _padded(self.k) // (2 if self._fmt == 0 else 1)
-        c = self._buffer[:self._code_bytes].view(self._g, self.rows, pitch)[..., :per].contiguous()
+        c = self._buffer[:self._code_bytes].view(self._g, self.rows, pitch)[..., :per].clone(
+            memory_format=torch.contiguous_format)
+        if self._fmt == 0 and self.k % 2:
+            c[..., -1] &= 15                    # a block with the NaN scale has codes behind its end too
         return c if self.groups is not None else c[0]
 
     def scales(self):

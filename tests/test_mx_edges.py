@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import mx_reference as R
-from test_mx import FMTS, _f64, _norm_want, _put
+from test_mx import FMTS, _f64, _norm_want, _put, _same
 
 
 def _near(q, y, fmt):
@@ -72,3 +72,44 @@ def test_norm_of_long_rows_of_the_largest_values(pkg, d):
     w = _put(1.3 + 0.1 * rng.standard_normal(d), "float32")
     q, _ = pkg.mx_rms_norm(x, w)
     _near(q, _norm_want(_f64(x), _f64(w), None, 1e-6)[1], "e4m3")
+
+
+# ---- blocks that end inside their 32 -------------------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("fmt", FMTS)
+@pytest.mark.parametrize("name", ["float32", "float16", "bfloat16"])
+def test_codes_of_bad_blocks_end_with_the_vector(pkg, fmt, name):
+    """A NaN or an infinite value in the last block: the stored codes are the definition's, with nothing in the half of a
+    byte behind an odd length, and the same after a round trip; rows, columns and both, aligned or not, in groups."""
+    import torch
+    rng = np.random.default_rng(44)
+    for k in (1, 31, 33, 97, 200):
+        for bad in (np.nan, np.inf):
+            x = rng.standard_normal((5, k + 3))
+            x[1, k - 1] = bad
+            x[3, 0] = -bad
+            t = _put(x, name)[:, :k]
+            down = _put(x.T, name)[:k]
+            for q in (pkg.mx_quantize(t, fmt), pkg.mx_quantize(down, fmt, axis=0), pkg.mx_quantize(t.contiguous(), fmt),
+                      pkg.mx_quantize(down.T.contiguous().T, fmt, axis=0), pkg.mx_quantize_both(t, fmt)[0],
+                      pkg.mx_quantize_both(down, fmt)[1], pkg.mx_quantize_both(down.T.contiguous().T, fmt)[1]):
+                _same(q, _f64(t), fmt, "floor")
+                back = pkg.MXMatrix.from_codes(q.codes(), q.scales(), fmt, k)
+                assert torch.equal(back.codes(), q.codes())
+                one, w = pkg.mx_quantize(torch.ones(2, k, device="cuda"), fmt), q.dequantize(torch.float32)
+                assert torch.equal(pkg.mx_matmul(q, one)[:, 0].isnan(), w.isnan().any(1))
+            _same(pkg.mx_quantize(t.expand(2, 5, k), fmt), np.stack([_f64(t)] * 2), fmt, "floor")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [4, 700])
+def test_codes_of_a_bad_row_of_the_norm(pkg, rows):
+    import torch
+    for d in (33, 777):
+        x = torch.ones(rows, d, device="cuda")
+        x[1, 3] = float("nan")
+        q, _ = pkg.mx_rms_norm(x, torch.ones(d, device="cuda"), fmt="e2m1")
+        assert (q.scales()[1] == 255).all() and (q.codes()[1, :-1] == 0x77).all() and (q.codes()[1, -1] == 7).all()
+        assert torch.equal(pkg.MXMatrix.from_codes(q.codes(), q.scales(), "e2m1", d).codes(), q.codes())
+        w = pkg.mx_quantize(torch.ones(3, d, device="cuda"))
+        assert pkg.mx_matmul(q, w).isnan().all(1).nonzero().flatten().tolist() == [1]
