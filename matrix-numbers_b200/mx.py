@@ -102,7 +102,10 @@ def _error_word(device: int):
         with _error_lock:
             w = _error_words.get(device)
             if w is None:
-                w = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+                with torch.inference_mode(False):    # mx_check_errors clears it in whatever mode it is called
+                    w = torch.zeros(1, dtype=torch.int32, device=f"cuda:{device}")
+                if type(w) is not _Tensor or not w.data_ptr():      # a tracer's stand-in, which has no memory
+                    raise OzkError("the first MX product on a device allocates its error word: make one call before tracing")
                 torch.cuda.synchronize(device)       # products on any stream may use it from here on
                 _error_words[device] = w
     return w.data_ptr()

@@ -113,3 +113,74 @@ def test_codes_of_a_bad_row_of_the_norm(pkg, rows):
         assert torch.equal(pkg.MXMatrix.from_codes(q.codes(), q.scales(), "e2m1", d).codes(), q.codes())
         w = pkg.mx_quantize(torch.ones(3, d, device="cuda"))
         assert pkg.mx_matmul(q, w).isnan().all(1).nonzero().flatten().tolist() == [1]
+
+
+# ---- the first product on a device ---------------------------------------------------------------------------------------
+@pytest.fixture
+def no_word(pkg):
+    """The state before the first product on the device."""
+    import torch
+    torch.cuda.synchronize()
+    at = torch.cuda.current_device()
+    kept = pkg.mx._error_words.pop(at, None)
+    yield at
+    torch.cuda.synchronize()
+    if kept is not None:
+        pkg.mx._error_words[at] = kept
+
+
+def _word_works(pkg, at, q):
+    import torch
+    assert (pkg.mx_matmul(q, q, dtype=torch.float32) == 64).all()
+    for mode in (torch.no_grad, torch.inference_mode, torch.enable_grad):
+        with mode():
+            pkg.mx._error_words[at].add_(4)
+        with pytest.raises(pkg._lib.OzkError):
+            pkg.mx_check_errors()
+        pkg.mx_check_errors()
+
+
+@pytest.mark.gpu
+def test_first_product_in_inference_mode(pkg, no_word):
+    """The error word that it allocates can be read and cleared in any mode."""
+    import torch
+    q = pkg.mx_quantize(torch.ones(8, 64, device="cuda"))
+    with torch.inference_mode():
+        assert (pkg.mx_matmul(q, q) == 64).all()
+    pkg.mx._error_words[no_word].add_(4)
+    with pytest.raises(pkg._lib.OzkError):
+        pkg.mx_check_errors()
+    _word_works(pkg, no_word, q)
+
+
+@pytest.mark.gpu
+def test_first_product_under_a_tracer(pkg, no_word):
+    """Tensors without memory are refused, and nothing of them is kept."""
+    import torch
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    q = pkg.mx_quantize(torch.ones(8, 64, device="cuda"))
+    with FakeTensorMode(allow_non_fake_inputs=True):
+        C = torch.empty(8, 8, device="cuda")
+        for call in (lambda: pkg.mx_matmul(q, q), lambda: pkg.mx_matmul(q, q, C=C)):
+            with pytest.raises((pkg._lib.OzkError, RuntimeError)):
+                call()
+    _word_works(pkg, no_word, q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("transform", ["grad", "vmap", "device"])
+def test_first_product_under_a_transform(pkg, no_word, transform):
+    import torch
+    q = pkg.mx_quantize(torch.ones(8, 64, device="cuda"))
+    def f(x):
+        return x + pkg.mx_matmul(q, q, C=C).sum()
+    C = torch.empty(8, 8, device="cuda")
+    try:
+        if transform == "device":
+            with torch.device("cpu"):
+                f(torch.ones(3, device="cuda"))
+        else:
+            getattr(torch.func, transform)(lambda x: f(x).sum())(torch.ones(3, device="cuda"))
+    except (RuntimeError, ValueError, pkg._lib.OzkError):
+        pass                                                     # refused is fine; what counts is what is left behind
+    _word_works(pkg, no_word, q)
