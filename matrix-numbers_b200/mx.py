@@ -15,7 +15,8 @@ everything it touches is NaN).  Any sizes; the operands are laid out for the ten
 
 All calls are enqueued on the current stream of the operand's device and may be captured in a CUDA graph (after one
 eager product on that device).  A product whose bounded waits ran out leaves a flag that ``mx_check_errors`` raises.
-Only ``mx_linear`` has gradients; the other results carry none, whatever their inputs require.
+Only ``mx_linear`` has gradients: ``mx_rms_norm`` refuses inputs that require one (under ``torch.no_grad()`` it takes
+them), and an ``MXMatrix`` is not a tensor and carries none.
 """
 from __future__ import annotations
 
@@ -420,7 +421,8 @@ def mx_grouped_matmul(A, B, ends, C=None, dtype=torch.bfloat16):
 def mx_rms_norm(x, weight, residual=None, eps=1e-6, fmt="e4m3", rule="floor"):
     """Root-mean-square norm into an MX operand: t = x + residual, y = t / sqrt(mean(t^2) + eps) * weight over the last
     axis, in FP32 from the loads to the codes.  Returns (y as MXMatrix (rows, d) with the leading axes of x as rows, t
-    rounded to the type of x and in its shape, or None without a residual)."""
+    rounded to the type of x and in its shape, or None without a residual).  It has no gradient: inputs that require one
+    are refused while gradients are recorded."""
     d = _tensor(x, "x")
     code, up = _format(fmt), _rule(rule)
     shape = x.shape
@@ -437,6 +439,12 @@ def mx_rms_norm(x, weight, residual=None, eps=1e-6, fmt="e4m3", rule="floor"):
     if residual is not None and (not isinstance(residual, _Tensor) or residual.shape != shape
                                  or residual.dtype is not dtype or residual.get_device() != device or residual.is_neg()):
         raise ValueError("residual: a tensor of x's shape, type and device required")
+    if (x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad) \
+            and torch.is_grad_enabled():        # it would be lost without a word
+        raise ValueError("mx_rms_norm has no gradient, and an input requires one (see torch.no_grad, torch.Tensor.detach)")
+    if _forward_ad._current_level >= 0 and any(t is not None and _forward_ad.unpack_dual(t).tangent is not None
+                                               for t in (x, weight, residual)):
+        raise ValueError("mx_rms_norm has no forward-mode derivative, and an input has a tangent")
     if _current_device() != device:
         with torch.cuda.device(device):
             return mx_rms_norm(x, weight, residual, eps, fmt, rule)

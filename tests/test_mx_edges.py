@@ -184,3 +184,31 @@ def test_first_product_under_a_transform(pkg, no_word, transform):
     except (RuntimeError, ValueError, pkg._lib.OzkError):
         pass                                                     # refused is fine; what counts is what is left behind
     _word_works(pkg, no_word, q)
+
+
+# ---- gradients that there are not ----------------------------------------------------------------------------------------
+@pytest.mark.gpu
+def test_norm_refuses_what_would_lose_a_gradient(pkg):
+    """An input that requires a gradient is refused while gradients are recorded, and so is a dual number; without them the
+    call is the plain one."""
+    import torch
+    x, r, w = (torch.randn(8, 64, device="cuda"), torch.randn(8, 64, device="cuda"), torch.ones(64, device="cuda"))
+    q, t = pkg.mx_rms_norm(x, w, residual=r)
+    for at in range(3):
+        args = [a.clone().requires_grad_(i == at) for i, a in enumerate((x, w, r))]
+        with pytest.raises(ValueError, match="gradient"):
+            pkg.mx_rms_norm(args[0], args[1], residual=args[2])
+        if at < 2:
+            with pytest.raises(ValueError, match="gradient"):
+                pkg.mx_rms_norm(args[0], args[1])
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode():
+                q1, t1 = pkg.mx_rms_norm(args[0], args[1], residual=args[2])
+            assert torch.equal(t1, t) and torch.equal(q1.codes(), q.codes()) and torch.equal(q1.scales(), q.scales())
+            assert not t1.requires_grad
+    with torch.autograd.forward_ad.dual_level():
+        for at in range(3):
+            args = [torch.autograd.forward_ad.make_dual(a, a) if i == at else a for i, a in enumerate((x, w, r))]
+            with pytest.raises(ValueError, match="tangent"):
+                pkg.mx_rms_norm(args[0], args[1], residual=args[2])
+        assert torch.equal(pkg.mx_rms_norm(x, w, residual=r)[1], t)
