@@ -266,6 +266,13 @@ int ozk_mx_dequantize(const uint8_t* codes, const uint8_t* scales, int fmt, int 
 int ozk_mx_gemm(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
                 const uint8_t* B_scales, int B_fmt, int m, int n, int k, void* C, int64_t ldc, int dtype, int32_t* err,
                 ozk_stream_t stream);
+/* Self-test of the products' failure path: ozk_mx_gemm with limit_ns (100 ns .. 4 s of wall time) for every wait of the
+ * kernel's roles and, with `hold` non-zero, 16 bytes more expected of every stage than its loads bring, so that no stage is
+ * ever full.  A role whose wait runs out ORs its OZK_DEVERR_TIMEOUT_* flag into *err; the others leave, and the kernel waits
+ * (up to 1 s each) for the loads and MMAs in flight, frees its TMEM and returns.  C is valid if *err stays 0.   */
+int ozk_mx_wait_selftest(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
+                         const uint8_t* B_scales, int B_fmt, int m, int n, int k, void* C, int64_t ldc, int dtype,
+                         int64_t limit_ns, int hold, int32_t* err, ozk_stream_t stream);
 /* The product grouped by expert: rows [ends[g - 1], ends[g]) of A (from 0 for g = 0) are multiplied with group g of
  * B (groups x n x k).  ends[groups]: device int32, ascending; a value below its predecessor or above `rows` is read as
  * the nearest one in order.  Rows from the last end on are set to zero when `fill` is non-zero and left alone

@@ -66,6 +66,7 @@ _SIGNATURES = {
     "ozk_mx_linear_backward": ([P, I32, I64, I64, P, P, I32, I32, I32, I32, I32, P, P, P, I32, P, I32, P, P], I32),
     "ozk_mx_dequantize": ([P, P, I32, I32, I32, I32, P, I32, P], I32),
     "ozk_mx_gemm": ([P, P, I32, P, P, I32, I32, I32, I32, P, I64, I32, P, P], I32),
+    "ozk_mx_wait_selftest": ([P, P, I32, P, P, I32, I32, I32, I32, P, I64, I32, I64, I32, P, P], I32),
     "ozk_mx_grouped_gemm": ([P, P, I32, P, P, I32, I32, I32, I32, I32, P, I32, P, I64, I32, P, P], I32),
     "ozk_mx_rms_norm": ([P, P, P, I32, I32, I32, I32, I64, I64, F32, I32, I32, P, P, P, P], I32),
     "ozk_core": ([P, P, P, P, P, P, I32, I32, I32, I32, I32, P, P, P, P, P, P], I32),

@@ -28,8 +28,9 @@
 // kernel (8192 x 4096 x 8192 in e2m1: 163 us, tensor pipe 41 % active; elected: 99 us, 75 %).
 // Measured on one B200 at its power cap (1.4 - 1.5 GHz): e2m1 16384 x 8192 x 8192 in 394 us, 5.6 PFLOP/s; e4m3 8192 x 8192 x
 // 8192 in 396 us, 2.8 PFLOP/s: four and two times the rate that the card sustains in bf16, and bound by the same cap.
-// Every mbarrier wait is bounded; on a timeout the CTA records a flag in *err, stops, waits (bounded) for its own copies
-// and MMAs in flight, frees TMEM and exits.  No multicast is used.
+// Every mbarrier wait is bounded; when a role's wait runs out it records a flag in *err and raises the CTA's abort flag (both
+// CTAs' of a pair), through which the other roles leave.  When all have, whichever it was, the CTA waits (bounded) for its
+// loads and MMAs in flight, frees TMEM and exits.  No multicast is used.
 #include <cuda.h>
 
 #include <atomic>
@@ -49,6 +50,7 @@ constexpr uint32_t OUT_WARP_BYTES = 32 * 128;   // one epilogue warp's 32 rows o
 constexpr int THREADS = (2 + EPI_WARPS) * 32;
 constexpr int GROUP_L = 16;                  // left tiles per raster group
 constexpr uint64_t WAIT_LIMIT_NS = 4000000000ull;   // 4 s of wall time per wait
+constexpr uint64_t DRAIN_LIMIT_NS = 1000000000ull;  // 1 s for each load, and for the MMAs, that were in flight at a timeout
 constexpr int MXF4 = 0, MXF8F6F4 = 1;
 constexpr size_t SMEM_MAX = 232448;
 constexpr size_t TABLE_BYTES = (2 * (OZK_MX_MAX_GROUPS + 1) * 4 + 15) / 16 * 16;
@@ -101,6 +103,7 @@ struct Args {
     bool vec;                                // rows of C are 16-byte aligned, and tmC describes it
     uint32_t idesc;
     int32_t* err;
+    uint64_t limit_ns;                       // of every wait of the roles
 };
 
 struct Unit {
@@ -150,11 +153,6 @@ struct Work {
         return w;
     }
 };
-
-__device__ __forceinline__ void raise_abort(volatile int* abort_flag, int32_t* err, int code) {
-    *abort_flag = 1;
-    atomicOr(err, code);
-}
 
 __device__ __forceinline__ uint32_t pack2(float a, float b, int dtype) {
     if (dtype == OZK_BF16) {
@@ -349,6 +347,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(sSR + STAGES * S::SR_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::NUM_BARS);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile long long* peer_issued = reinterpret_cast<volatile long long*>(tmem_slot + 2);   // loads that CTA 1 of a pair issued
     int* pre = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(bars) + 256);
     int* bound = pre + OZK_MX_MAX_GROUPS + 1;
 
@@ -368,6 +367,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int b = 0; b < 2; b++) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), S::CTAS * EPI_WARPS); }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
+        if (PAIR) *peer_issued = 0;
         mbar_fence_init();
         tma_prefetch_desc(&tmL);
         tma_prefetch_desc(&tmR);
@@ -398,13 +398,27 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int rank = PAIR ? uniform((int)cluster_ctarank()) : 0;
     const int part = !PAIR && parts > 1 ? uniform((int)cluster_ctarank()) : 0;
     const long long u0 = blockIdx.x / (parts * S::CTAS), du = gridDim.x / (parts * S::CTAS);
+    auto give_up = [&](int code) {             // one lane of a role whose wait ran out
+        if (*abort_flag) return;               // it left through the flag: another role has reported
+        *abort_flag = 1;
+        if (PAIR) st_cluster_u32(map_to_rank(smem_addr(const_cast<const int*>(abort_flag)), (uint32_t)(rank ^ 1)), 1u);
+        atomicOr(a.err, code);
+    };
+    auto commit = [&](uint32_t bar) {          // an arrival on that barrier of every CTA when all issued so far is done
+        if (PAIR) {
+            umma_commit_pair(map_to_rank(bar, 0u));
+            umma_commit_pair(map_to_rank(bar, 1u));
+        } else {
+            umma_commit(bar);
+        }
+    };
+    long long issued = 0;                      // loads, by the producer
     const int kb0 = (int)((long long)a.kblocks * part / parts), kb1 = (int)((long long)a.kblocks * (part + 1) / parts);
 
     if (warp == 0) {
         // ---------------------------------------------------------------- producer (the whole warp; one lane issues)
         int stage = 0;
         uint32_t phase = 0;
-        long long issued = 0;
         bool ok = true;
         const uint32_t aL = smem_addr(sL), aR = smem_addr(sR), aSL = smem_addr(sSL), aSR = smem_addr(sSR);
         for (long long u = u0; ok && u < work.units; u += du) {
@@ -412,7 +426,7 @@ __global__ void __launch_bounds__(THREADS, 1)
             const int l0 = uniform(w.l0) + rank * BM, rt = uniform(w.r0), r0 = rt + rank * S::RN;
             const int rg = uniform(w.rg);
             for (int kb = kb0; kb < kb1; kb++) {
-                ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS);
+                ok = mbar_wait_warp(empty_bar(stage), phase ^ 1u, abort_flag, a.limit_ns);
                 if (!ok) break;
                 if (elect_one()) {
                     // a pair's loads all complete on CTA 0's barrier, which expects the bytes of both
@@ -438,17 +452,9 @@ __global__ void __launch_bounds__(THREADS, 1)
                 if (++stage == STAGES) { stage = 0; phase ^= 1u; }
             }
         }
-        if (!ok) {
-            if (lane == 0 && !*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_PRODUCER);
-            if (rank == 0) {
-                // let the loads already issued land before the CTA (or the pair) exits (bounded)
-                const long long first = issued > STAGES ? issued - STAGES : 0;
-                for (long long j = first; j < issued; j++) {
-                    int dummy = 0;
-                    mbar_wait_bounded(full_bar((int)(j % STAGES)), (uint32_t)((j / STAGES) & 1), &dummy, WAIT_LIMIT_NS);
-                }
-            }
-        }
+        if (!ok && lane == 0) give_up(OZK_DEVERR_TIMEOUT_PRODUCER);
+        if (PAIR && rank == 1 && lane == 0)
+            st_cluster_u64(map_to_rank(smem_addr(const_cast<const long long*>(peer_issued)), 0u), (uint64_t)issued);
     } else if (warp == 1) {
         if (rank == 0) {
             // ------------------------------------------------------------ scales to TMEM, MMAs (the whole warp; one lane issues)
@@ -459,20 +465,12 @@ __global__ void __launch_bounds__(THREADS, 1)
             // descriptors: the address part advances with the stage, the rest is constant
             const uint64_t dL = umma_desc_sw128(smem_addr(sL)), dR = umma_desc_sw128(smem_addr(sR));
             const uint64_t dSL = smem_desc_scales(smem_addr(sSL)), dSR = smem_desc_scales(smem_addr(sSR));
-            auto commit = [&](uint32_t bar) {      // an arrival on that barrier of every CTA when all issued so far is done
-                if (PAIR) {
-                    umma_commit_pair(map_to_rank(bar, 0u));
-                    umma_commit_pair(map_to_rank(bar, 1u));
-                } else {
-                    umma_commit(bar);
-                }
-            };
             for (long long u = u0; ok && u < work.units; u += du) {
                 const int b = (int)(it & 1u);
                 if (it >= (uint32_t)S::LAG) {
                     const uint32_t bar = S::LAG == 1 ? acce_bar(0) : acce_bar(b);
                     const uint32_t par = S::LAG == 1 ? (it - 1u) & 1u : ((it >> 1) - 1u) & 1u;
-                    ok = mbar_wait_warp(bar, par, abort_flag, WAIT_LIMIT_NS);
+                    ok = mbar_wait_warp(bar, par, abort_flag, a.limit_ns);
                     if (!ok) break;
                     tc_fence_after();
                 }
@@ -499,7 +497,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     commit(empty_bar(sg));
                 };
                 for (int kb = kb0; kb < kb1; kb++) {
-                    ok = mbar_wait_warp(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS);
+                    ok = mbar_wait_warp(full_bar(stage), phase, abort_flag, a.limit_ns);
                     if (!ok) break;
                     tc_fence_after();
                     if (elect_one()) {
@@ -532,19 +530,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 __syncwarp();
                 it++;
             }
-            if (!ok) {
-                if (lane == 0 && !*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_MMA);
-                if (step > 0) {
-                    // all that this warp issued must finish before TMEM is released
-                    if (elect_one()) {
-                        if (PAIR) umma_commit_pair(map_to_rank(drain_bar, 0u));
-                        else umma_commit(drain_bar);
-                    }
-                    __syncwarp();
-                    int dummy = 0;
-                    mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
-                }
-            }
+            if (!ok && lane == 0) give_up(OZK_DEVERR_TIMEOUT_MMA);
         }
     } else {
         // ---------------------------------------------------------------- epilogue warps
@@ -561,8 +547,8 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (long long u = u0; ok && u < work.units; u += du) {
             const Unit w = work.at(u);
             const int b = (int)(it & 1u);
-            if (!mbar_wait_warp(accf_bar(b), (it >> 1) & 1u, abort_flag, WAIT_LIMIT_NS)) {
-                if (lane == 0 && !*abort_flag) raise_abort(abort_flag, a.err, OZK_DEVERR_TIMEOUT_EPILOGUE);
+            if (!mbar_wait_warp(accf_bar(b), (it >> 1) & 1u, abort_flag, a.limit_ns)) {
+                if (lane == 0) give_up(OZK_DEVERR_TIMEOUT_EPILOGUE);
                 ok = false;
                 break;
             }
@@ -678,6 +664,35 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (__builtin_expect(*abort_flag, 0)) {
+        // All roles of the CTA (of the pair) have left, by a wait that ran out or at their end.  What they issued still writes
+        // shared memory, TMEM and barriers, so it has to land before those are given up.
+        int none = 0;
+        if (warp == 0 && rank == 0) {
+            // The last loads of the ring, on CTA 0's barriers.  Those that only CTA 1 of a pair issued are expected now, those
+            // that were expected of it and never issued count as arrived: neither is more than a ring ahead of the MMAs,
+            // so a slot's earlier loads have been waited for.
+            const long long other = PAIR ? *peer_issued : issued, most = issued > other ? issued : other;
+            for (long long j = most > STAGES ? most - STAGES : 0; j < most; j++) {
+                const uint32_t bar = full_bar((int)(j % STAGES));
+                if (PAIR && lane == 0) {
+                    if (j >= issued) mbar_arrive_expect_tx(bar, a.load_bytes);
+                    else if (j >= other) mbar_complete_tx(bar, a.load_bytes);
+                }
+                __syncwarp();
+                mbar_wait_bounded(bar, (uint32_t)((j / STAGES) & 1), &none, DRAIN_LIMIT_NS);
+            }
+        } else if (warp == 1) {
+            if (rank == 0 && elect_one()) commit(drain_bar);
+            __syncwarp();
+            mbar_wait_bounded(drain_bar, 0u, &none, DRAIN_LIMIT_NS);
+        }
+        __syncwarp();
+        if (PAIR) cluster_sync();
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    }
     if (warp == 1) {
         __syncwarp();
         if (PAIR) tmem_dealloc_pair(tmem_base, S::TMEM_COLS);
@@ -776,6 +791,7 @@ struct Call {
     Args args;
     cudaStream_t st;
     int dev, sms;
+    bool hold;                               // self-test: expect more of every stage than its loads bring
 };
 
 uint32_t format_bits(int kind, int fmt) { return kind == MXF4 ? 1u : fmt == OZK_MX_E2M1 ? 5u : 0u; }
@@ -791,7 +807,8 @@ int launch(const Call& c, int parts) {
     a.ktiles = padded_k(c.k) / TILE;
     a.kblocks = (a.ktiles + S::KT - 1) / S::KT;
     // a load that spreads 4-bit codes counts the bytes it reads, not the bytes it fills
-    a.load_bytes = S::L_BYTES / (spreads(L, KIND) ? 2u : 1u) + S::R_BYTES / (spreads(R, KIND) ? 2u : 1u) + S::SL_BYTES + S::SR_BYTES;
+    a.load_bytes = S::L_BYTES / (spreads(L, KIND) ? 2u : 1u) + S::R_BYTES / (spreads(R, KIND) ? 2u : 1u) + S::SL_BYTES + S::SR_BYTES +
+                   (c.hold ? 16u : 0u);
     a.idesc = umma_idesc_mx(format_bits(KIND, L.fmt), format_bits(KIND, R.fmt), S::BL, BN);
     CUtensorMap tl, tr, tsl, tsr, tc = {};
     int rc;
@@ -876,7 +893,8 @@ int choose(const Call& c) {
 }
 
 int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const uint8_t* Bs, int Bf, int m, int n, int k,
-        int groups, const int32_t* ends, int fill, void* C, int64_t ldc, int dtype, int32_t* err, ozk_stream_t stream) {
+        int groups, const int32_t* ends, int fill, void* C, int64_t ldc, int dtype, int32_t* err, ozk_stream_t stream,
+        uint64_t limit_ns = WAIT_LIMIT_NS, bool hold = false) {
     if (!Ac || !As || !Bc || !Bs || !C || !err || !fmt_ok(Af) || !fmt_ok(Bf)) return OZK_ERR_ARG;
     if (m < 1 || n < 1 || m > OZK_MX_ROWS_MAX || n > OZK_MX_ROWS_MAX || k < 1 || k > OZK_MX_KMAX || ldc < n) return OZK_ERR_ARG;
     if (!dtype_ok(dtype)) return OZK_ERR_ARG;
@@ -893,6 +911,7 @@ int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const u
     c.k = k;
     c.kind = Af == OZK_MX_E2M1 && Bf == OZK_MX_E2M1 ? MXF4 : MXF8F6F4;
     c.st = reinterpret_cast<cudaStream_t>(stream);
+    c.hold = hold;
     Args& a = c.args;
     a = Args{};
     a.groups = groups;
@@ -906,6 +925,7 @@ int run(const uint8_t* Ac, const uint8_t* As, int Af, const uint8_t* Bc, const u
     // (a tensor map's stride ends at 2^40 bytes)
     a.vec = (reinterpret_cast<uintptr_t>(C) & 15) == 0 && ldc * (int64_t)size % 16 == 0 && ldc < ((int64_t)1 << 37);
     a.err = err;
+    a.limit_ns = limit_ns;
     return c.kind == MXF4 ? choose<MXF4>(c) : choose<MXF8F6F4>(c);
 }
 
@@ -924,4 +944,12 @@ extern "C" int ozk_mx_grouped_gemm(const uint8_t* A_codes, const uint8_t* A_scal
     if (!ends || (reinterpret_cast<uintptr_t>(ends) & 3) || groups < 1 || groups > OZK_MX_MAX_GROUPS) return OZK_ERR_ARG;
     return run(A_codes, A_scales, A_fmt, B_codes, B_scales, B_fmt, rows, n, k, groups, ends, fill, C, ldc, dtype, err,
                stream);
+}
+
+extern "C" int ozk_mx_wait_selftest(const uint8_t* A_codes, const uint8_t* A_scales, int A_fmt, const uint8_t* B_codes,
+                                    const uint8_t* B_scales, int B_fmt, int m, int n, int k, void* C, int64_t ldc, int dtype,
+                                    int64_t limit_ns, int hold, int32_t* err, ozk_stream_t stream) {
+    if (limit_ns < 100 || limit_ns > (int64_t)WAIT_LIMIT_NS) return OZK_ERR_ARG;
+    return run(A_codes, A_scales, A_fmt, B_codes, B_scales, B_fmt, m, n, k, 0, nullptr, 0, C, ldc, dtype, err, stream,
+               (uint64_t)limit_ns, hold != 0);
 }

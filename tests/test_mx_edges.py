@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import mx_reference as R
-from test_mx import FMTS, _f64, _norm_want, _put, _same
+from test_mx import FMTS, _exact_operand, _f64, _norm_want, _put, _same
 
 
 def _near(q, y, fmt):
@@ -212,3 +212,79 @@ def test_norm_refuses_what_would_lose_a_gradient(pkg):
             with pytest.raises(ValueError, match="tangent"):
                 pkg.mx_rms_norm(args[0], args[1], residual=args[2])
         assert torch.equal(pkg.mx_rms_norm(x, w, residual=r)[1], t)
+
+
+# ---- waits that run out --------------------------------------------------------------------------------------------------
+def test_wait_selftest_refusals(pkg):
+    L = pkg._lib.lib()
+    p = 4096                                                     # an aligned address that nothing reads
+    good = [p, p, 0, p, p, 1, 4, 8, 64, p, 8, 2, 10 ** 6, 0, p, None]
+    for at, v in [(0, None), (3, p + 16), (6, 0), (10, 7), (11, 3), (12, 99), (12, 4 * 10 ** 9 + 1), (14, None)]:
+        a = list(good)
+        a[at] = v
+        assert L.ozk_mx_wait_selftest(*a) == -1, (at, v)
+
+
+def _selftest(pkg, A, B, limit_ns, hold):
+    """(C, error flags, milliseconds on the device) of a product whose waits end after limit_ns."""
+    import torch
+    err = torch.zeros(1, dtype=torch.int32, device="cuda")
+    C = torch.full((A.rows, B.rows), float("nan"), device="cuda")
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    a.record()
+    pkg._lib.check(pkg._lib.lib().ozk_mx_wait_selftest(
+        A._code_ptr, A._scale_ptr, A._fmt, B._code_ptr, B._scale_ptr, B._fmt, A.rows, B.rows, A.k, C.data_ptr(), B.rows, 0,
+        limit_ns, hold, err.data_ptr(), torch.cuda.current_stream().cuda_stream), "ozk_mx_wait_selftest")
+    b.record()
+    torch.cuda.synchronize()
+    return C, int(err.item()), a.elapsed_time(b)
+
+
+# rows, columns, k, formats, loads of the CTA with the most: one shape for each tile
+TILES = [(20, 300, 1024, "e4m3", "e2m1", 2), (50, 300, 1024, "e2m1", "e4m3", 2), (100, 300, 100, "e2m1", "e2m1", 1),
+         (100, 384 * 148 + 8, 128, "e4m3", "e4m3", 2), (1700, 1700, 100, "e2m1", "e2m1", 1), (1700, 1700, 100, "e4m3", "e2m1", 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,a,b,loads", TILES)
+def test_timeout_waits_for_the_loads_in_flight(pkg, m, n, k, a, b, loads):
+    """No stage is ever full, so the issuing warp and the epilogue give up after 20 ms, when the producer has long issued its
+    last load and left.  The kernel must not end before it has waited for those loads, which shows in its time: their
+    barriers, of which more is expected than comes, take the limit of 1 s each."""
+    rng = np.random.default_rng(51)
+    (A, av), (B, bv) = _exact_operand(pkg, rng, a, m, k), _exact_operand(pkg, rng, b, n, k)
+    _, err, ms = _selftest(pkg, A, B, 20_000_000, 1)
+    assert err in (2, 4, 6)                                      # the issuing warp's flag, the epilogue's, or both
+    assert 1000 * loads < ms < 1000 * loads + 900
+    C, err, _ = _selftest(pkg, A, B, 4 * 10 ** 9, 0)             # and the device is as it was
+    assert err == 0
+    np.testing.assert_array_equal(C[:64].double().cpu().numpy(), av[:64] @ bv.T)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k,a,b", [(20, 200, 2 ** 25, "e2m1", "e2m1"), (50, 200, 2 ** 24, "e4m3", "e2m1"),
+                                       (300, 300, 2 ** 22, "e2m1", "e4m3"), (100, 384 * 148 + 8, 2 ** 15, "e4m3", "e2m1"),
+                                       (1700, 1700, 2 ** 22, "e2m1", "e2m1"), (1700, 1700, 2 ** 20, "e4m3", "e4m3")])
+def test_timeout_in_the_middle(pkg, m, n, k, a, b):
+    """Limits that end the waits of an ordinary long product wherever they happen to be, its loads and MMAs in flight: flags,
+    or the right product; and the right product from the call that follows, whose CTAs take over the same shared memory and
+    TMEM.  (A wait looks at the clock after some hundred polls, so how many end is up to the device.)"""
+    import torch
+    torch.manual_seed(52)
+
+    def operand(rows, fmt):
+        codes = torch.randint(0, 256 if fmt == "e2m1" else 120, (rows, k // (2 if fmt == "e2m1" else 1)), dtype=torch.uint8, device="cuda")
+        return pkg.MXMatrix.from_codes(codes, torch.full((rows, k // 32), 120, dtype=torch.uint8, device="cuda"), fmt)
+
+    A, B = operand(m, a), operand(n, b)
+    want = pkg.mx_matmul(A, B, dtype=torch.float32)
+    flags = []
+    for limit in (100, 10_000, 100_000, 300_000, 4 * 10 ** 9):
+        for _ in range(3):
+            C, err, _ = _selftest(pkg, A, B, limit, 0)
+            assert 0 <= err < 8 and (err or torch.equal(C, want))
+            flags.append(err)
+            assert torch.equal(pkg.mx_matmul(A, B, dtype=torch.float32), want)
+    assert flags[-3:] == [0, 0, 0]                               # the last limit is the ordinary one
+    pkg.mx_check_errors()
+    assert any(flags) or n > 50000                               # whose tiles are too short for it
