@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import mx_reference as R
-from test_mx import FMTS, _exact_operand, _f64, _norm_want, _put, _same
+from test_mx import FMTS, PAIRS, _exact_operand, _f64, _norm_want, _put, _same
 
 
 def _near(q, y, fmt):
@@ -288,3 +288,68 @@ def test_timeout_in_the_middle(pkg, m, n, k, a, b):
     assert flags[-3:] == [0, 0, 0]                               # the last limit is the ordinary one
     pkg.mx_check_errors()
     assert any(flags) or n > 50000                               # whose tiles are too short for it
+
+
+# ---- every tile of the products, over sizes where its rings and accumulators wrap ----------------------------------------
+def _exact_on_device(pkg, fmt, rows, k, groups=None):
+    """As test_mx._exact_operand, made on the device: the operand and its numbers in FP32 (multiples of 1/4 up to 12)."""
+    import torch
+    shape = (rows, k) if groups is None else (groups, rows, k)
+    table = torch.tensor([0.0, 0.5, 1.0, 1.5, 2.0, 3.0, 4.0, 6.0], device="cuda")
+    c = torch.randint(0, 16, shape, dtype=torch.uint8, device="cuda")
+    v = table[(c & 7).int()] * torch.where(c > 7, -1.0, 1.0)
+    scales = torch.randint(126, 129, (*shape[:-1], -(-k // 32)), dtype=torch.uint8, device="cuda")
+    v *= torch.exp2(scales.float() - 127).repeat_interleave(32, -1)[..., :k]
+    if fmt == "e4m3":
+        of = torch.tensor([0, 0x30, 0x38, 0x3c, 0x40, 0x44, 0x48, 0x4c], dtype=torch.uint8, device="cuda")
+        codes = of[(c & 7).int()] | (c >> 3 << 7)
+    else:
+        c = torch.nn.functional.pad(c, (0, k % 2))
+        codes = c[..., 0::2] | (c[..., 1::2] << 4)
+    return pkg.MXMatrix.from_codes(codes.contiguous(), scales, fmt, k), v
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("a,b", PAIRS)
+@pytest.mark.parametrize("k", [32, 1100])
+def test_product_of_some_rows_and_many_columns(pkg, a, b, k):
+    """33 to 128 rows and columns enough for the 128 x 256 tile, two of which a CTA takes in turn, bit for bit."""
+    import torch
+    torch.manual_seed(61)
+    n = 384 * torch.cuda.get_device_properties(0).multi_processor_count + 8
+    B, bv = _exact_on_device(pkg, b, n, k)
+    for m in (33, 128):
+        A, av = _exact_on_device(pkg, a, m, k)
+        want = av.double() @ bv.double().T
+        for dt in (torch.float32, torch.bfloat16):
+            assert torch.equal(pkg.mx_matmul(A, B, dtype=dt), want.to(dt)), (m, dt)
+    pkg.mx_check_errors()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("a,b", PAIRS)
+@pytest.mark.parametrize("k", [1100, 4096])
+@pytest.mark.parametrize("rows,experts", [(1500, 32), (4000, 12)])
+def test_grouped_of_long_rows(pkg, rows, experts, k, a, b):
+    """Groups of fewer and of more rows than the rule's border (64 on average), long K and several tiles a CTA, with empty
+    groups, groups that start and end inside a tile, and rows behind the last: bit for bit in FP32, and in bf16 with rows
+    that leave as boxes."""
+    import torch
+    torch.manual_seed(62)
+    rng = np.random.default_rng(63)
+    ends = np.sort(rng.integers(0, rows - 6, size=experts))
+    ends[3], ends[4], ends[experts // 2] = ends[5], ends[5], ends[experts // 2 + 1]
+    ends = ends.tolist()
+    e = torch.tensor(ends, dtype=torch.int32, device="cuda")
+    for n, dt in ((2100, torch.float32), (2104, torch.bfloat16)):
+        A, av = _exact_on_device(pkg, a, rows, k)
+        B, bv = _exact_on_device(pkg, b, n, k, experts)
+        want = torch.zeros(rows, n, dtype=torch.float64, device="cuda")
+        for g, (first, last) in enumerate(zip([0] + ends, ends)):
+            want[first:last] = av[first:last].double() @ bv[g].double().T
+        assert torch.equal(pkg.mx_grouped_matmul(A, B, e, dtype=dt), want.to(dt))
+        given = torch.full((rows, n + 8), 5.0, dtype=dt, device="cuda")
+        pkg.mx_grouped_matmul(A, B, e, C=given[:, :n])
+        assert torch.equal(given[:ends[-1], :n], want[:ends[-1]].to(dt))
+        assert (given[ends[-1]:] == 5.0).all() and (given[:, n:] == 5.0).all()
+    pkg.mx_check_errors()
