@@ -214,12 +214,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int tiles_m = (m + BM - 1) / BM, tiles_n = (n + BN - 1) / BN;
     const int tiles = tiles_m * tiles_n;
     const int kblocks = (2 * cp.k + BKB - 1) / BKB;
+    long long issued = 0;                              // loads, by the producer
 
     if (warp == 0) {
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0;
-            long long issued = 0;
             bool ok = true;
             for (int u = blockIdx.x; ok && u < tiles; u += gridDim.x) {
                 int tm, tn;
@@ -237,19 +237,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
-            if (!ok) {
-                const long long first = issued > STAGES ? issued - STAGES : 0;
-                for (long long j = first; j < issued; j++) {
-                    int dummy = 0;
-                    mbar_wait_bounded(full_bar((int)(j % STAGES)), (uint32_t)((j / STAGES) & 1), &dummy, WAIT_LIMIT_NS);
-                }
-            }
         }
     } else if (warp == 1) {
         if (lane == 0) {
             int stage = 0;
             uint32_t phase = 0, acc_it = 0;
-            bool ok = true, issued_any = false;
+            bool ok = true;
             for (int u = blockIdx.x; ok && u < tiles; u += gridDim.x) {
                 const int b = (int)(acc_it & 1u);
                 const uint32_t aph = (acc_it >> 1) & 1u;
@@ -273,18 +266,12 @@ __global__ void __launch_bounds__(THREADS, 1)
                     for (int kk = 0; kk < BKB / 32; kk++)   // K = 16 fp16 = 32 bytes per instruction
                         umma_f16(d_tmem, adesc + (uint64_t)(2 * kk), bdesc + (uint64_t)(2 * kk), IDESC,
                                  (kb > 0 || kk > 0) ? 1u : 0u);
-                    issued_any = true;
                     umma_commit(empty_bar(stage));
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
                 if (!ok) break;
                 umma_commit(accf_bar(b));
                 acc_it++;
-            }
-            if (!ok && issued_any) {
-                umma_commit(drain_bar);
-                int dummy = 0;
-                mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
             }
         }
     } else {
@@ -404,6 +391,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (__builtin_expect(*abort_flag, 0)) {
+        // all roles have left, by a wait that ran out or at their end: what they issued lands before TMEM is freed
+        if (warp == 0 && lane == 0) {
+            drain_loads<STAGES>(issued, issued, STAGE_BYTES, full_bar, WAIT_LIMIT_NS);
+        } else if (warp == 1 && lane == 0) {
+            umma_commit(drain_bar);
+            int none = 0;
+            mbar_wait_bounded(drain_bar, 0u, &none, WAIT_LIMIT_NS);
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    }
     if (warp == 1) {
         __syncwarp();
         tmem_dealloc(tmem_base, TMEM_COLS);

@@ -148,13 +148,13 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int units = N * tiles;
     const int kblocks = (k + BK - 1) / BK;
     const int nseg = (kblocks + SEG_KB - 1) / SEG_KB;
+    long long issued = 0;                              // loads, by the producer
 
     if (warp == 0) {
         if (lane == 0) {
             // ------------------------------------------------------------ TMA producer
             int stage = 0;
             uint32_t phase = 0;
-            long long issued = 0;
             bool ok = true;
             for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
                 int t, tm, tn;
@@ -172,23 +172,13 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                 }
             }
-            if (!ok) {
-                // let the loads already issued land before the CTA exits (bounded)
-                const long long first = issued > STAGES ? issued - STAGES : 0;
-                for (long long j = first; j < issued; j++) {
-                    const int s = (int)(j % STAGES);
-                    const uint32_t par = (uint32_t)((j / STAGES) & 1);
-                    int dummy = 0;
-                    mbar_wait_bounded(full_bar(s), par, &dummy, WAIT_LIMIT_NS);
-                }
-            }
         }
     } else if (warp == 1) {
         if (lane == 0) {
             // ------------------------------------------------------------ MMA issuer
             int stage = 0;
             uint32_t phase = 0, acc_it = 0;
-            bool ok = true, issued_any = false;
+            bool ok = true;
             for (int u = blockIdx.x; ok && u < units; u += gridDim.x) {
                 for (int seg = 0; ok && seg < nseg; seg++) {
                     const int b = (int)(acc_it & 1u);
@@ -216,7 +206,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                             umma_i8(d_tmem, adesc + (uint64_t)(2 * kk), bdesc + (uint64_t)(2 * kk), IDESC,
                                     (kb > kb0 || kk > 0) ? 1u : 0u);
                         }
-                        issued_any = true;
                         umma_commit(empty_bar(stage));
                         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
                     }
@@ -224,12 +213,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                     umma_commit(accf_bar(b));
                     acc_it++;
                 }
-            }
-            if (!ok && issued_any) {
-                // all MMAs issued by this thread must finish before TMEM is released
-                umma_commit(drain_bar);
-                int dummy = 0;
-                mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
             }
         }
     } else {
@@ -273,6 +256,19 @@ __global__ void __launch_bounds__(THREADS, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    if (__builtin_expect(*abort_flag, 0)) {
+        // all roles have left, by a wait that ran out or at their end: what they issued lands before TMEM is freed
+        if (warp == 0 && lane == 0) {
+            drain_loads<STAGES>(issued, issued, STAGE_BYTES, full_bar, WAIT_LIMIT_NS);
+        } else if (warp == 1 && lane == 0) {
+            umma_commit(drain_bar);
+            int none = 0;
+            mbar_wait_bounded(drain_bar, 0u, &none, WAIT_LIMIT_NS);
+        }
+        tc_fence_before();
+        __syncthreads();
+        tc_fence_after();
+    }
     if (warp == 1) {
         __syncwarp();
         tmem_dealloc(tmem_base, TMEM_COLS);
@@ -328,6 +324,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES2 * STAGE2_BYTES);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + NUM_BARS2);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    volatile long long* peer_issued = reinterpret_cast<volatile long long*>(tmem_slot + 2);   // loads that CTA 1 issued
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = cluster_ctarank();           // 0: issues the MMAs; 1: its peer
@@ -343,6 +340,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         for (int b = 0; b < 2; b++) { mbar_init(accf_bar(b), 1); mbar_init(acce_bar(b), 2 * EPI_WARPS); }
         mbar_init(drain_bar, 1);
         *abort_flag = 0;
+        *peer_issued = 0;
         mbar_fence_init();
         tma_prefetch_desc(&tmA);
         tma_prefetch_desc(&tmB);
@@ -363,20 +361,25 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int kblocks = (k + BK - 1) / BK;
     const int nseg = (kblocks + SEG_KB - 1) / SEG_KB;
     const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
+    long long issued = 0;                              // loads, by this CTA's producer
+    auto give_up = [&](int code) {                     // a role whose wait ran out; both CTAs' roles leave through their flags
+        if (*abort_flag) return;
+        raise_abort(abort_flag, err, code);
+        st_cluster_u32(map_to_rank(smem_addr(const_cast<const int*>(abort_flag)), rank ^ 1u), 1u);
+    };
 
     if (warp == 0) {
         if (lane == 0) {
             // ------------------------------------------------------------ TMA producer (both CTAs)
             int stage = 0;
             uint32_t phase = 0;
-            long long issued = 0;
             bool ok = true;
             for (int u = pair; ok && u < units; u += npairs) {
                 int t, tm, tn;
                 decode_unit2(u, tiles, tiles_m, tiles_n, t, tm, tn);
                 for (int kb = 0; kb < kblocks; kb++) {
                     if (!mbar_wait_bounded(empty_bar(stage), phase ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
-                        if (!*abort_flag) raise_abort(abort_flag, err, OZK_DEVERR_TIMEOUT_PRODUCER);
+                        give_up(OZK_DEVERR_TIMEOUT_PRODUCER);
                         ok = false;
                         break;
                     }
@@ -390,29 +393,20 @@ __global__ void __launch_bounds__(THREADS, 1)
                     if (++stage == STAGES2) { stage = 0; phase ^= 1u; }
                 }
             }
-            if (!ok && rank == 0) {
-                // let the loads already armed land before the pair exits (bounded)
-                const long long first = issued > STAGES2 ? issued - STAGES2 : 0;
-                for (long long j = first; j < issued; j++) {
-                    const int s = (int)(j % STAGES2);
-                    const uint32_t par = (uint32_t)((j / STAGES2) & 1);
-                    int dummy = 0;
-                    mbar_wait_bounded(full_bar(s), par, &dummy, WAIT_LIMIT_NS);
-                }
-            }
+            if (rank == 1) st_cluster_u64(map_to_rank(smem_addr(const_cast<const long long*>(peer_issued)), 0u), (uint64_t)issued);
         }
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             // ------------------------------------------------------------ MMA issuer (CTA 0 of the pair)
             int stage = 0;
             uint32_t phase = 0, acc_it = 0;
-            bool ok = true, issued_any = false;
+            bool ok = true;
             for (int u = pair; ok && u < units; u += npairs) {
                 for (int seg = 0; ok && seg < nseg; seg++) {
                     const int b = (int)(acc_it & 1u);
                     const uint32_t aph = (acc_it >> 1) & 1u;
                     if (!mbar_wait_bounded(acce_bar(b), aph ^ 1u, abort_flag, WAIT_LIMIT_NS)) {
-                        if (!*abort_flag) raise_abort(abort_flag, err, OZK_DEVERR_TIMEOUT_MMA);
+                        give_up(OZK_DEVERR_TIMEOUT_MMA);
                         ok = false;
                         break;
                     }
@@ -421,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                     const int kb0 = seg * SEG_KB, kb1 = min(kblocks, kb0 + SEG_KB);
                     for (int kb = kb0; kb < kb1; kb++) {
                         if (!mbar_wait_bounded(full_bar(stage), phase, abort_flag, WAIT_LIMIT_NS)) {
-                            if (!*abort_flag) raise_abort(abort_flag, err, OZK_DEVERR_TIMEOUT_MMA);
+                            give_up(OZK_DEVERR_TIMEOUT_MMA);
                             ok = false;
                             break;
                         }
@@ -432,7 +426,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                         for (int kk = 0; kk < BK / 32; kk++)
                             umma_i8_pair(d_tmem, adesc + (uint64_t)(2 * kk), bdesc + (uint64_t)(2 * kk), IDESC2,
                                          (kb > kb0 || kk > 0) ? 1u : 0u);
-                        issued_any = true;
                         umma_commit_pair(empty_bar(stage));
                         umma_commit_pair(map_to_rank(empty_bar(stage), 1u));
                         if (++stage == STAGES2) { stage = 0; phase ^= 1u; }
@@ -442,12 +435,6 @@ __global__ void __launch_bounds__(THREADS, 1)
                     umma_commit_pair(map_to_rank(accf_bar(b), 1u));
                     acc_it++;
                 }
-            }
-            if (!ok && issued_any) {
-                // every MMA issued by this thread finishes before the pair's TMEM is released
-                umma_commit_pair(drain_bar);
-                int dummy = 0;
-                mbar_wait_bounded(drain_bar, 0u, &dummy, WAIT_LIMIT_NS);
             }
         }
     } else {
@@ -465,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1)
                 const int b = (int)(acc_it & 1u);
                 const uint32_t aph = (acc_it >> 1) & 1u;
                 bool w = mbar_wait_bounded(accf_bar(b), aph, abort_flag, WAIT_LIMIT_NS);
-                if (!w && !*abort_flag) raise_abort(abort_flag, err, OZK_DEVERR_TIMEOUT_EPILOGUE);
+                if (!w) give_up(OZK_DEVERR_TIMEOUT_EPILOGUE);
                 if (!__all_sync(0xffffffffu, w)) { ok = false; break; }
                 tc_fence_after();
 #pragma unroll 1
@@ -489,6 +476,23 @@ __global__ void __launch_bounds__(THREADS, 1)
     __syncthreads();
     cluster_sync();                                    // neither CTA leaves while its peer may still reach it
     tc_fence_after();
+    if (__builtin_expect(*abort_flag, 0)) {            // in both CTAs or in none
+        // all roles have left, by a wait that ran out or at their end: what they issued lands before the pair's TMEM is freed
+        if (warp == 0 && lane == 0 && rank == 0) {
+            drain_loads<STAGES2>(issued, *peer_issued, STAGE2_BYTES, full_bar, WAIT_LIMIT_NS);
+        } else if (warp == 1 && lane == 0) {
+            if (rank == 0) {
+                umma_commit_pair(drain_bar);
+                umma_commit_pair(map_to_rank(drain_bar, 1u));
+            }
+            int none = 0;
+            mbar_wait_bounded(drain_bar, 0u, &none, WAIT_LIMIT_NS);
+        }
+        tc_fence_before();
+        __syncthreads();
+        cluster_sync();
+        tc_fence_after();
+    }
     if (warp == 1) {
         __syncwarp();
         tmem_dealloc_pair(tmem_base, TMEM_COLS);

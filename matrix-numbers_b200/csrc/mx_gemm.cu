@@ -667,24 +667,12 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (__builtin_expect(*abort_flag, 0)) {
         // All roles of the CTA (of the pair) have left, by a wait that ran out or at their end.  What they issued still writes
         // shared memory, TMEM and barriers, so it has to land before those are given up.
-        int none = 0;
         if (warp == 0 && rank == 0) {
-            // The last loads of the ring, on CTA 0's barriers.  Those that only CTA 1 of a pair issued are expected now, those
-            // that were expected of it and never issued count as arrived: neither is more than a ring ahead of the MMAs,
-            // so a slot's earlier loads have been waited for.
-            const long long other = PAIR ? *peer_issued : issued, most = issued > other ? issued : other;
-            for (long long j = most > STAGES ? most - STAGES : 0; j < most; j++) {
-                const uint32_t bar = full_bar((int)(j % STAGES));
-                if (PAIR && lane == 0) {
-                    if (j >= issued) mbar_arrive_expect_tx(bar, a.load_bytes);
-                    else if (j >= other) mbar_complete_tx(bar, a.load_bytes);
-                }
-                __syncwarp();
-                mbar_wait_bounded(bar, (uint32_t)((j / STAGES) & 1), &none, DRAIN_LIMIT_NS);
-            }
+            if (lane == 0) drain_loads<STAGES>(issued, PAIR ? *peer_issued : issued, a.load_bytes, full_bar, DRAIN_LIMIT_NS);
         } else if (warp == 1) {
             if (rank == 0 && elect_one()) commit(drain_bar);
             __syncwarp();
+            int none = 0;
             mbar_wait_bounded(drain_bar, 0u, &none, DRAIN_LIMIT_NS);
         }
         __syncwarp();

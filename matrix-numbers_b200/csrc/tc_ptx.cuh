@@ -276,6 +276,22 @@ __device__ __forceinline__ void st_cluster_u32(uint32_t addr, uint32_t v) {
 __device__ __forceinline__ void st_cluster_u64(uint32_t addr, uint64_t v) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(addr), "l"(v) : "memory");
 }
+// After a timeout, when every role of the CTA (of a pair: of both CTAs) has left: one thread waits (up to limit_ns each) for the
+// last loads of the ring, which still write shared memory and the full barriers (of a pair: CTA 0's, by CTA 0).  `mine` and
+// `other`: loads issued by this CTA and by the pair's other one (the same where there is none), of `bytes` each on the
+// barriers.  Loads that only the other CTA issued are expected now, and those that were expected of it and never issued
+// count as arrived: neither CTA is more than a ring ahead of the MMAs, so a slot's earlier loads have been waited for.
+template <int STAGES, typename Full>
+__device__ __forceinline__ void drain_loads(long long mine, long long other, uint32_t bytes, Full full_bar, uint64_t limit_ns) {
+    const long long most = mine > other ? mine : other;
+    for (long long j = most > STAGES ? most - STAGES : 0; j < most; j++) {
+        const uint32_t bar = full_bar((int)(j % STAGES));
+        if (j >= mine) mbar_arrive_expect_tx(bar, bytes);
+        else if (j >= other) mbar_complete_tx(bar, bytes);
+        int none = 0;
+        mbar_wait_bounded(bar, (uint32_t)((j / STAGES) & 1), &none, limit_ns);
+    }
+}
 // four 32-bit words of the shared memory of a CTA of the cluster (address from map_to_rank, 16-byte aligned)
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
     float4 v;
