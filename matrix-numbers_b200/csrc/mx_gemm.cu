@@ -25,9 +25,9 @@
 // most one more tile per group than packing would need.
 // The producer and the issuing warp run their loops as whole warps and let one elected lane issue: with the loops in one
 // lane alone each operand of a tcgen05 instruction was moved to a uniform register on its way, and the issue bound the
-// kernel (8192 x 4096 x 8192 in e2m1: 163 us, tensor pipe 41 % active; elected: 99 us, 75 %).
-// Measured on one B200 at its power cap (1.4 - 1.5 GHz): e2m1 16384 x 8192 x 8192 in 394 us, 5.6 PFLOP/s; e4m3 8192 x 8192 x
-// 8192 in 396 us, 2.8 PFLOP/s: four and two times the rate that the card sustains in bf16, and bound by the same cap.
+// kernel (8192 x 4096 x 8192 in e2m1: 163 us, tensor pipe 41 % active; elected: 102 us, 70 %).
+// Measured on one B200 at its power cap (1.4 - 1.5 GHz): e2m1 16384 x 8192 x 8192 in 392 us, 5.6 PFLOP/s; e4m3 8192 x 8192 x
+// 8192 in 394 - 414 us, 2.7 - 2.8 PFLOP/s: four and two times the rate that the card sustains in bf16, and bound by the same cap.
 // Every mbarrier wait is bounded; when a role's wait runs out it records a flag in *err and raises the CTA's abort flag (both
 // CTAs' of a pair), through which the other roles leave.  When all have, whichever it was, the CTA waits (bounded) for its
 // loads and MMAs in flight, frees TMEM and exits.  No multicast is used.
@@ -862,7 +862,10 @@ int parts_for(long long units, int kblocks, int sms, int least) {
 // Grouped, 16 experts of 4096 x 2048 in e2m1, A in e4m3 (in brackets e2m1), by the rows of an average group:
 //   8: 128 x 256 22.6 (15.6), pair 31.8 (23.9); 32: 30.0 (19.3), 32.3 (23.7); 64: 35.8 (21.6), 33.6 (23.7);
 //   100: 46.0 (26.8), 35.3 (24.4); 256: 73.1 (44.6), 53.6 (37.8); 1024: 181 (107), 138 (90).
-// (The 4-bit kind stays with 128 x 128 a little longer; the difference is at most 6 % and has no rule of its own.)
+// (The 4-bit kind does better with the smaller tile for a little longer: by 6 % at m = 512, by 9 % at groups of 64 rows.  It
+// has no rule of its own.)  For 65 to 128 rows and n from 128 to 384 times the SMs the pair runs with its second 128
+// rows empty; only n = 65536, where 128 x 256 won, was measured.
+// Rows of C off 16-byte boundaries leave value by value: 4096 x 50257 x 1024 in e4m3 takes 1995 us, 4096 x 50256 x 1024 221.
 template <int KIND>
 int choose(const Call& c) {
     const int kblocks = (padded_k(c.k) / TILE + (KIND == MXF4 ? 1 : 0)) / (KIND == MXF4 ? 2 : 1);

@@ -137,8 +137,11 @@ struct Kept8 {
 // the next row's loads under way while a row is summed and encoded, and the weights in registers.  Rows need not start on
 // 16 bytes (`SHIFTED`), as long as those of x, residual and sum do so alike: everything up to the sum of squares and the
 // new residual happens in units of memory, and only then do the values move by `lead` places to where their blocks of 32
-// begin.  bf16 16384 x 8192 with the residual to e4m3: 149 - 168 us, 5.6 - 6.3 TB/s (264 us with a CTA a row); bf16 8192 x 4097: 76 us (153).
-// CTAs an SM: 1024 threads with 64 registers, 768 with 85 for three units a thread
+// begin.  bf16 16384 x 8192 with the residual to e4m3: 148 us, 6.3 TB/s (264 us with a CTA a row); to e2m1 145; bf16 8192 x
+// 4097: 80 us (153).
+// CTAs an SM: 1024 threads with 64 registers, 768 with 85 for three units a thread.  FP32 rows, and FP32 weights of 16-bit
+// rows, do not fit there with two units or more a thread and spill (16-bit rows up to 160 bytes, FP32 up to 760): FP32 8192 x
+// 8192 with the residual 144 - 154 us, 5.7 - 6.1 TB/s; 8192 x 5120, three units, 111 us, 4.9 TB/s.
 constexpr int stream_blocks(int tpr, int nc) { return (nc > 2 ? 768 : 1024) / tpr; }
 
 template <typename T, typename W, int FMT, int TPR, int NC, bool SHIFTED>

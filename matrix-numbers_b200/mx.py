@@ -14,7 +14,8 @@ and one scale byte s per block of 32 along the contracted axis (255: the block h
 everything it touches is NaN).  Any sizes; the operands are laid out for the tensor cores once, by the quantisation.
 
 All calls are enqueued on the current stream of the operand's device and may be captured in a CUDA graph (after one
-eager product on that device).  A product whose bounded waits ran out leaves a flag that ``mx_check_errors`` raises.
+eager product on that device).  They call the library on the tensors' memory, which ``torch.compile`` cannot trace: it
+breaks its graph at each of them.  A product whose bounded waits ran out leaves a flag that ``mx_check_errors`` raises.
 Only ``mx_linear`` has gradients: ``mx_rms_norm`` refuses inputs that require one (under ``torch.no_grad()`` it takes
 them), and an ``MXMatrix`` is not a tensor and carries none.
 """
@@ -555,8 +556,8 @@ def mx_linear(x, weight, fmt="e4m3", rule="floor"):
 
     Every operand is quantised along the axis its product contracts: y from x and weight along k, dx = dy weight from
     both along n, dweight = dy^T x from both along the rows of x.  The roundings themselves are passed over in the
-    backward pass (their derivative is taken as one).  A second derivative and forward-mode differentiation are refused.  A captured backward pass needs
-    what torch needs of any: no eager graph of the same leaves alive on another stream."""
+    backward pass (their derivative is taken as one).  A second derivative and forward-mode differentiation are refused.
+    A captured backward pass needs what torch needs of any: no eager graph of the same leaves alive on another stream."""
     _tensor(x, "x")
     _tensor(weight, "weight")
     code, up = _format(fmt), _rule(rule)
